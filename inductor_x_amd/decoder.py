@@ -1,0 +1,85 @@
+"""Decoder-layer operators as graph ops.
+
+The entry points of kernels.py (residual norm with an 8-bit result, rotary positions over several axes, attention with a
+sliding window and visible first tokens) registered in the package's operator library npu_graph with shape
+functions and gradients, so that torch.compile keeps them in its graph and autograd passes through them.  The functions
+of this module are what a model calls.
+"""
+from __future__ import annotations
+
+from typing import Optional, Sequence
+
+import torch
+from torch.library import register_autograd
+
+from . import kernels
+from .fusion_attention_graph import gpu_lib, meta_lib, npu_def
+
+npu_def.define("add_rmsnorm_quant(Tensor h, Tensor r, Tensor w, float eps=1e-6, int group=0) -> (Tensor, Tensor, Tensor)")
+npu_def.define(
+    "rotary_axes(Tensor q, Tensor k, Tensor positions, Tensor inv_freq, int[]? sections=None, bool interleaved=False, "
+    "bool inverse=False) -> (Tensor, Tensor)"
+)
+npu_def.define(
+    "window_attention_decode(Tensor q, Tensor k_cache, Tensor v_cache, Tensor lengths, float scale, int window, "
+    "int sinks=0) -> Tensor"
+)
+
+gpu_lib.impl("add_rmsnorm_quant", kernels.add_rmsnorm_quant)
+gpu_lib.impl("rotary_axes", kernels.rotary_axes)
+gpu_lib.impl("window_attention_decode", kernels.window_attention_decode)
+
+
+def _add_rmsnorm_quant_meta(h, r, w, eps=1e-6, group=0):
+    groups = (h.shape[-1] + 127) // 128 if group else 1
+    return (torch.empty(h.shape, dtype=torch.float8_e4m3fn, device=h.device),
+            torch.empty(tuple(h.shape[:-1]) + (groups,), dtype=torch.float32, device=h.device),
+            torch.empty(h.shape, dtype=h.dtype, device=h.device))
+
+
+def _rotary_axes_meta(q, k, positions, inv_freq, sections=None, interleaved=False, inverse=False):
+    return torch.empty_like(q), torch.empty_like(k)
+
+
+def _window_attention_decode_meta(q, k_cache, v_cache, lengths, scale, window, sinks=0):
+    return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+
+
+meta_lib.impl("add_rmsnorm_quant", _add_rmsnorm_quant_meta)
+meta_lib.impl("rotary_axes", _rotary_axes_meta)
+meta_lib.impl("window_attention_decode", _window_attention_decode_meta)
+
+
+def _rotary_context(ctx, inputs, output):
+    _, _, positions, inv_freq, sections, interleaved, inverse = inputs
+    ctx.save_for_backward(positions, inv_freq)
+    ctx.form = (sections, interleaved, inverse)
+
+
+def _rotary_backward(ctx, dq, dk):
+    positions, inv_freq = ctx.saved_tensors
+    sections, interleaved, inverse = ctx.form
+    # a rotation's gradient is the rotation back
+    last = lambda t: t if t.stride(-1) == 1 else t.contiguous()  # noqa: E731
+    gq, gk = torch.ops.npu_graph.rotary_axes(last(dq), last(dk), positions, inv_freq, sections, interleaved, not inverse)
+    return gq, gk, None, None, None, None, None
+
+
+register_autograd("npu_graph::rotary_axes", _rotary_backward, setup_context=_rotary_context)
+
+
+def add_rmsnorm_quant(h: torch.Tensor, r: torch.Tensor, w: torch.Tensor, eps: float = 1e-6, group: int = 0):
+    """(q, scales, h + r): kernels.add_rmsnorm_quant as a graph op.  Serving only: an 8-bit result has no gradient."""
+    return torch.ops.npu_graph.add_rmsnorm_quant(h, r, w, eps, group)
+
+
+def rotary_axes(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
+                sections: Optional[Sequence[int]] = None, interleaved: bool = False, inverse: bool = False):
+    """kernels.rotary_axes as a graph op with gradients for q and k."""
+    return torch.ops.npu_graph.rotary_axes(q, k, positions, inv_freq, sections, interleaved, inverse)
+
+
+def window_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
+                            scale: float, window: int, sinks: int = 0) -> torch.Tensor:
+    """kernels.window_attention_decode as a graph op (inference)."""
+    return torch.ops.npu_graph.window_attention_decode(q, k_cache, v_cache, lengths, scale, window, sinks)

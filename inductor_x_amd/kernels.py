@@ -52,6 +52,12 @@ def _check_cuda(*tensors: torch.Tensor) -> None:
         _require(t.device == tensors[0].device, "tensors must share a device")
 
 
+def _check_here(*tensors: torch.Tensor) -> None:
+    """_check_cuda, and the tensors live on the current device, whose stream the launch goes to."""
+    _check_cuda(*tensors)
+    _require(tensors[0].device.index == torch.cuda.current_device(), "tensors must live on the current GPU")
+
+
 # ---------------------------------------------------------------------------
 # code objects (one per aot file), loaded lazily
 # ---------------------------------------------------------------------------
@@ -325,6 +331,70 @@ def add_rmsnorm(
         idx = l.pick(f"{rows}x{cols}", idx, fits, args, row_grid(rows), _stream())
     l._launch(idx, args, (cdiv(rows, l.launchers[idx][0].meta["PER_WG0"]), 1, 1), _stream())
     return out, s
+
+
+_NORM_QUANT_VARIANTS = [(256, 64, 1), (256, 64, 2), (256, 256, 1), (512, 512, 1), (512, 512, 2), (1024, 1024, 2), (1024, 1024, 4)]
+
+
+@functools.lru_cache(maxsize=None)
+def _norm_quant_launcher() -> CachingLauncher:
+    cfgs = [
+        LaunchConfig(f"add_rmsnorm_quant_{ty}_b{b}_t{t}_i{i}{g}{o}", b, meta={"DTYPE": ty, "TPR": t, "ITERS": i})
+        for ty in _ATTN_DTYPES.values() for b, t, i in _NORM_QUANT_VARIANTS for g in ("", "_g128") for o in ("", "_odd")
+    ]
+    return CachingLauncher(
+        "add_rmsnorm_quant", codecache.aot_source("norm_quant_kernels.hip"), "PPPPPPiiqqf", cfgs, prefer_intree=True
+    )
+
+
+def _as_rows(t: torch.Tensor, name: str) -> torch.Tensor:
+    """[rows, cols] view of a tensor whose rows are evenly spaced."""
+    try:
+        m = t if t.dim() == 2 else t.view(-1, t.shape[-1])
+    except RuntimeError:
+        raise ValueError(f"{name}: the leading axes must collapse into evenly spaced rows") from None
+    _require(m.shape[1] == 1 or m.stride(1) == 1, f"{name}: columns must be contiguous")
+    return m
+
+
+def add_rmsnorm_quant(
+    h: torch.Tensor, r: torch.Tensor, w: torch.Tensor, eps: float = 1e-6, group: int = 0
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """s = h + r and y = s * rsqrt(mean(s^2) + eps) * w as add_rmsnorm computes them, with y in 8 bits for a
+    product that takes such operands: returns (q, scales, s) with y ~ q.float() * scales.
+
+    q is float8_e4m3fn in the shape of h; scales (fp32) has one value per row (group = 0, shape [..., 1]) or per
+    128 columns (group = 128, shape [..., ceil(cols / 128)]): the largest |y| there divided by 448, 1 where
+    all are zero, never below the smallest normal number.  A NaN or infinity in a row gives that row (every
+    128 columns of it that it reaches) NaN, as the formula does.
+    h, r: bf16 or fp16 of one shape with contiguous columns and evenly spaced rows; w one vector of the same type."""
+    _check_here(h, r, w)
+    _require(h.dtype == r.dtype == w.dtype and h.dtype in _ATTN_DTYPES, "h, r, w must share bf16 or fp16")
+    _require(h.shape == r.shape and h.dim() >= 1, "h and r must have the same shape")
+    _require(group in (0, 128), "group must be 0 (one scale per row) or 128")
+    cols = h.shape[-1]
+    _require(w.shape == (cols,) and (cols <= 1 or w.stride(0) == 1), "w must be a contiguous vector of the row length")
+    _require(0 < cols <= 32768, "row length must lie in 1..32768")
+    groups = cdiv(cols, 128) if group else 1
+    s = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    q = torch.empty(h.shape, dtype=torch.float8_e4m3fn, device=h.device)
+    scales = torch.empty(h.shape[:-1] + (groups,), dtype=torch.float32, device=h.device)
+    rows = h.numel() // cols
+    if rows == 0:
+        return q, scales, s
+    _require(rows < 2**31, "too many rows")
+    hm, rm = _as_rows(h, "h"), _as_rows(r, "r")
+    hs, rs = hm.stride(0), rm.stride(0)
+    wide = (cols | hs | rs) % 8 == 0 and all(_aligned(t) for t in (h, r, w, s)) and _aligned(q, 8)
+    b, t, i = next(v for v in _NORM_QUANT_VARIANTS if cols <= v[1] * v[2] * 8)
+    l = _norm_quant_launcher()
+    idx = _find(l, f"add_rmsnorm_quant_{_ATTN_DTYPES[h.dtype]}_b{b}_t{t}_i{i}{'_g128' if group else ''}{'' if wide else '_odd'}")
+    l._launch(
+        idx, (h.data_ptr(), r.data_ptr(), w.data_ptr(), q.data_ptr(), scales.data_ptr(), s.data_ptr(), rows, cols, hs, rs,
+              float(eps)),
+        (cdiv(rows, b // t), 1, 1), _stream(),
+    )
+    return q, scales, s
 
 
 def _snap_split_plan(plan: SplitPlan, rows: int, cols: int) -> SplitPlan:
@@ -779,6 +849,178 @@ def fused_attention(
         _stream(),
     )
     return out, smax, ssum
+
+
+# ---------------------------------------------------------------------------
+# rotary positions over several axes
+# ---------------------------------------------------------------------------
+_ROTARY_DTYPES = {torch.bfloat16: "bf16", torch.float16: "f16", torch.float32: "f32"}
+_ROTARY_MAX_PAIRS = 1024  # angles a workgroup keeps
+
+
+@functools.lru_cache(maxsize=None)
+def _rotary_launcher() -> CachingLauncher:
+    cfgs = [
+        LaunchConfig(f"rotary_axes_{t}_{layout}{o}", 256, meta={"DTYPE": t})
+        for t in _ROTARY_DTYPES.values() for layout in ("half", "beside") for o in ("", "_odd")
+    ]
+    return CachingLauncher(
+        "rotary_axes", codecache.aot_source("rotary_kernels.hip"), "PPPPPP" + "q" * 12 + "i" * 12 + "f", cfgs,
+        prefer_intree=True,
+    )
+
+
+def rotary_axes(
+    q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, sections=None,
+    interleaved: bool = False, inverse: bool = False,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rotary positions over one to four axes (text; time, height and width): returns q and k with pair p of the first
+    2 * len(inv_freq) columns of every head turned by positions[axis(p)] * inv_freq[p], the other columns copied.
+
+    q [B, S, N, D] and k [B, S, Nk, D] (bf16, fp16 or fp32, any strides with contiguous columns).  positions: int32
+    or int64, [A, B, S] or, for one axis, [B, S].  inv_freq: fp32 or fp64, one frequency per pair.  sections: how many
+    consecutive pairs each axis turns (default: all on one axis).  A pair is (column p, column p + P) of P pairs, or
+    with interleaved=True (column 2 p, column 2 p + 1).  inverse turns back: the gradient of the rotation.
+    Angles are formed in 64 bits, the products in 32, rounded once."""
+    _check_here(q, k, positions, inv_freq)
+    _require(q.dtype == k.dtype and q.dtype in _ROTARY_DTYPES, "q and k must share bf16, fp16 or fp32")
+    _require(q.dim() == 4 and k.dim() == 4, "q [B, S, N, D] and k [B, S, Nk, D]")
+    B, S, N, D = q.shape
+    _require(k.shape[0] == B and k.shape[1] == S and k.shape[3] == D, "q and k must share batch, length and head dimension")
+    for x in (q, k):
+        _require(D <= 1 or x.stride(3) == 1, "columns of a head must be contiguous")
+    if positions.dim() == 2:
+        positions = positions.unsqueeze(0)
+    axes = positions.shape[0] if positions.dim() == 3 else 0
+    _require(positions.dim() == 3 and 1 <= axes <= 4 and tuple(positions.shape[1:]) == (B, S), "positions must be [A, B, S], A 1 to 4, or [B, S]")
+    _require(positions.dtype in (torch.int32, torch.int64) and positions.is_contiguous(), "positions must be contiguous int32 or int64")
+    _require(inv_freq.dim() == 1 and inv_freq.dtype in (torch.float32, torch.float64) and inv_freq.is_contiguous(),
+             "inv_freq must be a contiguous vector of fp32 or fp64")
+    pairs = inv_freq.numel()
+    _require(0 < pairs <= _ROTARY_MAX_PAIRS and 2 * pairs <= D, "inv_freq must have 1 to D / 2 (at most 1024) values")
+    sections = [pairs] if sections is None else [int(x) for x in sections]
+    _require(len(sections) == axes and min(sections) >= 0 and sum(sections) == pairs, "sections must give every axis its share of the pairs")
+    ends = [sum(sections[: i + 1]) for i in range(axes - 1)] + [pairs] * (4 - axes)
+    q_out, k_out = torch.empty_like(q), torch.empty_like(k)
+    if q.numel() + k.numel() == 0:
+        return q_out, k_out
+    tokens = B * S
+    _require(tokens < 2**31 and N + k.shape[2] < 2**16, "extents must fit int32 indexing")
+    vec = 16 // q.element_size()
+    strides = []
+    for x in (q, q_out, k, k_out):
+        _require(D <= 1 or x.stride(3) == 1, "columns of a head must be contiguous")
+        strides += [x.stride(0), x.stride(1), x.stride(2)]
+    step = vec if interleaved else 2 * vec
+    wide = (2 * pairs) % step == 0 and D % vec == 0 and all(x % vec == 0 for x in strides) and all(_aligned(x) for x in (q, q_out, k, k_out))
+    # tokens per workgroup: as many as give every thread an angle, fewer where that would leave compute units idle
+    per_block = max(1, min(256 // pairs, tokens // (2 * config.hardware().cu_count)))
+    l = _rotary_launcher()
+    i = _find(l, f"rotary_axes_{_ROTARY_DTYPES[q.dtype]}_{'beside' if interleaved else 'half'}{'' if wide else '_odd'}")
+    l._launch(
+        i,
+        (q.data_ptr(), q_out.data_ptr(), k.data_ptr(), k_out.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), *strides,
+         N, k.shape[2], positions.dtype == torch.int64, inv_freq.dtype == torch.float64, tokens, S, D, 2 * pairs,
+         ends[0], ends[1], ends[2], per_block, -1.0 if inverse else 1.0),
+        (cdiv(tokens, per_block), 1, 1), _stream(),
+    )
+    return q_out, k_out
+
+
+# ---------------------------------------------------------------------------
+# attention with a sliding window and first tokens that stay visible
+# ---------------------------------------------------------------------------
+_WINDOW_LIMIT = 2**30      # windows and lengths beyond mean "all"
+_STRIDE_LIMIT = 2**23      # elements between two tokens: byte offsets inside a tile fit 31 bits
+
+
+def _window_operands(q, k, v, scale, window, sinks, what="k and v"):
+    """Checks that the window attention entry points share; returns (DH, window, sinks)."""
+    _require(q.dtype == k.dtype == v.dtype and q.dtype in _ATTN_DTYPES, "q, k, v must share bf16 or fp16")
+    _require(k.dim() == 4 and k.shape == v.shape, f"{what} must share one [B, Nk, S, D] shape")
+    B, Nk, _, D = k.shape
+    _require(q.shape[0] == B and q.shape[-1] == D, "q, k, v must share batch and head dimension")
+    _require(Nk > 0 and q.shape[1] > 0 and q.shape[1] % Nk == 0, "query heads must be a multiple of the key heads")
+    _require(0 < D <= 128 and D % 8 == 0, "head dimension must be a multiple of 8 up to 128")
+    for t in (q, k, v):
+        _require(t.stride(-1) == 1 and _aligned(t) and all(s % 8 == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1),
+                 "columns must be contiguous, and rows 16-byte aligned")
+    _require(k.stride(2) < _STRIDE_LIMIT and v.stride(2) < _STRIDE_LIMIT, "tokens lie too far apart")
+    _require(scale > 0 and math.isfinite(scale), "scale must be positive and finite")
+    _require(window >= 1 and sinks >= 0, "window must be at least 1 and sinks at least 0")
+    return 64 if D <= 64 else 128, min(int(window), _WINDOW_LIMIT), min(int(sinks), _WINDOW_LIMIT)
+
+
+def _check_lengths(lengths, t):
+    _check_here(lengths, t)
+    _require(lengths.dtype == torch.int32 and lengths.shape == (t.shape[0],) and lengths.is_contiguous(),
+             "lengths must be a contiguous int32 vector with one value per sequence")
+
+
+@functools.lru_cache(maxsize=None)
+def _window_decode_launchers() -> tuple[CachingLauncher, CachingLauncher]:
+    src = codecache.aot_source("window_decode_kernels.hip")
+    shapes = [(t, d) for t in _ATTN_DTYPES.values() for d in (64, 128)]
+    # every wavefront: two buffers of a K and a V tile of 32 keys
+    main = CachingLauncher("window_decode", src, "PPPPPP" + "q" * 10 + "i" * 7 + "f",
+                           [LaunchConfig(f"window_decode_{t}_d{d}", 256, lds_bytes=4 * 4 * 32 * d * 2) for t, d in shapes], prefer_intree=True)
+    join = CachingLauncher("window_decode_join", src, "PPPiiiqq", [LaunchConfig(f"window_decode_join_{t}_d{d}", d) for t, d in shapes],
+                           prefer_intree=True)
+    return main, join
+
+
+def _decode_splits(units: int, tiles: int) -> int:
+    """Shares the visible keys of a sequence are cut into: enough workgroups for the chip, and at least two tiles of
+    32 keys for each of a workgroup's four wavefronts."""
+    return max(1, min(cdiv(2 * config.hardware().cu_count, units), tiles // 8, 64))
+
+
+def window_attention_decode(
+    q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor, scale: float, window: int,
+    sinks: int = 0,
+) -> torch.Tensor:
+    """window_attention for one new token per sequence against a cache: returns [B, N, D] for q [B, N, D] and caches
+    [B, Nk, capacity, D] (bf16 or fp16, any strides with contiguous 16-byte aligned rows; N a multiple of Nk, D a
+    multiple of 8 up to 128).  lengths (int32 on the device): the keys a sequence holds, the new token's included, so
+    the token sits at position lengths[b] - 1 and sees the keys j >= lengths[b] - window and j < sinks; values past
+    the capacity count as the capacity.  A sequence of length 0 gets zeros.  What lies behind a sequence's
+    length is not read."""
+    _check_here(q, k_cache, v_cache)
+    _require(q.dim() == 3, "q must be [B, N, D]")
+    dh, window, sinks = _window_operands(q, k_cache, v_cache, scale, window, sinks, "caches")
+    _check_lengths(lengths, q)
+    B, N, D = q.shape
+    Nk, capacity = k_cache.shape[1:3]
+    _require(capacity < _WINDOW_LIMIT, "capacity must stay below 2**30")
+    out = torch.empty((B, N, D), dtype=q.dtype, device=q.device)
+    if B == 0:
+        return out
+    if capacity == 0:
+        return out.zero_()
+    group = N // Nk
+    units = B * Nk * cdiv(group, 16)
+    tiles = cdiv(min(window, capacity), 32) + cdiv(min(sinks, max(capacity - window, 0)), 32)
+    splits = _decode_splits(units, tiles)
+    _require(units * splits < 2**31, "too many heads and sequences for one launch")
+    part = torch.empty(B * N * splits * (dh + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
+    main, join = _window_decode_launchers()
+    name = f"{_ATTN_DTYPES[q.dtype]}_d{dh}"
+    st = _stream()
+    main._launch(
+        _find(main, f"window_decode_{name}"),
+        (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), part.data_ptr() if part is not None else 0,
+         lengths.data_ptr(), q.stride(0), q.stride(1), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
+         v_cache.stride(0), v_cache.stride(1), v_cache.stride(2), out.stride(0), out.stride(1), Nk, group, splits, capacity, D,
+         window, sinks, float(scale) * 1.4426950408889634),
+        (units * splits, 1, 1), st,
+    )
+    if part is not None:
+        join._launch(
+            _find(join, f"window_decode_join_{name}"),
+            (part.data_ptr(), out.data_ptr(), lengths.data_ptr(), N, splits, D, out.stride(0), out.stride(1)),
+            (B * N, 1, 1), st,
+        )
+    return out
 
 
 # ---------------------------------------------------------------------------

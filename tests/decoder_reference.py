@@ -1,0 +1,99 @@
+"""Plain fp64 forms of the decoder-layer operators, and the error bounds their kernels are held to."""
+import math
+
+import torch
+
+
+def norm_quant(h, r, w, eps, group):
+    """(y / scale unrounded, scales, s unrounded) in fp64 for [rows, cols] operands."""
+    s = h.double() + r.double()
+    y = s / (s.square().mean(-1, keepdim=True) + eps).sqrt() * w.double()
+    x, scales = torch.empty_like(y), []
+    for c in range(0, y.shape[1], group or y.shape[1]):
+        part = y[:, c : c + (group or y.shape[1])]
+        largest = part.abs().amax(-1, keepdim=True)
+        unit = torch.where(largest == 0, torch.ones_like(largest), largest / 448)
+        x[:, c : c + part.shape[1]] = part / unit
+        scales.append(unit)
+    return x, torch.cat(scales, 1), s
+
+
+def rotary(x, positions, inv_freq, sections, interleaved, inverse):
+    """[B, S, N, D] turned in fp64; positions [A, B, S]."""
+    angle = torch.cat([positions[a].double().unsqueeze(-1) * f.double()
+                       for a, f in enumerate(torch.split(inv_freq, sections))], -1).unsqueeze(2)
+    cos, sin = angle.cos(), angle.sin() * (-1 if inverse else 1)
+    pairs = inv_freq.numel()
+    y = x.double().clone()
+    if interleaved:
+        a, b = y[..., 0 : 2 * pairs : 2].clone(), y[..., 1 : 2 * pairs : 2].clone()
+        y[..., 0 : 2 * pairs : 2], y[..., 1 : 2 * pairs : 2] = a * cos - b * sin, b * cos + a * sin
+    else:
+        a, b = y[..., :pairs].clone(), y[..., pairs : 2 * pairs].clone()
+        y[..., :pairs], y[..., pairs : 2 * pairs] = a * cos - b * sin, b * cos + a * sin
+    return y
+
+
+def visible(first, queries, keys, window, sinks, length):
+    """[queries, keys] bool: query i sits at position first + i; positions from `length` on do not exist."""
+    at = torch.arange(first, first + queries).unsqueeze(1)
+    key = torch.arange(keys).unsqueeze(0)
+    return (key <= at) & ((at - key < window) | (key < sinks)) & (at < length)
+
+
+def attention(q, k, v, scale, window, sinks, lengths=None, dout=None):
+    """fp64 attention of [B, N, Sq, D] queries, the last Sq of Sk positions.  Returns a dict: out, lse, `weight`
+    (sum of p |v|, what the rounding of the probabilities acts on), and with dout the gradients."""
+    B, N, Sq, D = q.shape
+    Nk, Sk = k.shape[1:3]
+    G = N // Nk
+    q, k, v = q.double(), k.double(), v.double()
+    out, weight = torch.zeros(B, N, Sq, D, dtype=torch.float64), torch.zeros(B, N, Sq, D, dtype=torch.float64)
+    lse = torch.full((B, N, Sq), -math.inf, dtype=torch.float64)
+    grads = {}
+    if dout is not None:
+        dout = dout.double()
+        for name, like in (("dq", q), ("dk", k), ("dv", v)):
+            grads[name] = torch.zeros_like(like, memory_format=torch.contiguous_format)
+            grads[name + "_weight"] = torch.zeros_like(grads[name])
+    for b in range(B):
+        length = Sk if lengths is None else int(lengths[b])
+        see = visible(Sk - Sq, Sq, Sk, window, sinks, length)
+        rows = see.any(-1)
+        for h in range(N):
+            kk, vv = k[b, h // G].clone(), v[b, h // G].clone()
+            kk[length:], vv[length:] = 0, 0
+            qq = torch.where(rows.unsqueeze(1), q[b, h], torch.zeros_like(q[b, h]))
+            s = (qq @ kk.T * scale).masked_fill(~see, -math.inf)
+            z = torch.logsumexp(s, -1)
+            p = torch.where(see, (s - torch.where(rows, z, torch.zeros_like(z)).unsqueeze(1)).exp(), torch.zeros_like(s))
+            out[b, h], weight[b, h], lse[b, h] = p @ vv, p @ vv.abs(), z
+            if dout is not None:
+                g = torch.where(rows.unsqueeze(1), dout[b, h], torch.zeros_like(dout[b, h]))
+                slope = g @ vv.T
+                delta = (g * out[b, h]).sum(-1, keepdim=True)
+                ds = p * (slope - delta)
+                # what the kernels round: P to the operand type, dS to the operand type, O inside delta
+                ds_size = p * (slope.abs() + delta.abs() + (g.abs() * weight[b, h]).sum(-1, keepdim=True))
+                grads["dv"][b, h // G] += p.T @ g
+                grads["dv_weight"][b, h // G] += p.T @ g.abs()
+                grads["dq"][b, h] = ds @ kk * scale
+                grads["dq_weight"][b, h] = ds_size @ kk.abs() * scale
+                grads["dk"][b, h // G] += ds.T @ qq * scale
+                grads["dk_weight"][b, h // G] += ds_size.T @ qq.abs() * scale
+    return {"out": out, "lse": lse, "weight": weight, **grads}
+
+
+def half_step(dtype):
+    """Largest relative error of one rounding to dtype."""
+    return torch.finfo(dtype).eps / 2
+
+
+def attention_bound(want, weight, dtype):
+    """Error bound of an attention result.  The stored value is rounded once (half a step of it).  Every term of the
+    sum carries one rounding of its probability (or dS) to the operand type, half a step of the sum of the terms'
+    sizes `weight`; and the error of its score in fp32: at most (D + 2) 2^-24 sum |q k| scale, for normal operands
+    of D <= 128 below 130 * 6e-8 * 8 = 6.2e-5, twice (the term and the normalising sum), rounded up to 2e-4.
+    fp16 probabilities below its smallest normal number are off by up to 2^-25 of the largest, which 1e-5 covers."""
+    h = half_step(dtype)
+    return want.abs() * h + weight * (h + 2e-4) + 1e-5

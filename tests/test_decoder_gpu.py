@@ -1,0 +1,259 @@
+"""Decoder-layer operators against their plain forms in 64 bits: residual norm with an 8-bit result, rotary
+positions over several axes, attention with a sliding window and visible first tokens.
+
+Tolerances are error bounds derived from the roundings each kernel makes (half a step of the type per rounding, the
+fp32 accumulation bounds beside it); tests/decoder_reference.py holds those of attention."""
+import math
+
+import pytest
+import torch
+
+from tests import decoder_reference as R
+from tests.helpers import announce
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+BF, HF = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module")
+def K():
+    from inductor_x_amd import kernels
+
+    return kernels
+
+
+def within(got, want, bound, what):
+    got = got.detach().double().cpu()
+    assert got.shape == want.shape, f"{what}: shape {tuple(got.shape)} against {tuple(want.shape)}"
+    assert torch.isfinite(got).all(), f"{what}: not finite"
+    over = ((got - want).abs() - bound).amax() if got.numel() else torch.tensor(-1.0)
+    assert over <= 0, f"{what}: {over.item():.3g} over the bound"
+
+
+# ------------------------------------------------------------------------------------ norm
+def norm_operands(rows, cols, dtype, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    h = torch.randn(rows, cols, generator=gen).to(dtype)
+    r = (2 * torch.randn(rows, cols, generator=gen)).to(dtype)
+    r[:, :: max(1, cols // 5)] *= 20
+    w = (1 + 0.1 * torch.randn(cols, generator=gen)).to(dtype)
+    return h, r, w
+
+
+def check_norm(got, h, r, w, eps, group):
+    q, scales, s = got
+    x, unit, total = R.norm_quant(h, r, w, eps, group)
+    assert q.dtype == torch.float8_e4m3fn and scales.dtype == torch.float32 and s.dtype == h.dtype
+    within(s.reshape(total.shape), total, total.abs() * R.half_step(h.dtype) + 2.0**-25, "s")
+    # the sum of squares: at most 32 terms in a row per thread and ten folding steps, halved by the square root,
+    # and a handful of single roundings: below 4e-6
+    within(scales.reshape(unit.shape), unit, unit * 4e-6, "scales")
+    # e4m3: half a step of the value, half the smallest step near zero, and 8e-6 from y and the scale
+    within(q.reshape(x.shape), x, x.abs() * (2.0**-4 + 8e-6) + 2.0**-10, "q")
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("group", [0, 128])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 7), (5, 128), (2, 129), (7, 512), (9, 1000), (4, 1024), (6, 2048), (3, 2051),
+                                       (33, 4096), (2, 5120), (2, 8192), (2, 16384), (1, 20001), (1, 32768)])
+def test_norm_quant(K, rows, cols, group, dtype):
+    announce(f"add_rmsnorm_quant rows={rows} cols={cols} group={group} {dtype}")
+    h, r, w = norm_operands(rows, cols, dtype)
+    check_norm(K.add_rmsnorm_quant(h.to(DEV), r.to(DEV), w.to(DEV), 1e-6, group=group), h, r, w, 1e-6, group)
+
+
+def test_norm_quant_strides_and_axes(K):
+    announce("add_rmsnorm_quant strides")
+    h, r, w = norm_operands(24, 384, BF)
+    wide = torch.zeros(24, 1024, dtype=BF, device=DEV)
+    wide[:, 128:512] = h.to(DEV)
+    odd = torch.zeros(24 * 384 + 1, dtype=BF, device=DEV)[1:].view(24, 384)  # rows off the 16-byte grid
+    odd.copy_(r)
+    got = K.add_rmsnorm_quant(wide[:, 128:512], odd, w.to(DEV), 1e-6, group=128)
+    check_norm(got, h, r, w, 1e-6, 128)
+    got3 = K.add_rmsnorm_quant(h.to(DEV).view(2, 12, 384), r.to(DEV).view(2, 12, 384), w.to(DEV), 1e-6, group=128)
+    assert got3[0].shape == (2, 12, 384) and got3[1].shape == (2, 12, 3) and got3[2].shape == (2, 12, 384)
+    check_norm(got3, h, r, w, 1e-6, 128)
+
+
+def test_norm_quant_empty_zero_and_nonfinite(K):
+    announce("add_rmsnorm_quant edge values")
+    w = torch.ones(256, dtype=BF, device=DEV)
+    q, scales, s = K.add_rmsnorm_quant(torch.empty(0, 256, dtype=BF, device=DEV), torch.empty(0, 256, dtype=BF, device=DEV), w)
+    assert q.shape == (0, 256) and scales.shape == (0, 1) and s.shape == (0, 256)
+    h = torch.randn(4, 256).to(BF)
+    h[0] = 0
+    h[1, 3] = float("nan")
+    h[2, 200] = float("inf")
+    z = torch.zeros(4, 256, dtype=BF, device=DEV)
+    q, scales, s = (t.float().cpu() for t in K.add_rmsnorm_quant(h.to(DEV), z, w, 1e-6, group=128))
+    assert (q[0] == 0).all() and (scales[0] == 1).all()
+    assert torch.isnan(q[1]).all() and torch.isnan(scales[1]).all()
+    # an infinity: its own 128 columns become NaN, the others zero, as inf * 0 and x * 0 say
+    assert torch.isnan(scales[2, 1]) and scales[2, 0] == 1 and (q[2, :128] == 0).all()
+    assert torch.isfinite(q[3]).all() and scales[3].min() > 0
+    assert torch.equal(s.isnan(), h.float().isnan())
+    # the smallest numbers of the type: no division by a scale that underflowed
+    tiny = torch.full((2, 256), 2.0**-133).to(BF)
+    q, scales, _ = K.add_rmsnorm_quant(tiny.to(DEV), torch.zeros_like(tiny).to(DEV), w, 1e-6)
+    assert torch.isfinite(q.float()).all() and (scales > 0).all()
+
+
+# ------------------------------------------------------------------------------------ rotary
+def check_rotary(got, x, positions, inv_freq, sections, interleaved, inverse):
+    want = R.rotary(x, positions, inv_freq, sections, interleaved, inverse)
+    # a rounding of the result, and in fp32: sine and cosine off by 4e-7 (angle 2e-7, function 2 ulp), two products
+    # and a sum of numbers no larger than the pair, 2e-7
+    size = x.double().abs().amax(-1, keepdim=True).expand_as(want)
+    within(got, want, want.abs() * R.half_step(x.dtype) + 1.5e-6 * size + 2.0**-25, "rotary")
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, torch.float32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("B,S,N,Nk,D,pairs,sections,first", [
+    (1, 1, 1, 1, 2, 1, [1], 0),
+    (2, 5, 4, 2, 64, 32, [32], 0),
+    (1, 7, 3, 1, 80, 20, [12, 8], 1000000),
+    (3, 33, 8, 2, 128, 64, [16, 24, 24], 123456),
+    (2, 3, 2, 2, 96, 48, [1, 46, 0, 1], 50),
+    (1, 4, 5, 5, 22, 7, [3, 4], 9),
+    (1, 515, 16, 4, 128, 64, [64], 0),
+])
+def test_rotary(K, B, S, N, Nk, D, pairs, sections, first, interleaved, dtype):
+    announce(f"rotary_axes {B, S, N, Nk, D, pairs, sections, first, interleaved} {dtype}")
+    gen = torch.Generator().manual_seed(1)
+    q, k = torch.randn(B, S, N, D, generator=gen).to(dtype), torch.randn(B, S, Nk, D, generator=gen).to(dtype)
+    positions = first + torch.randint(0, 5000, (len(sections), B, S), generator=gen)
+    inv_freq = (10000.0 ** (-torch.arange(pairs).double() / pairs)).float()
+    for inverse in (False, True):
+        got = K.rotary_axes(q.to(DEV), k.to(DEV), positions.to(torch.int32).to(DEV), inv_freq.to(DEV), sections, interleaved, inverse)
+        for x, y in zip((q, k), got):
+            check_rotary(y, x, positions, inv_freq, sections, interleaved, inverse)
+
+
+def test_rotary_forms_of_operands(K):
+    announce("rotary_axes strides, int64 far positions, fp64 frequencies, one axis without its dimension, empty")
+    gen = torch.Generator().manual_seed(2)
+    qkv = torch.randn(2, 9, 3, 4, 64, generator=gen).to(BF)  # [B, S, (q, k, v), N, D] as one projection leaves it
+    dev = qkv.to(DEV)
+    positions = torch.randint(2**33, 2**33 + 10, (2, 9), generator=gen)
+    inv_freq = 10000.0 ** (-torch.arange(32).double() / 32)
+    got = K.rotary_axes(dev[:, :, 0], dev[:, :, 1], positions.to(DEV), inv_freq.to(DEV))
+    for x, y in zip((qkv[:, :, 0], qkv[:, :, 1]), got):
+        # 2^33 positions at frequency 1: 1.4e9 turns in 64 bits, 2e-7 of a turn off, 1.3e-6 of the angle
+        want = R.rotary(x, positions.unsqueeze(0), inv_freq, [32], False, False)
+        within(y, want, want.abs() * R.half_step(BF) + 1e-5 * x.double().abs().amax(), "far")
+    heads_first = torch.randn(2, 4, 9, 64, generator=gen).to(BF)
+    t = heads_first.to(DEV).transpose(1, 2)
+    y, _ = K.rotary_axes(t, t, torch.zeros(2, 9, dtype=torch.int32, device=DEV), inv_freq.to(DEV))
+    assert torch.equal(y.cpu(), heads_first.transpose(1, 2)) and y.stride() == t.stride()  # position 0 turns nothing
+    e, _ = K.rotary_axes(t[:, :0], t[:, :0], torch.zeros(2, 0, dtype=torch.int32, device=DEV), inv_freq.to(DEV))
+    assert e.shape == (2, 0, 4, 64)
+
+
+# ------------------------------------------------------------------------------------ decode
+def caches(B, Nk, capacity, D, dtype, token_major, gen):
+    shape = (B, capacity, Nk, D) if token_major else (B, Nk, capacity, D)
+    c = torch.randn(*shape, generator=gen).to(dtype)
+    return c.transpose(1, 2) if token_major else c
+
+
+def same_memory(t):
+    """The tensor on the GPU with its strides."""
+    out = torch.empty_strided(t.shape, t.stride(), dtype=t.dtype, device=DEV)
+    return out.copy_(t)
+
+
+def decode_reference(q, k, v, lengths, scale, window, sinks):
+    B, N, D = q.shape
+    out, weight = torch.zeros(B, N, D, dtype=torch.float64), torch.zeros(B, N, D, dtype=torch.float64)
+    for b, n in enumerate(lengths):
+        n = min(max(n, 0), k.shape[2])
+        if n:
+            r = R.attention(q[b : b + 1].unsqueeze(2), k[b : b + 1, :, :n], v[b : b + 1, :, :n], scale, window, sinks)
+            out[b], weight[b] = r["out"][0, :, 0], r["weight"][0, :, 0]
+    return out, weight
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("token_major", [False, True])
+@pytest.mark.parametrize("B,N,Nk,D,capacity,window,sinks,lengths", [
+    (1, 1, 1, 8, 1, 1, 0, [1]),
+    (3, 4, 2, 64, 40, 16, 3, [0, 17, 40]),
+    (2, 8, 1, 128, 300, 64, 4, [300, 66]),
+    (1, 40, 2, 96, 200, 1000, 0, [199]),           # 20 query heads on a key head: two workgroups' worth
+    (5, 6, 3, 80, 129, 33, 64, [1, 2, 98, 129, 97]),
+    (1, 8, 2, 128, 5000, 4096, 4, [4999]),           # many splits
+    (2, 3, 1, 56, 700, 512, 100, [611, 700]),
+    (4, 2, 2, 64, 65, 2**31 - 1, 2**31 - 1, [65, 1, 0, 64]),
+])
+def test_decode(K, B, N, Nk, D, capacity, window, sinks, lengths, token_major, dtype):
+    announce(f"window_attention_decode {B, N, Nk, D, capacity, window, sinks, lengths, token_major} {dtype}")
+    gen = torch.Generator().manual_seed(3)
+    q = torch.randn(B, N, D, generator=gen).to(dtype)
+    k, v = (caches(B, Nk, capacity, D, dtype, token_major, gen) for _ in range(2))
+    want, weight = decode_reference(q, k, v, lengths, D**-0.5, window, sinks)
+    # what lies behind a sequence's length, or between its first tokens and its window, must not matter
+    for b, n in enumerate(lengths):
+        for c in (k, v):
+            c[b, :, n:] = float("nan")
+            c[b, :, min(sinks, n) : max(0, n - window)] = float("inf")
+    got = K.window_attention_decode(q.to(DEV), same_memory(k), same_memory(v), torch.tensor(lengths, dtype=torch.int32, device=DEV),
+                                    D**-0.5, window, sinks)
+    assert got.dtype == dtype
+    within(got, want, R.attention_bound(want, weight, dtype), "decode")
+
+
+def test_decode_lengths_beyond_the_cache(K):
+    announce("window_attention_decode lengths beyond the capacity and below zero")
+    gen = torch.Generator().manual_seed(4)
+    q = torch.randn(3, 4, 64, generator=gen).to(BF)
+    k, v = (caches(3, 2, 50, 64, BF, False, gen) for _ in range(2))
+    want, weight = decode_reference(q, k, v, [50, 0, 50], 0.125, 20, 2)
+    got = K.window_attention_decode(q.to(DEV), k.to(DEV), v.to(DEV), torch.tensor([51, -3, 2**31 - 1], dtype=torch.int32, device=DEV),
+                                    0.125, 20, 2)
+    within(got, want, R.attention_bound(want, weight, BF), "clamped")
+
+
+def test_decode_offsets_past_32_bits(K):
+    announce("window_attention_decode in a cache whose byte offsets pass 2^32")
+    # two sequences of 8 heads: rows 2 KiB apart, 1.2 million tokens: 2.4 GB a sequence, the window at its end
+    capacity, n = 1_200_000, 1_199_990
+    gen = torch.Generator().manual_seed(5)
+    cache = torch.zeros(2, capacity, 8, 128, dtype=BF, device=DEV)
+    near = torch.randn(2, 64, 8, 128, generator=gen).to(BF)
+    cache[:, n - 64 : n] = near.to(DEV)
+    q = torch.randn(2, 8, 128, generator=gen).to(BF)
+    view = cache.transpose(1, 2)
+    got = K.window_attention_decode(q.to(DEV), view, view, torch.tensor([n, n], dtype=torch.int32, device=DEV), 0.1, 64, 0)
+    small = near.transpose(1, 2)
+    want, weight = decode_reference(q, small, small, [64, 64], 0.1, 64, 0)
+    within(got, want, R.attention_bound(want, weight, BF), "far")
+
+
+def test_decode_captured_and_on_another_stream(K):
+    announce("window_attention_decode captured in a graph, on a side stream")
+    gen = torch.Generator().manual_seed(6)
+    q = torch.randn(2, 8, 128, generator=gen).to(BF).to(DEV)
+    k, v = (caches(2, 2, 2000, 128, BF, False, gen).to(DEV) for _ in range(2))
+    lengths = torch.tensor([2000, 700], dtype=torch.int32, device=DEV)
+    call = lambda: K.window_attention_decode(q, k, v, lengths, 0.09, 1500, 4)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = call()
+    for step in range(4):
+        q.copy_(torch.randn(2, 8, 128, generator=gen).to(BF))
+        lengths.copy_(torch.tensor([1 + 400 * step, 2000 - 300 * step], dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, call()), f"replay {step}"
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = call()
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(other, call())

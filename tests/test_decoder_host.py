@@ -1,0 +1,131 @@
+"""Argument checks and shape functions of the decoder-layer operators, without a GPU: the device check and the launch are
+replaced, everything between them is the product's."""
+import pytest
+import torch
+
+from inductor_x_amd import decoder, kernels as K
+
+BF = torch.bfloat16
+
+
+class Launched(Exception):
+    pass
+
+
+@pytest.fixture(autouse=True)
+def no_gpu(monkeypatch):
+    def launched(self, *a, **k):
+        raise Launched(self.name)
+
+    monkeypatch.setattr(K, "_check_cuda", lambda *t: None)
+    monkeypatch.setattr(K, "_check_here", lambda *t: None)
+    monkeypatch.setattr(K, "_stream", lambda: 0)
+    monkeypatch.setattr(K, "_find", lambda l, symbol: 0)
+    monkeypatch.setattr(K.CachingLauncher, "_launch", launched)
+
+
+def test_tensors_on_the_host_are_refused(monkeypatch):
+    monkeypatch.undo()
+    x = torch.zeros(2, 64, dtype=BF)
+    with pytest.raises(ValueError, match="GPU"):
+        K.add_rmsnorm_quant(x, x, x[0])
+    with pytest.raises(ValueError, match="GPU"):
+        K.rotary_axes(x.view(1, 1, 2, 64), x.view(1, 1, 2, 64), torch.zeros(1, 1, dtype=torch.int32), torch.ones(4))
+    with pytest.raises(ValueError, match="GPU"):
+        K.window_attention_decode(x.view(1, 2, 64), x.view(1, 1, 2, 64), x.view(1, 1, 2, 64), torch.ones(1, dtype=torch.int32), 1.0, 1)
+
+
+def test_norm_quant_refusals():
+    h, w = torch.zeros(4, 256, dtype=BF), torch.ones(256, dtype=BF)
+    with pytest.raises(Launched):
+        K.add_rmsnorm_quant(h, h, w, group=128)
+    for args, kw, text in [
+        ((h, h.half(), w), {}, "share bf16 or fp16"),
+        ((h.float(), h.float(), w.float()), {}, "share bf16 or fp16"),
+        ((h, h[:2], w), {}, "same shape"),
+        ((h, h, w[:128]), {}, "vector of the row length"),
+        ((h, h, torch.ones(512, dtype=BF)[::2]), {}, "contiguous vector"),
+        ((h, h, w), {"group": 64}, "group"),
+        ((h[:, :0], h[:, :0], w[:0]), {}, "1..32768"),
+        ((torch.zeros(1, 40000, dtype=BF),) * 2 + (torch.zeros(40000, dtype=BF),), {}, "1..32768"),
+        ((torch.zeros(256, 4, dtype=BF).t(), h, w), {}, "columns must be contiguous"),
+        ((torch.zeros(4, 3, 256, dtype=BF)[:, :2], torch.zeros(4, 2, 256, dtype=BF), w), {}, "evenly spaced"),
+    ]:
+        with pytest.raises(ValueError, match=text):
+            K.add_rmsnorm_quant(*args, **kw)
+
+
+def test_rotary_refusals():
+    q, k = torch.zeros(2, 3, 4, 64, dtype=BF), torch.zeros(2, 3, 2, 64, dtype=BF)
+    at, f = torch.zeros(2, 2, 3, dtype=torch.int32), torch.ones(32)
+    with pytest.raises(Launched):
+        K.rotary_axes(q, k, at, f, [20, 12])
+    with pytest.raises(Launched):
+        K.rotary_axes(q, k, at[0], f)
+    for args, text in [
+        ((q, k.half(), at, f, [20, 12]), "share"),
+        ((q.double(), k.double(), at, f, [20, 12]), "share"),
+        ((q[0], k[0], at, f, [20, 12]), r"\[B, S, N, D\]"),
+        ((q, k[:, :2], at, f, [20, 12]), "share batch"),
+        ((q.transpose(2, 3).contiguous().transpose(2, 3), k, at, f, [20, 12]), "contiguous"),
+        ((q, k, at[:, :1], f, [20, 12]), "positions"),
+        ((q, k, torch.zeros(5, 2, 3, dtype=torch.int32), f, [10, 10, 10, 1, 1]), "positions"),
+        ((q, k, at.float(), f, [20, 12]), "positions"),
+        ((q, k, at.transpose(1, 2).contiguous().transpose(1, 2), f, [20, 12]), "positions"),
+        ((q, k, at, f.half(), [20, 12]), "inv_freq"),
+        ((q, k, at, torch.ones(33), [20, 13]), "inv_freq"),
+        ((q, k, at, torch.ones(0), [0, 0]), "inv_freq"),
+        ((q, k, at, f, None), "sections"),
+        ((q, k, at, f, [20, 13]), "sections"),
+        ((q, k, at, f, [33, -1]), "sections"),
+    ]:
+        with pytest.raises(ValueError, match=text):
+            K.rotary_axes(*args)
+
+
+def decode_operands(B=2, N=4, Nk=2, capacity=16, D=64):
+    return (torch.zeros(B, N, D, dtype=BF), torch.zeros(B, Nk, capacity, D, dtype=BF), torch.zeros(B, Nk, capacity, D, dtype=BF),
+            torch.ones(B, dtype=torch.int32))
+
+
+def test_decode_refusals():
+    q, k, v, n = decode_operands()
+    with pytest.raises(Launched):
+        K.window_attention_decode(q, k, v, n, 0.1, 4, 1)
+    for args, text in [
+        ((q.unsqueeze(2), k, v, n, 0.1, 4, 1), r"\[B, N, D\]"),
+        ((q, k, v[:, :, :8], n, 0.1, 4, 1), "share one"),
+        ((q.half(), k, v, n, 0.1, 4, 1), "share bf16"),
+        ((q[:, :3], k, v, n, 0.1, 4, 1), "multiple of the key heads"),
+        ((q[..., :60], k[..., :60], v[..., :60], n, 0.1, 4, 1), "multiple of 8"),
+        ((*decode_operands(D=136), 0.1, 4, 1), "multiple of 8"),
+        ((q, k, v, n.long(), 0.1, 4, 1), "int32"),
+        ((q, k, v, n[:1], 0.1, 4, 1), "one value per sequence"),
+        ((q, k, v, n, 0.0, 4, 1), "scale"),
+        ((q, k, v, n, float("nan"), 4, 1), "scale"),
+        ((q, k, v, n, 0.1, 0, 1), "window"),
+        ((q, k, v, n, 0.1, 4, -1), "sinks"),
+        ((q, torch.zeros(2, 2, 16, 68, dtype=BF)[..., :64], v, n, 0.1, 4, 1), "16-byte aligned"),
+        ((q, torch.zeros(2, 2, 64, 16, dtype=BF).transpose(2, 3), v, n, 0.1, 4, 1), "contiguous"),
+        ((q, k.new_empty(1).expand(2, 2, 16, 64), v, n, 0.1, 4, 1), "contiguous"),
+    ]:
+        with pytest.raises(ValueError, match=text):
+            K.window_attention_decode(*args)
+    assert K.window_attention_decode(q[:0], k[:0], v[:0], n[:0], 0.1, 4).shape == (0, 4, 64)
+    assert (K.window_attention_decode(q, k[:, :, :0], v[:, :, :0], n, 0.1, 4) == 0).all()
+
+
+def test_shape_functions():
+    m = lambda *s, dtype=BF: torch.empty(*s, dtype=dtype, device="meta")  # noqa: E731
+    q, scales, s = decoder.add_rmsnorm_quant(m(3, 5, 300), m(3, 5, 300), m(300), 1e-6, 128)
+    assert q.dtype == torch.float8_e4m3fn and q.shape == s.shape == (3, 5, 300) and scales.shape == (3, 5, 3)
+    a, b = decoder.rotary_axes(m(2, 3, 4, 64), m(2, 3, 1, 64), m(1, 2, 3, dtype=torch.int32), m(32, dtype=torch.float32))
+    assert a.shape == (2, 3, 4, 64) and b.shape == (2, 3, 1, 64)
+    assert decoder.window_attention_decode(m(2, 4, 64), m(2, 2, 9, 64), m(2, 2, 9, 64), m(2, dtype=torch.int32), 0.1, 4).shape == (2, 4, 64)
+
+
+def test_splits_of_a_decode():
+    for units in (1, 7, 64, 512, 5000):
+        for tiles in (1, 3, 33, 129, 40000):
+            n = K._decode_splits(units, tiles)
+            assert 1 <= n <= 64 and (n == 1 or tiles // n >= 8)
