@@ -1,0 +1,349 @@
+// Attention with a sliding window and first tokens that stay visible (sinks), for heads that share keys.
+//
+//   position of query i:  p = i + (Sk - Sq)          (the queries are the last Sq of Sk positions)
+//   key j is visible:     j <= p  and  (p - j < window  or  j < sinks)
+//   O = softmax(Q K^T * scale over the visible keys) V,   lse = log sum exp of the scaled scores
+//
+// Positions from lengths[b] on do not exist (right padding): their keys are hidden and not read, their rows are
+// zero, lse -inf.
+//
+// Work of a workgroup: eight wavefronts of 32 queries on one key head.  They are HB = 1, 2, 4 or 8 query heads
+// that share the key head times 256 / HB consecutive queries, so that heads in a group read a key tile once
+// between them, and a block visits the keys of a window plus 256 / HB - 1 others instead of 255.  The key
+// tiles of 64 it visits are the tiles that hold sinks, then those from the window of its first query to the
+// position of its last; nothing between them is read, and no mask exists in memory: a wavefront compares
+// positions in the few tiles that are neither wholly visible nor wholly hidden to it.
+//
+// Operand layouts and the transposed products are those of attention.h.  Tiles travel memory -> LDS by direct
+// 16-byte loads, [64][DH] as they lie in memory with the chunks of a row swizzled; rows past the end and
+// columns past the head dimension arrive as zeros (bounds of the buffer descriptor).
+#pragma once
+
+#include "attention.h"
+
+namespace mi {
+
+constexpr int kWinWaves = 8;
+constexpr int kWinThreads = 64 * kWinWaves;
+constexpr int kWinRows = 32 * kWinWaves;  // (head, query) rows or keys of a workgroup
+constexpr int kWinTile = 64;              // keys (queries) of a tile
+constexpr float kWinLog2e = 1.4426950408889634f;
+constexpr float kWinLn2 = 0.69314718055994530942f;
+constexpr float kWinFloor = -1e30f;       // below every score: keeps rows without a visible key so far free of inf - inf
+
+// Strides in elements of a [batch, head, token, column] tensor with contiguous columns.
+struct WindowStride {
+  long long batch, head, token;
+};
+
+// Shared problem description; every kernel takes one as its last argument.
+struct WindowShape {
+  const int* lengths;  // may be null: every position exists
+  int batch, heads, kv_heads, group, Sq, Sk, dim, window, sinks, hb_shift, mixed;
+  float scale;
+
+  __device__ __forceinline__ int offset() const { return Sk - Sq; }
+  __device__ __forceinline__ int length(int b) const { return lengths ? min(max(lengths[b], 0), Sk) : Sk; }
+  // queries that exist (may be <= 0)
+  __device__ __forceinline__ int query_end(int b) const { return min(Sq, length(b) - offset()); }
+};
+
+// The key tiles a block visits: `front` tiles with sinks, then a run that starts `skip` tiles further on.
+struct WindowTiles {
+  int front, skip, n;
+  __device__ __forceinline__ int at(int i) const { return i < front ? i : i + skip; }
+};
+__device__ __forceinline__ WindowTiles window_tiles(int p_lo, int p_hi, int window, int sinks) {
+  const int first = max(0, p_lo - window + 1) / kWinTile, last = p_hi / kWinTile;
+  WindowTiles t;
+  t.front = min((min(sinks, p_hi + 1) + kWinTile - 1) / kWinTile, first);
+  t.skip = first - t.front;
+  t.n = last - first + 1 + t.front;
+  return t;
+}
+
+// Chunk swizzle of a tile row: the 16-byte chunk c of row r lies at position c ^ win_swz(r).  One swizzle serves the
+// reads along the rows (one row per lane) and the transposing reads (four rows x 64 bytes per 32 lanes).
+template <int DH>
+__device__ __forceinline__ int win_swz(int row) {
+  const int r0 = row & 1, r1 = (row >> 1) & 1, r2 = (row >> 2) & 1, r3 = (row >> 3) & 1;
+  if constexpr (DH == 128) return (r0 << 1) | (r1 << 2) | r2 | ((r0 ^ r3) << 3);
+  return r0 | (r1 << 2) | (r2 << 1);
+}
+
+// ROWS rows of DH columns, memory -> LDS, by WAVES wavefronts.  `rows` of them exist (<= 0: none), `dim` columns hold data.
+// Byte offsets stay inside the tile: the caller's pointer is the tile's first row.
+template <typename T, int DH, int ROWS, int WAVES>
+__device__ __forceinline__ void win_copy(const T* src, long long stride, int rows, int dim, T* dst, int wave, int lane) {
+  constexpr int CH = DH / 8;            // chunks of a row
+  constexpr int PER = 64 / CH;          // rows of one instruction
+  constexpr int N = ROWS / PER / WAVES;  // instructions of a wavefront
+  const int bytes = rows > 0 ? static_cast<int>((min(rows, ROWS) - 1) * stride * 2) + dim * 2 : 0;
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    const int blk = wave * N + u;
+    const int row = blk * PER + lane / CH;
+    const int chunk = (lane % CH) ^ win_swz<DH>(row);
+    const int voff = 8 * chunk < dim ? row * static_cast<int>(stride) * 2 + 16 * chunk : 0x7ffffff0;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(src), 0, bytes, 0x00020000),
+        (__attribute__((address_space(3))) void*)(dst + blk * 512), 16, voff, 0, 0, 0);
+  }
+}
+
+// A operand along the rows of a tile: row `row`, d slice s, half g
+template <typename T, int DH>
+__device__ __forceinline__ typename AttnElem<T>::x8 win_row_frag(const T* tile, int row, int s, int g) {
+  return *reinterpret_cast<const typename AttnElem<T>::x8*>(tile + row * DH + 8 * ((2 * s + g) ^ win_swz<DH>(row)));
+}
+// Per-lane offsets of the transposing reads, one per block of 32 columns: in every group of 16 lanes, lane s points at
+// four consecutive d of row 4 g + s / 4 (+ 8 for the second read) and receives, for its own d, the four rows.
+template <int DH, int DB>
+__device__ __forceinline__ void win_tr_offsets(int (&off)[DB], int lane) {
+  const int sl = lane & 15, grp = lane >> 4;
+  const int row = 4 * (grp >> 1) + (sl >> 2);
+  const int c = 2 * (grp & 1) + ((sl & 3) >> 1);
+#pragma unroll
+  for (int db = 0; db < DB; ++db) off[db] = row * DH + 8 * ((4 * db + c) ^ win_swz<DH>(row)) + 4 * (sl & 1);
+}
+// A operand across the rows (the tile transposed): columns of block db via its offset, row slice t of 16
+template <typename T, int DH>
+__device__ __forceinline__ typename AttnElem<T>::x8 win_tr_frag(const T* tile, int off, int t) {
+  typedef AttnElem<T> E;
+  const typename E::x4 lo = E::read_tr(tile + 16 * t * DH + off);
+  const typename E::x4 hi = E::read_tr(tile + (16 * t + 8) * DH + (off ^ (8 * win_swz<DH>(8))));
+  typename E::x8 r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    r[e] = lo[e];
+    r[4 + e] = hi[e];
+  }
+  return r;
+}
+
+// B operand fragments of one row in memory: zeros past the head dimension
+template <typename T, int DS>
+__device__ __forceinline__ void win_load_row(typename AttnElem<T>::x8 (&f)[DS], const T* row, int dim, int g) {
+#pragma unroll
+  for (int s = 0; s < DS; ++s) {
+    const int c = 16 * s + 8 * g;
+    if (c < dim) {
+      f[s] = *reinterpret_cast<const typename AttnElem<T>::x8*>(row + c);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[s][e] = static_cast<T>(0.f);
+    }
+  }
+}
+
+template <int DB>
+__device__ __forceinline__ void win_zero(f32x16_t (&acc)[DB]) {
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[db][r] = 0.f;
+}
+
+// Transposed accumulators (lane = row, registers = columns) of a wavefront's 32 rows -> memory, through the
+// wavefront's own 32 x DH piece of LDS so that whole rows leave.  Rows below `exist` get the values times the lane's
+// factor, those from there to `rows` zeros.
+template <typename T, int DH, int DB>
+__device__ __forceinline__ void win_store(T* dst, long long stride, const f32x16_t (&acc)[DB], float factor, T* stage,
+                                          int lane, int exist, int rows, int dim) {
+  typedef typename AttnElem<T>::x4 x4_t;
+  constexpr int CH = DH / 8;
+  const int li = lane & 31, g = lane >> 5;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int rq = 0; rq < 4; ++rq) {
+      x4_t o4;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o4[e] = static_cast<T>(li < exist ? acc[db][4 * rq + e] * factor : 0.f);
+      *reinterpret_cast<x4_t*>(stage + li * DH + 8 * ((4 * db + rq) ^ (li % CH)) + 4 * g) = o4;
+    }
+  const int c = lane % CH;
+#pragma unroll
+  for (int j = 0; j < CH / 2; ++j) {
+    const int row = j * (64 / CH) + lane / CH;
+    const u32x4_t v16 = *reinterpret_cast<const u32x4_t*>(stage + row * DH + 8 * (c ^ (row % CH)));
+    if (row < rows && 8 * c < dim) *reinterpret_cast<u32x4_t*>(dst + row * stride + 8 * c) = v16;
+  }
+}
+
+// Where a workgroup works.  Consecutive ids go round-robin to the eight dies, each with its own L2: a die takes a
+// contiguous eighth of the items, which run through one key head's query blocks before the next.  Blocks run from the
+// last to the first (a block without a full window before it is shorter); with `mixed` the two ends alternate, so that
+// any run of items has the same work also where a die's share is part of a head.
+struct WindowBlock {
+  int b, kvh, qb, hg;
+  bool any;
+};
+__device__ __forceinline__ WindowBlock window_block(const WindowShape& s, int blocks, int parts) {
+  const int per_kv = blocks * parts;
+  const int total = s.batch * s.kv_heads * per_kv;
+  const int share = (total + 7) / 8;
+  const int item = (blockIdx.x % 8) * share + blockIdx.x / 8;
+  WindowBlock w;
+  w.any = static_cast<int>(blockIdx.x / 8) < share && item < total;
+  const int unit = item / per_kv, rest = item % per_kv;
+  w.b = unit / s.kv_heads;
+  w.kvh = unit % s.kv_heads;
+  const int at = rest / parts;
+  w.hg = rest % parts;
+  w.qb = s.mixed ? (at & 1 ? at >> 1 : blocks - 1 - (at >> 1)) : blocks - 1 - at;
+  return w;
+}
+
+// What one wavefront sees of the block: 32 queries of one head.
+struct WindowWave {
+  int head, q0, exist, rows;  // first query, how many of the 32 exist, how many lie inside Sq
+  int p_lo, p_hi;             // positions of the first and last that exist
+  int window, sinks;
+  // some query sees some key of the tile / every query sees every key
+  __device__ __forceinline__ bool active(int tile) const {
+    const int k = tile * kWinTile;
+    return exist > 0 && k <= p_hi && (k + kWinTile > p_lo - window + 1 || k < sinks);
+  }
+  __device__ __forceinline__ bool whole(int tile) const {
+    const int k = tile * kWinTile;
+    return k + kWinTile - 1 <= p_lo && (k > p_hi - window || k + kWinTile <= sinks);
+  }
+  // key `k` seen from position p
+  __device__ __forceinline__ bool sees(int p, int k) const { return k <= p && (k > p - window || k < sinks); }
+};
+__device__ __forceinline__ WindowWave window_wave(const WindowShape& s, const WindowBlock& w, int wave, int query_end) {
+  WindowWave v;
+  const int per_head = kWinWaves >> s.hb_shift;  // wavefronts of a head
+  v.head = w.kvh * s.group + (w.hg << s.hb_shift) + wave / per_head;
+  v.q0 = w.qb * (32 * per_head) + 32 * (wave % per_head);
+  v.exist = min(32, query_end - v.q0);
+  v.rows = min(32, s.Sq - v.q0);
+  v.p_lo = v.q0 + s.offset();
+  v.p_hi = v.p_lo + v.exist - 1;
+  v.window = s.window;
+  v.sinks = s.sinks;
+  return v;
+}
+
+// ---------------------------------------------------------------------------------------------
+// forward
+// ---------------------------------------------------------------------------------------------
+struct WindowFwdArgs {
+  const void *q, *k, *v;
+  void* o;
+  float* lse;  // [B, N, Sq]
+  WindowStride qs, ks, vs, os;
+  WindowShape shape;
+};
+
+template <typename T, int DH>
+__device__ __forceinline__ void window_attention_fwd(const WindowFwdArgs& a) {
+  typedef AttnElem<T> E;
+  typedef typename E::x8 x8_t;
+  constexpr int DS = DH / 16, DB = DH / 32, TILE = kWinTile * DH;
+  extern __shared__ __attribute__((aligned(16))) unsigned char attn_lds[];
+  const WindowShape& s = a.shape;
+  const int lane = threadIdx.x & 63, li = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int per_block = kWinRows >> s.hb_shift;
+  const WindowBlock w = window_block(s, (s.Sq + per_block - 1) / per_block, s.group >> s.hb_shift);
+  if (!w.any) return;
+  const int length = s.length(w.b), query_end = s.query_end(w.b);
+  const WindowWave me = window_wave(s, w, wave, query_end);
+  T* O = static_cast<T*>(a.o) + w.b * a.os.batch + me.head * a.os.head + me.q0 * a.os.token;
+  float* lse = a.lse + (static_cast<size_t>(w.b) * s.heads + me.head) * s.Sq + me.q0;
+  T* stage = reinterpret_cast<T*>(attn_lds) + wave * (32 * DH);
+  f32x16_t oacc[DB];
+  win_zero(oacc);
+  const int block_q0 = w.qb * per_block;
+  if (block_q0 >= query_end) {  // nothing here exists
+    win_store<T, DH>(O, a.os.token, oacc, 0.f, stage, lane, 0, me.rows, s.dim);
+    if (g == 0 && li < me.rows) lse[li] = -__builtin_inff();
+    return;
+  }
+  const int p_lo = block_q0 + s.offset();
+  const int p_hi = min(block_q0 + per_block, query_end) - 1 + s.offset();
+  const WindowTiles tiles = window_tiles(p_lo, p_hi, s.window, s.sinks);
+
+  x8_t qf[DS];
+  const int qi = min(me.q0 + li, s.Sq - 1);  // rows past the end work on a copy of the last row and are not stored
+  win_load_row<T>(qf, static_cast<const T*>(a.q) + w.b * a.qs.batch + me.head * a.qs.head + qi * a.qs.token, s.dim, g);
+  const int p = me.p_lo + li;
+  const float scale2 = s.scale * kWinLog2e;
+
+  const T* K = static_cast<const T*>(a.k) + w.b * a.ks.batch + w.kvh * a.ks.head;
+  const T* V = static_cast<const T*>(a.v) + w.b * a.vs.batch + w.kvh * a.vs.head;
+  T* buffers = reinterpret_cast<T*>(attn_lds);  // two of K and V
+  auto request = [&](int i) {
+    const int t = tiles.at(i);
+    T* dst = buffers + (i & 1) * 2 * TILE;
+    win_copy<T, DH, kWinTile, kWinWaves>(K + static_cast<long long>(t) * kWinTile * a.ks.token, a.ks.token, length - t * kWinTile, s.dim, dst, wave, lane);
+    win_copy<T, DH, kWinTile, kWinWaves>(V + static_cast<long long>(t) * kWinTile * a.vs.token, a.vs.token, length - t * kWinTile, s.dim, dst + TILE, wave, lane);
+  };
+  int tr_off[DB];
+  win_tr_offsets<DH>(tr_off, lane);
+  float m = kWinFloor, l = 0.f;
+  request(0);
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  __syncthreads();
+  for (int i = 0; i < tiles.n; ++i) {
+    if (i + 1 < tiles.n) request(i + 1);
+    const int t = tiles.at(i);
+    if (me.active(t)) {
+      const T* Ks = buffers + (i & 1) * 2 * TILE;
+      const T* Vs = Ks + TILE;
+      f32x16_t sacc[2];
+      win_zero(sacc);
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int d = 0; d < DS; ++d) sacc[kb] = E::mfma(win_row_frag<T, DH>(Ks, 32 * kb + li, d, g), qf[d], sacc[kb]);
+      if (!me.whole(t)) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (!me.sees(p, t * kWinTile + 32 * kb + 8 * (r >> 2) + 4 * g + (r & 3))) sacc[kb][r] = -__builtin_inff();
+      }
+      float mx = kWinFloor;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sacc[kb][r] * scale2);
+      mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+      const float m_new = mx > m + kAttnSlack ? mx : m;
+      const float alpha = __builtin_amdgcn_exp2f(m - m_new);
+      m = m_new;
+      x8_t pf[4];
+      float sum = 0.f;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float e = __builtin_amdgcn_exp2f(fmaf(sacc[kb][r], scale2, -m));
+          sum += e;
+          pf[2 * kb + (r >> 3)][r & 7] = static_cast<T>(e);  // the product with V takes 16 bits; the sum keeps 32
+        }
+      l = fmaf(l, alpha, sum);
+      if (__any(alpha != 1.f)) {
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) oacc[db][r] *= alpha;
+      }
+#pragma unroll
+      for (int k4 = 0; k4 < 4; ++k4)
+#pragma unroll
+        for (int db = 0; db < DB; ++db) oacc[db] = E::mfma(win_tr_frag<T, DH>(Vs, tr_off[db], k4), pf[k4], oacc[db]);
+    }
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the next tile has landed
+    __syncthreads();
+  }
+  l += __shfl_xor(l, 32, kWave);
+  win_store<T, DH>(O, a.os.token, oacc, 1.0f / l, stage, lane, me.exist, me.rows, s.dim);
+  if (g == 0 && li < me.rows)
+    lse[li] = li < me.exist ? (m + __builtin_amdgcn_logf(l)) * kWinLn2 : -__builtin_inff();
+}
+
+}  // namespace mi

@@ -1,0 +1,420 @@
+// Gradients of window_attention.h.  With P = exp(S - lse) recomputed from the forward's row statistic, D = rowsum(dO * O)
+// and dS = P * (dO V^T - D) over the visible pairs:
+//     dV = P^T dO        dK = scale * dS^T Q        dQ = scale * dS K        (dK, dV summed over the heads of a group)
+//
+//   statistics  (lse log2 e, D) per row; a row that does not exist gets 1e30 and 0, which makes its P zero.
+//   dQ          blocks and key tiles of the forward: eight wavefronts of 32 queries of heads that share a key head.
+//   dK, dV      a wavefront owns 32 keys, a workgroup 256 of one key head, and walks the query tiles of 64 that see
+//               them through the window, head after head of the group.  The two gradients are separate halves of the
+//               launch: with both a wavefront's accumulators and operands outgrow the 256 registers it has at two
+//               wavefronts per SIMD.
+//   first keys  the keys j < sinks are also seen by every query beyond their window, hundreds of tiles for a few keys.
+//               That part is a kernel of its own: a workgroup takes 32 such keys and a share of those queries, each
+//               wavefront streams its own tiles of 32 queries, and the sums go to fp32 slots; the dK / dV kernel
+//               puts its part of these keys in slot 0 and a last kernel adds the slots in order and rounds once.
+// No atomics: results do not depend on the order of execution.
+#pragma once
+
+#include "window_attention.h"
+
+namespace mi {
+
+struct WindowBwdArgs {
+  const void *q, *k, *v, *o, *dout;
+  void *dq, *dk, *dv;
+  const float* lse;  // [B, N, Sq]
+  float* stats;      // [B, N, Sq, 2]
+  float* slots;      // [B * Nk][n_slots][2][sink_rows][DH] (dK without its scale, dV); null without such keys
+  WindowStride qs, ks, vs, os, dos, dqs, dks, dvs;
+  int n_slots, sink_rows;  // sink_rows: keys below `sinks`, rounded up to 32
+  WindowShape shape;
+};
+
+// ---- statistics: 16 lanes per row ----
+template <typename T>
+__device__ __forceinline__ void window_bwd_stats(const WindowBwdArgs& a) {
+  typedef typename AttnElem<T>::x8 x8_t;
+  const WindowShape& s = a.shape;
+  const long long rows = static_cast<long long>(s.batch) * s.heads * s.Sq;
+  const long long row = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 4;
+  const int part = threadIdx.x & 15;
+  float acc = 0.f;
+  bool exists = false;
+  if (row < rows) {
+    const int i = row % s.Sq, head = row / s.Sq % s.heads, b = row / s.Sq / s.heads;
+    exists = i < s.query_end(b);
+    if (exists && 8 * part < s.dim) {
+      const x8_t o = *reinterpret_cast<const x8_t*>(static_cast<const T*>(a.o) + b * a.os.batch + head * a.os.head + i * a.os.token + 8 * part);
+      const x8_t d = *reinterpret_cast<const x8_t*>(static_cast<const T*>(a.dout) + b * a.dos.batch + head * a.dos.head + i * a.dos.token + 8 * part);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc = fmaf(static_cast<float>(o[e]), static_cast<float>(d[e]), acc);
+    }
+  }
+  acc = wave_reduce<16>(acc, SumOp());
+  if (row < rows && part == 0) {
+    Vec<float, 2> st;
+    st[0] = exists ? a.lse[row] * kWinLog2e : 1e30f;
+    st[1] = exists ? acc : 0.f;
+    store_vec<float, 2>(a.stats + 2 * row, st);
+  }
+}
+
+// ---- dQ ----
+template <typename T, int DH>
+__device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
+  typedef AttnElem<T> E;
+  typedef typename E::x8 x8_t;
+  constexpr int DS = DH / 16, DB = DH / 32, TILE = kWinTile * DH;
+  extern __shared__ __attribute__((aligned(16))) unsigned char attn_lds[];
+  const WindowShape& s = a.shape;
+  const int lane = threadIdx.x & 63, li = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int per_block = kWinRows >> s.hb_shift;
+  const WindowBlock w = window_block(s, (s.Sq + per_block - 1) / per_block, s.group >> s.hb_shift);
+  if (!w.any) return;
+  const int length = s.length(w.b), query_end = s.query_end(w.b);
+  const WindowWave me = window_wave(s, w, wave, query_end);
+  T* dQ = static_cast<T*>(a.dq) + w.b * a.dqs.batch + me.head * a.dqs.head + me.q0 * a.dqs.token;
+  T* stage = reinterpret_cast<T*>(attn_lds) + wave * (32 * DH);
+  f32x16_t acc[DB];
+  win_zero(acc);
+  const int block_q0 = w.qb * per_block;
+  if (block_q0 >= query_end) {
+    win_store<T, DH>(dQ, a.dqs.token, acc, 0.f, stage, lane, 0, me.rows, s.dim);
+    return;
+  }
+  const WindowTiles tiles = window_tiles(block_q0 + s.offset(), min(block_q0 + per_block, query_end) - 1 + s.offset(), s.window, s.sinks);
+  const int qi = min(me.q0 + li, s.Sq - 1);
+  x8_t qf[DS], dof[DS];
+  win_load_row<T>(qf, static_cast<const T*>(a.q) + w.b * a.qs.batch + me.head * a.qs.head + qi * a.qs.token, s.dim, g);
+  win_load_row<T>(dof, static_cast<const T*>(a.dout) + w.b * a.dos.batch + me.head * a.dos.head + qi * a.dos.token, s.dim, g);
+  const Vec<float, 2> st = load_vec<float, 2>(a.stats + 2 * ((static_cast<size_t>(w.b) * s.heads + me.head) * s.Sq + qi));
+  const float m2 = st[0], delta = st[1];
+  const float c2 = s.scale * kWinLog2e;
+  const int p = me.p_lo + li;
+
+  const T* K = static_cast<const T*>(a.k) + w.b * a.ks.batch + w.kvh * a.ks.head;
+  const T* V = static_cast<const T*>(a.v) + w.b * a.vs.batch + w.kvh * a.vs.head;
+  T* buffers = reinterpret_cast<T*>(attn_lds);
+  auto request = [&](int i) {
+    const int t = tiles.at(i);
+    T* dst = buffers + (i & 1) * 2 * TILE;
+    win_copy<T, DH, kWinTile, kWinWaves>(K + static_cast<long long>(t) * kWinTile * a.ks.token, a.ks.token, length - t * kWinTile, s.dim, dst, wave, lane);
+    win_copy<T, DH, kWinTile, kWinWaves>(V + static_cast<long long>(t) * kWinTile * a.vs.token, a.vs.token, length - t * kWinTile, s.dim, dst + TILE, wave, lane);
+  };
+  int tr_off[DB];
+  win_tr_offsets<DH>(tr_off, lane);
+  auto compute = [&](int i, int t, auto mask_c) {
+    constexpr bool MASK = decltype(mask_c)::value;
+    const T* Ks = buffers + (i & 1) * 2 * TILE;
+    const T* Vs = Ks + TILE;
+    x8_t dsf[4];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      f32x16_t sp[2];
+      win_zero(sp);
+#pragma unroll
+      for (int d = 0; d < DS; ++d) {
+        sp[0] = E::mfma(win_row_frag<T, DH>(Ks, 32 * kb + li, d, g), qf[d], sp[0]);
+        sp[1] = E::mfma(win_row_frag<T, DH>(Vs, 32 * kb + li, d, g), dof[d], sp[1]);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float e = __builtin_amdgcn_exp2f(fmaf(sp[0][r], c2, -m2));
+        if (MASK && !me.sees(p, t * kWinTile + 32 * kb + 8 * (r >> 2) + 4 * g + (r & 3))) e = 0.f;
+        dsf[2 * kb + (r >> 3)][r & 7] = static_cast<T>(e * (sp[1][r] - delta));
+      }
+    }
+#pragma unroll
+    for (int k4 = 0; k4 < 4; ++k4)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) acc[db] = E::mfma(win_tr_frag<T, DH>(Ks, tr_off[db], k4), dsf[k4], acc[db]);
+  };
+  request(0);
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  __syncthreads();
+  for (int i = 0; i < tiles.n; ++i) {
+    if (i + 1 < tiles.n) request(i + 1);
+    const int t = tiles.at(i);
+    if (me.active(t)) {
+      if (me.whole(t))
+        compute(i, t, attn_flag<false>{});
+      else
+        compute(i, t, attn_flag<true>{});
+    }
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the next tile has landed
+    __syncthreads();
+  }
+  win_store<T, DH>(dQ, a.dqs.token, acc, s.scale, stage, lane, me.exist, me.rows, s.dim);
+}
+
+// ---- dK (WHICH = 0) and dV (WHICH = 1): the pairs inside the window ----
+template <typename T, int DH, int WHICH>
+__device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
+  constexpr bool DK = WHICH == 0;
+  typedef AttnElem<T> E;
+  typedef typename E::x8 x8_t;
+  constexpr int DS = DH / 16, DB = DH / 32, TILE = kWinTile * DH;
+  constexpr int BUF = 2 * TILE * 2 + kWinTile * 8;  // bytes: Q, dO, statistics of the tile
+  extern __shared__ __attribute__((aligned(16))) unsigned char attn_lds[];
+  const WindowShape& s = a.shape;
+  const int lane = threadIdx.x & 63, li = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const WindowBlock w = window_block(s, (s.Sk + kWinRows - 1) / kWinRows, 1);
+  if (!w.any) return;
+  const int length = s.length(w.b), query_end = s.query_end(w.b), off = s.offset();
+  const int k0 = w.qb * kWinRows, kw = k0 + 32 * wave;
+  const int exist = min(32, length - kw), rows = min(32, s.Sk - kw);
+  const WindowStride& ds = DK ? a.dks : a.dvs;
+  T* out = static_cast<T*>(DK ? a.dk : a.dv) + w.b * ds.batch + w.kvh * ds.head + kw * ds.token;
+  T* stage = reinterpret_cast<T*>(attn_lds) + wave * (32 * DH);
+  f32x16_t acc[DB];
+  win_zero(acc);
+
+  // query tiles that see a key of the block through the window
+  const int t_lo = max(0, k0 - off) / kWinTile;
+  const int q_last = min(query_end - 1, min(k0 + kWinRows, length) - 2 + s.window - off);
+  const int nt = k0 < length && q_last >= 0 ? max(0, q_last / kWinTile - t_lo + 1) : 0;
+  const int steps = nt * s.group;
+  const int kj = kw + li, kc = min(kj, s.Sk - 1);
+  x8_t kf[DS], vf[DK ? DS : 1];
+  win_load_row<T>(kf, static_cast<const T*>(a.k) + w.b * a.ks.batch + w.kvh * a.ks.head + kc * a.ks.token, s.dim, g);
+  if constexpr (DK) win_load_row<T>(vf, static_cast<const T*>(a.v) + w.b * a.vs.batch + w.kvh * a.vs.head + kc * a.vs.token, s.dim, g);
+  const float c2 = s.scale * kWinLog2e;
+  int tr_off[DB];
+  win_tr_offsets<DH>(tr_off, lane);
+
+  Vec<float, 2> sst;
+  int next_h = 0, next_t = t_lo;  // head of the group and query tile of the next request
+  auto request = [&](int i) {
+    const int head = w.kvh * s.group + next_h;
+    T* dst = reinterpret_cast<T*>(attn_lds + (i & 1) * BUF);
+    const long long q0 = static_cast<long long>(next_t) * kWinTile;
+    win_copy<T, DH, kWinTile, kWinWaves>(static_cast<const T*>(a.q) + w.b * a.qs.batch + head * a.qs.head + q0 * a.qs.token, a.qs.token,
+                                         query_end - static_cast<int>(q0), s.dim, dst, wave, lane);
+    win_copy<T, DH, kWinTile, kWinWaves>(static_cast<const T*>(a.dout) + w.b * a.dos.batch + head * a.dos.head + q0 * a.dos.token, a.dos.token,
+                                         query_end - static_cast<int>(q0), s.dim, dst + TILE, wave, lane);
+    if (threadIdx.x < kWinTile) {
+      const int q = static_cast<int>(q0) + threadIdx.x;
+      sst[0] = 1e30f;
+      sst[1] = 0.f;
+      if (q < s.Sq) sst = load_vec<float, 2>(a.stats + 2 * ((static_cast<size_t>(w.b) * s.heads + head) * s.Sq + q));
+    }
+    if (++next_t == t_lo + nt) {
+      next_t = t_lo;
+      ++next_h;
+    }
+  };
+  // the requested tile has landed and its statistics go behind it
+  auto finish = [&](int i) {
+    if (threadIdx.x < kWinTile) store_vec<float, 2>(reinterpret_cast<float*>(attn_lds + (i & 1) * BUF + 2 * TILE * 2) + 2 * threadIdx.x, sst);
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  };
+  auto compute = [&](int i, int t, auto mask_c) {
+    constexpr bool MASK = decltype(mask_c)::value;
+    const T* Qs = reinterpret_cast<const T*>(attn_lds + (i & 1) * BUF);
+    const T* dOs = Qs + TILE;
+    const float* st = reinterpret_cast<const float*>(dOs + TILE);
+    const int p0 = t * kWinTile + off;
+    x8_t bf[4];
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+      f32x16_t sp[DK ? 2 : 1];
+      win_zero(sp);
+#pragma unroll
+      for (int d = 0; d < DS; ++d) {
+        sp[0] = E::mfma(win_row_frag<T, DH>(Qs, 32 * qb + li, d, g), kf[d], sp[0]);
+        if constexpr (DK) sp[1] = E::mfma(win_row_frag<T, DH>(dOs, 32 * qb + li, d, g), vf[d], sp[1]);
+      }
+#pragma unroll
+      for (int rq = 0; rq < 4; ++rq) {
+        const int row = 32 * qb + 8 * rq + 4 * g;
+        const Vec<float, 4> sa = load_vec<float, 4>(st + 2 * row), sb = load_vec<float, 4>(st + 2 * row + 4);
+        const float m2[4] = {sa[0], sa[2], sb[0], sb[2]}, delta[4] = {sa[1], sa[3], sb[1], sb[3]};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * rq + e;
+          float x = __builtin_amdgcn_exp2f(fmaf(sp[0][r], c2, -m2[e]));
+          if (MASK && !(kj <= p0 + row + e && kj > p0 + row + e - s.window)) x = 0.f;
+          bf[2 * qb + (r >> 3)][r & 7] = static_cast<T>(DK ? x * (sp[DK ? 1 : 0][r] - delta[e]) : x);
+        }
+      }
+    }
+    const T* tr = DK ? Qs : dOs;
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) acc[db] = E::mfma(win_tr_frag<T, DH>(tr, tr_off[db], q4), bf[q4], acc[db]);
+  };
+
+  if (steps > 0) {
+    request(0);
+    finish(0);
+  }
+  __syncthreads();
+  int t = t_lo;
+  for (int i = 0; i < steps; ++i) {
+    if (i + 1 < steps) request(i + 1);
+    const int p0 = t * kWinTile + off;  // positions p0 .. p0 + 63
+    if (exist > 0 && p0 + kWinTile > kw && p0 < kw + 32 - 1 + s.window) {
+      if (p0 >= kw + 31 && p0 + kWinTile - 1 < kw + s.window)
+        compute(i, t, attn_flag<false>{});
+      else
+        compute(i, t, attn_flag<true>{});
+    }
+    if (i + 1 < steps) finish(i + 1);
+    __syncthreads();
+    if (++t == t_lo + nt) t = t_lo;
+  }
+  if (a.slots != nullptr && kw < a.sink_rows) {  // kw and sink_rows are multiples of 32
+    float* slot = a.slots + ((static_cast<size_t>(w.b * s.kv_heads + w.kvh) * a.n_slots) * 2 + WHICH) * a.sink_rows * DH;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int rq = 0; rq < 4; ++rq) {
+        Vec<float, 4> v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = li < exist ? acc[db][4 * rq + e] : 0.f;
+        store_vec<float, 4>(slot + static_cast<size_t>(kj) * DH + 32 * db + 8 * rq + 4 * g, v);
+      }
+  }
+  win_store<T, DH>(out, ds.token, acc, DK ? s.scale : 1.0f, stage, lane, exist, rows, s.dim);
+}
+
+// ---- dK and dV of the first keys from the queries beyond their window ----
+constexpr int kSinkWaves = 4;
+constexpr int kSinkTile = 32;  // queries of a tile
+
+template <typename T, int DH>
+__device__ __forceinline__ void window_bwd_sinks(const WindowBwdArgs& a) {
+  typedef AttnElem<T> E;
+  typedef typename E::x8 x8_t;
+  constexpr int DS = DH / 16, DB = DH / 32, TILE = kSinkTile * DH;
+  extern __shared__ __attribute__((aligned(16))) unsigned char attn_lds[];
+  const WindowShape& s = a.shape;
+  const int lane = threadIdx.x & 63, li = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // workgroups: [sequence and key head][32 keys][split]
+  const int splits = a.n_slots - 1, key_blocks = a.sink_rows / 32;
+  const int split = blockIdx.x % splits, rest = blockIdx.x / splits;
+  const int k0 = rest % key_blocks * 32, unit = rest / key_blocks;
+  const int b = unit / s.kv_heads, kvh = unit % s.kv_heads;
+  const int length = s.length(b), query_end = s.query_end(b), off = s.offset();
+  const int keys = min(min(s.sinks, length) - k0, 32);  // of these 32, the ones that exist and stay visible
+  const int t_lo = max(0, k0 + s.window - off) / kSinkTile;
+  const int nt = keys > 0 && query_end > 0 ? max(0, (query_end - 1) / kSinkTile - t_lo + 1) : 0;
+  const long long total = static_cast<long long>(nt) * s.group;
+  const int begin = static_cast<int>(total * split / splits), end = static_cast<int>(total * (split + 1) / splits);
+
+  const int kj = k0 + li, kc = min(kj, s.Sk - 1);
+  x8_t kf[DS], vf[DS];
+  win_load_row<T>(kf, static_cast<const T*>(a.k) + b * a.ks.batch + kvh * a.ks.head + kc * a.ks.token, s.dim, g);
+  win_load_row<T>(vf, static_cast<const T*>(a.v) + b * a.vs.batch + kvh * a.vs.head + kc * a.vs.token, s.dim, g);
+  const float c2 = s.scale * kWinLog2e;
+  int tr_off[DB];
+  win_tr_offsets<DH>(tr_off, lane);
+  f32x16_t dk[DB], dv[DB];
+  win_zero(dk);
+  win_zero(dv);
+  T* mine = reinterpret_cast<T*>(attn_lds) + wave * 4 * TILE;  // two buffers of Q and dO
+  auto request = [&](int i, int buf) {
+    const int head = kvh * s.group + i / nt;
+    const long long q0 = static_cast<long long>(t_lo + i % nt) * kSinkTile;
+    win_copy<T, DH, kSinkTile, 1>(static_cast<const T*>(a.q) + b * a.qs.batch + head * a.qs.head + q0 * a.qs.token, a.qs.token,
+                                  query_end - static_cast<int>(q0), s.dim, mine + buf * 2 * TILE, 0, lane);
+    win_copy<T, DH, kSinkTile, 1>(static_cast<const T*>(a.dout) + b * a.dos.batch + head * a.dos.head + q0 * a.dos.token, a.dos.token,
+                                  query_end - static_cast<int>(q0), s.dim, mine + buf * 2 * TILE + TILE, 0, lane);
+  };
+  int i = begin + wave;
+  if (i < end) request(i, 0);
+  for (int buf = 0; i < end; i += kSinkWaves, buf ^= 1) {
+    const int head = kvh * s.group + i / nt;
+    const int q0 = (t_lo + i % nt) * kSinkTile;
+    // statistics of the lane's sixteen rows, requested before the next tile's copies
+    float m2[16], delta[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int q = min(q0 + 8 * (r >> 2) + 4 * g + (r & 3), s.Sq - 1);
+      const Vec<float, 2> st = load_vec<float, 2>(a.stats + 2 * ((static_cast<size_t>(b) * s.heads + head) * s.Sq + q));
+      m2[r] = st[0];
+      delta[r] = st[1];
+    }
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this tile has landed
+    __builtin_amdgcn_sched_barrier(0);
+    if (i + kSinkWaves < end) request(i + kSinkWaves, buf ^ 1);
+    const T* Qs = mine + buf * 2 * TILE;
+    const T* dOs = Qs + TILE;
+    f32x16_t sp[2];
+    win_zero(sp);
+#pragma unroll
+    for (int d = 0; d < DS; ++d) {
+      sp[0] = E::mfma(win_row_frag<T, DH>(Qs, li, d, g), kf[d], sp[0]);
+      sp[1] = E::mfma(win_row_frag<T, DH>(dOs, li, d, g), vf[d], sp[1]);
+    }
+    x8_t pf[2], dsf[2];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int q = q0 + 8 * (r >> 2) + 4 * g + (r & 3);
+      float x = __builtin_amdgcn_exp2f(fmaf(sp[0][r], c2, -m2[r]));
+      if (!(q < query_end && q + off - kj >= s.window && li < keys)) x = 0.f;
+      pf[r >> 3][r & 7] = static_cast<T>(x);
+      dsf[r >> 3][r & 7] = static_cast<T>(x * (sp[1][r] - delta[r]));
+    }
+#pragma unroll
+    for (int q2 = 0; q2 < 2; ++q2)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        dv[db] = E::mfma(win_tr_frag<T, DH>(dOs, tr_off[db], q2), pf[q2], dv[db]);
+        dk[db] = E::mfma(win_tr_frag<T, DH>(Qs, tr_off[db], q2), dsf[q2], dk[db]);
+      }
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the reads of this buffer are done before it is refilled
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  // the four wavefronts' sums meet in LDS, [wave][dK, dV][key][DH]
+  __syncthreads();
+  float* all = reinterpret_cast<float*>(attn_lds);
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int rq = 0; rq < 4; ++rq) {
+      Vec<float, 4> x, y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = li < keys ? dk[db][4 * rq + e] : 0.f;
+        y[e] = li < keys ? dv[db][4 * rq + e] : 0.f;
+      }
+      const int at = li * DH + 32 * db + 8 * rq + 4 * g;
+      store_vec<float, 4>(all + wave * 64 * DH + at, x);
+      store_vec<float, 4>(all + wave * 64 * DH + 32 * DH + at, y);
+    }
+  __syncthreads();
+  float* slot = a.slots + (static_cast<size_t>(unit) * a.n_slots + 1 + split) * 2 * a.sink_rows * DH;
+  for (int j = threadIdx.x; j < 64 * DH; j += 64 * kSinkWaves) {
+    float sum = 0.f;
+#pragma unroll
+    for (int v = 0; v < kSinkWaves; ++v) sum += all[v * 64 * DH + j];
+    const int which = j / (32 * DH), in = j % (32 * DH);
+    slot[static_cast<size_t>(which) * a.sink_rows * DH + static_cast<size_t>(k0) * DH + in] = sum;
+  }
+}
+
+// Adds the slots of one key row (blockIdx: sequence and key head, key) in order: a thread per column, dK then dV.
+template <typename T, int DH>
+__device__ __forceinline__ void window_bwd_join(const WindowBwdArgs& a) {
+  const WindowShape& s = a.shape;
+  const int keys = min(s.sinks, s.Sk);
+  const int unit = blockIdx.x / keys, j = blockIdx.x % keys;
+  const int b = unit / s.kv_heads, kvh = unit % s.kv_heads;
+  const int which = threadIdx.x / DH, d = threadIdx.x % DH;
+  float sum = 0.f;
+  for (int n = 0; n < a.n_slots; ++n)
+    sum += a.slots[(((static_cast<size_t>(unit) * a.n_slots + n) * 2 + which) * a.sink_rows + j) * DH + d];
+  if (d < s.dim) {
+    if (which == 0)
+      static_cast<T*>(a.dk)[b * a.dks.batch + kvh * a.dks.head + j * a.dks.token + d] = static_cast<T>(sum * s.scale);
+    else
+      static_cast<T*>(a.dv)[b * a.dvs.batch + kvh * a.dvs.head + j * a.dvs.token + d] = static_cast<T>(sum);
+  }
+}
+
+}  // namespace mi

@@ -21,12 +21,22 @@ npu_def.define(
     "bool inverse=False) -> (Tensor, Tensor)"
 )
 npu_def.define(
+    "window_attention(Tensor q, Tensor k, Tensor v, float scale, int window, int sinks=0, Tensor? lengths=None) "
+    "-> (Tensor, Tensor)"
+)
+npu_def.define(
+    "window_attention_backward(Tensor q, Tensor k, Tensor v, Tensor out, Tensor dout, Tensor lse, float scale, "
+    "int window, int sinks=0, Tensor? lengths=None) -> (Tensor, Tensor, Tensor)"
+)
+npu_def.define(
     "window_attention_decode(Tensor q, Tensor k_cache, Tensor v_cache, Tensor lengths, float scale, int window, "
     "int sinks=0) -> Tensor"
 )
 
 gpu_lib.impl("add_rmsnorm_quant", kernels.add_rmsnorm_quant)
 gpu_lib.impl("rotary_axes", kernels.rotary_axes)
+gpu_lib.impl("window_attention", kernels.window_attention)
+gpu_lib.impl("window_attention_backward", kernels.window_attention_backward)
 gpu_lib.impl("window_attention_decode", kernels.window_attention_decode)
 
 
@@ -41,12 +51,22 @@ def _rotary_axes_meta(q, k, positions, inv_freq, sections=None, interleaved=Fals
     return torch.empty_like(q), torch.empty_like(k)
 
 
+def _window_attention_meta(q, k, v, scale, window, sinks=0, lengths=None):
+    return torch.empty_like(q), torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
+
+
+def _window_attention_backward_meta(q, k, v, out, dout, lse, scale, window, sinks=0, lengths=None):
+    return torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+
+
 def _window_attention_decode_meta(q, k_cache, v_cache, lengths, scale, window, sinks=0):
     return torch.empty(q.shape, dtype=q.dtype, device=q.device)
 
 
 meta_lib.impl("add_rmsnorm_quant", _add_rmsnorm_quant_meta)
 meta_lib.impl("rotary_axes", _rotary_axes_meta)
+meta_lib.impl("window_attention", _window_attention_meta)
+meta_lib.impl("window_attention_backward", _window_attention_backward_meta)
 meta_lib.impl("window_attention_decode", _window_attention_decode_meta)
 
 
@@ -59,13 +79,31 @@ def _rotary_context(ctx, inputs, output):
 def _rotary_backward(ctx, dq, dk):
     positions, inv_freq = ctx.saved_tensors
     sections, interleaved, inverse = ctx.form
-    # a rotation's gradient is the rotation back
+    # a rotation's gradient is the rotation back; a gradient may arrive in any layout (a sum's is one number everywhere)
     last = lambda t: t if t.stride(-1) == 1 else t.contiguous()  # noqa: E731
     gq, gk = torch.ops.npu_graph.rotary_axes(last(dq), last(dk), positions, inv_freq, sections, interleaved, not inverse)
     return gq, gk, None, None, None, None, None
 
 
+def _window_context(ctx, inputs, output):
+    q, k, v, scale, window, sinks, lengths = inputs
+    ctx.save_for_backward(q, k, v, output[0], output[1], lengths)
+    ctx.form = (scale, window, sinks)
+    ctx.mark_non_differentiable(output[1])
+
+
+def _window_backward(ctx, dout, _):
+    q, k, v, out, lse, lengths = ctx.saved_tensors
+    scale, window, sinks = ctx.form
+    rows = (dout.stride(i) for i in range(3) if dout.shape[i] > 1)
+    if dout.stride(3) != 1 or dout.data_ptr() % 16 or any(s % 8 for s in rows):
+        dout = dout.contiguous()
+    return (*torch.ops.npu_graph.window_attention_backward(q, k, v, out, dout, lse, scale, window, sinks, lengths),
+            None, None, None, None)
+
+
 register_autograd("npu_graph::rotary_axes", _rotary_backward, setup_context=_rotary_context)
+register_autograd("npu_graph::window_attention", _window_backward, setup_context=_window_context)
 
 
 def add_rmsnorm_quant(h: torch.Tensor, r: torch.Tensor, w: torch.Tensor, eps: float = 1e-6, group: int = 0):
@@ -77,6 +115,12 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_f
                 sections: Optional[Sequence[int]] = None, interleaved: bool = False, inverse: bool = False):
     """kernels.rotary_axes as a graph op with gradients for q and k."""
     return torch.ops.npu_graph.rotary_axes(q, k, positions, inv_freq, sections, interleaved, inverse)
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, window: int, sinks: int = 0,
+                     lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The output of kernels.window_attention as a graph op with gradients for q, k and v."""
+    return torch.ops.npu_graph.window_attention(q, k, v, scale, window, sinks, lengths)[0]
 
 
 def window_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,

@@ -957,6 +957,153 @@ def _check_lengths(lengths, t):
              "lengths must be a contiguous int32 vector with one value per sequence")
 
 
+def _largest_share(group: int) -> int:
+    """log2 of the query heads of a group that a workgroup's eight wavefronts work on together."""
+    return next(e for e in (3, 2, 1, 0) if group % (1 << e) == 0)
+
+
+_WINDOW_SHAPE = "P" + "i" * 11 + "f"  # WindowShape of csrc/mi/window_attention.h
+
+
+def _window_shape(q, k, lengths, window, sinks, scale):
+    """The WindowShape members for these operands."""
+    B, N, Sq, D = q.shape
+    Nk, Sk = k.shape[1:3]
+    # Where a die's eighth of the work is not whole key heads, its query blocks alternate between the long and the
+    # short end; windows that are short against the sequence make all blocks alike, which then keep their order
+    mixed = int((B * Nk) % 8 != 0 and 2 * window > Sk)
+    return (lengths.data_ptr() if lengths is not None else 0, B, N, Nk, N // Nk, Sq, Sk, D, window, sinks,
+            _largest_share(N // Nk), mixed, float(scale))
+
+
+def _window_grid(units: int, blocks: int) -> int:
+    return 8 * cdiv(units * blocks, 8)
+
+
+def _window_check(q, k, v, scale, window, sinks, lengths):
+    _check_here(q, k, v)
+    _require(q.dim() == 4, "q must be [B, N, Sq, D]")
+    dh, window, sinks = _window_operands(q, k, v, scale, window, sinks)
+    _require(q.shape[2] <= k.shape[2], "there cannot be more queries than keys")
+    _require(k.shape[2] < _WINDOW_LIMIT, "lengths must stay below 2**30")
+    _require(q.shape[0] * q.shape[1] * max(1, cdiv(k.shape[2], 32)) < 2**28, "too many heads and positions for one launch")
+    if lengths is not None:
+        _check_lengths(lengths, q)
+    return dh, window, sinks
+
+
+@functools.lru_cache(maxsize=None)
+def _window_fwd_launcher() -> CachingLauncher:
+    cfgs = [LaunchConfig(f"window_attention_fwd_{t}_d{d}", 512, lds_bytes=4 * 64 * d * 2) for t in _ATTN_DTYPES.values() for d in (64, 128)]
+    return CachingLauncher("window_attention_fwd", codecache.aot_source("window_attention_kernels.hip"),
+                           "PPPPP" + "q" * 12 + _WINDOW_SHAPE, cfgs, prefer_intree=True)
+
+
+def window_attention(
+    q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, window: int, sinks: int = 0,
+    lengths: Optional[torch.Tensor] = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Causal attention with a sliding window and first tokens that stay visible, heads may share keys: returns (out
+    [B, N, Sq, D], lse fp32 [B, N, Sq]) for q [B, N, Sq, D] and k, v [B, Nk, Sk, D] (bf16 or fp16, N a multiple of Nk,
+    Sq <= Sk, D a multiple of 8 up to 128; any strides with contiguous 16-byte aligned rows, so [B, S, N, D] tensors go in
+    as transposed views).
+
+    The queries are the last Sq of Sk positions; position p sees the keys j <= p with p - j < window or
+    j < sinks.  window >= Sk is plain causal attention.  lengths (int32 [B], on the device): positions from lengths[b] on
+    do not exist (a right-padded batch): their keys are hidden and not read, their rows of out are zero and
+    of lse -inf.  lse is the natural logarithm of the sum of exp(score * scale).
+    A NaN or infinity in an existing key or value row can also reach queries of the 63 positions before it, for
+    which it is hidden but lies in the same tile."""
+    dh, window, sinks = _window_check(q, k, v, scale, window, sinks, lengths)
+    B, N, Sq, D = q.shape
+    out = torch.empty_like(q)
+    lse = torch.empty((B, N, Sq), dtype=torch.float32, device=q.device)
+    if q.numel() == 0:
+        return out, lse
+    shape = _window_shape(q, k, lengths, window, sinks, scale)
+    blocks = cdiv(Sq, 256 >> shape[10]) * ((N // k.shape[1]) >> shape[10])
+    l = _window_fwd_launcher()
+    l._launch(
+        _find(l, f"window_attention_fwd_{_ATTN_DTYPES[q.dtype]}_d{dh}"),
+        (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+         *out.stride()[:3], *shape),
+        (_window_grid(B * k.shape[1], blocks), 1, 1), _stream(),
+    )
+    return out, lse
+
+
+@functools.lru_cache(maxsize=None)
+def _window_bwd_launchers() -> dict:
+    src = codecache.aot_source("window_attention_bwd_kernels.hip")
+    sig = "P" * 11 + "q" * 24 + "ii" + _WINDOW_SHAPE
+    types = tuple(_ATTN_DTYPES.values())
+    mk = lambda which, block, lds: CachingLauncher(  # noqa: E731
+        f"window_attention_bwd_{which}", src, sig,
+        [LaunchConfig(f"window_attention_bwd_{which}_{t}_d{d}", block(d), lds_bytes=lds(d)) for t in types for d in (64, 128)],
+        prefer_intree=True)
+    return {
+        "stats": CachingLauncher("window_attention_bwd_stats", src, sig,
+                                 [LaunchConfig(f"window_attention_bwd_stats_{t}", 256) for t in types], prefer_intree=True),
+        "dq": mk("dq", lambda d: 512, lambda d: 4 * 64 * d * 2),
+        "dkv": mk("dkv", lambda d: 512, lambda d: 2 * (2 * 64 * d * 2 + 512)),
+        "sinks": mk("sinks", lambda d: 256, lambda d: 4 * 4 * 32 * d * 2),
+        "join": mk("join", lambda d: 2 * d, lambda d: 0),
+    }
+
+
+def _sink_splits(units: int, key_blocks: int, tiles: int) -> int:
+    """Shares into which the queries that see the first keys from beyond their window are cut: two workgroups for
+    each compute unit, and four tiles of 32 queries for each of a workgroup's four wavefronts."""
+    return max(1, min(cdiv(2 * config.hardware().cu_count, units * key_blocks), tiles // 16))
+
+
+def window_attention_backward(
+    q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, dout: torch.Tensor, lse: torch.Tensor, scale: float,
+    window: int, sinks: int = 0, lengths: Optional[torch.Tensor] = None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Gradients (dq, dk, dv) of window_attention; out and lse are the forward's, dout [B, N, Sq, D] in the type of q
+    (strides as for q).  dk and dv are summed over the query heads that share a key head, in fp32 and in a fixed
+    order.  Rows that do not exist get zeros, and what dout holds there is not read into anything else."""
+    dh, window, sinks = _window_check(q, k, v, scale, window, sinks, lengths)
+    _check_here(q, out, dout, lse)
+    for t in (out, dout):
+        _require(t.shape == q.shape and t.dtype == q.dtype, "out and dout must match q")
+        _require(t.stride(-1) == 1 and _aligned(t) and all(x % 8 == 0 for x, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1),
+                 "columns must be contiguous, and rows 16-byte aligned")
+    B, N, Sq, D = q.shape
+    Nk, Sk = k.shape[1:3]
+    _require(lse.shape == (B, N, Sq) and lse.dtype == torch.float32 and lse.is_contiguous(), "lse must be the forward's [B, N, Sq] fp32")
+    _require(q.stride(2) < _STRIDE_LIMIT and dout.stride(2) < _STRIDE_LIMIT, "tokens lie too far apart")
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    if q.numel() == 0:
+        return dq, dk.zero_(), dv.zero_()
+    units, group = B * Nk, N // Nk
+    stats = torch.empty((B, N, Sq, 2), dtype=torch.float32, device=q.device)
+    # queries that see the first keys from beyond their window: those at positions >= window
+    far = min(sinks, Sk) if Sk > window else 0
+    sink_rows, n_slots, slots = 0, 0, None
+    if far:
+        sink_rows = 32 * cdiv(far, 32)
+        n_slots = 1 + _sink_splits(units, sink_rows // 32, group * cdiv(min(Sq, Sk - window), 32))
+        slots = torch.empty(units * n_slots * 2 * sink_rows * dh, dtype=torch.float32, device=q.device)
+    shape = _window_shape(q, k, lengths, window, sinks, scale)
+    args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+            lse.data_ptr(), stats.data_ptr(), slots.data_ptr() if slots is not None else 0,
+            *(x for t in (q, k, v, out, dout, dq, dk, dv) for x in t.stride()[:3]), n_slots, sink_rows, *shape)
+    ls, st, ty = _window_bwd_launchers(), _stream(), _ATTN_DTYPES[q.dtype]
+
+    def launch(which, name, grid):
+        ls[which]._launch(_find(ls[which], f"window_attention_bwd_{which}_{name}"), args, grid, st)
+
+    launch("stats", ty, (cdiv(B * N * Sq * 16, 256), 1, 1))
+    launch("dkv", f"{ty}_d{dh}", (_window_grid(units, cdiv(Sk, 256)), 2, 1))
+    if far:
+        launch("sinks", f"{ty}_d{dh}", (units * (sink_rows // 32) * (n_slots - 1), 1, 1))
+        launch("join", f"{ty}_d{dh}", (units * far, 1, 1))
+    launch("dq", f"{ty}_d{dh}", (_window_grid(units, cdiv(Sq, 256 >> shape[10]) * (group >> shape[10])), 1, 1))
+    return dq, dk, dv
+
+
 @functools.lru_cache(maxsize=None)
 def _window_decode_launchers() -> tuple[CachingLauncher, CachingLauncher]:
     src = codecache.aot_source("window_decode_kernels.hip")

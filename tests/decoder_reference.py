@@ -73,8 +73,9 @@ def attention(q, k, v, scale, window, sinks, lengths=None, dout=None):
                 slope = g @ vv.T
                 delta = (g * out[b, h]).sum(-1, keepdim=True)
                 ds = p * (slope - delta)
-                # what the kernels round: P to the operand type, dS to the operand type, O inside delta
-                ds_size = p * (slope.abs() + delta.abs() + (g.abs() * weight[b, h]).sum(-1, keepdim=True))
+                # what the kernels round: P (dV) and dS (dQ, dK) to the operand type, and O inside delta, which holds
+                # two roundings itself: the probabilities' and its own
+                ds_size = p * (slope.abs() + delta.abs() + 2 * (g.abs() * weight[b, h]).sum(-1, keepdim=True))
                 grads["dv"][b, h // G] += p.T @ g
                 grads["dv_weight"][b, h // G] += p.T @ g.abs()
                 grads["dq"][b, h] = ds @ kk * scale

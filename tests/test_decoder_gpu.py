@@ -257,3 +257,73 @@ def test_decode_captured_and_on_another_stream(K):
         other = call()
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(other, call())
+
+
+# ------------------------------------------------------------------------------------ prefill and training
+WINDOW_CASES = [
+    # B, N, Nk, Sq, Sk, D, window, sinks, lengths
+    (1, 1, 1, 1, 1, 8, 1, 0, None),
+    (2, 2, 1, 5, 5, 64, 3, 0, None),
+    (1, 2, 2, 64, 64, 128, 64, 0, None),
+    (2, 3, 1, 65, 65, 128, 1, 1, None),                # every query sees itself and the first key
+    (1, 8, 1, 130, 130, 64, 40, 4, None),              # eight heads in a workgroup
+    (2, 4, 2, 333, 333, 80, 100, 3, [333, 41]),
+    (3, 6, 2, 200, 200, 128, 64, 70, [1, 200, 130]),   # more first keys than a window
+    (1, 5, 1, 300, 300, 96, 2**31 - 1, 0, None),       # plain causal, an odd group
+    (1, 4, 1, 1, 700, 128, 256, 4, None),              # one query over a cache
+    (2, 8, 2, 37, 612, 128, 129, 33, [612, 590]),
+    (2, 2, 1, 100, 900, 64, 70, 4, [850, 700]),        # in the second sequence no query exists
+    (1, 4, 4, 700, 700, 128, 200, 2, None),
+    (1, 4, 2, 517, 1030, 128, 64, 128, None),
+    (1, 2, 1, 900, 900, 128, 300, 900, None),          # everything is a first key
+]
+
+
+def window_operands(B, N, Nk, Sq, Sk, D, dtype, token_major, seed=7):
+    gen = torch.Generator().manual_seed(seed)
+    q, dout = (caches(B, N, Sq, D, dtype, token_major, gen) for _ in range(2))
+    k, v = (caches(B, Nk, Sk, D, dtype, token_major, gen) for _ in range(2))
+    return q, k, v, dout
+
+
+def device_lengths(lengths):
+    return None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=DEV)
+
+
+def poison(t, first, lengths):
+    """NaN in every row that does not exist (row i of a sequence sits at position first + i)."""
+    for b, n in enumerate(lengths or []):
+        t[b, :, max(0, n - first):] = float("nan")
+
+
+def lse_bound(want):
+    # each term of the sum carries the error of its score, 6.2e-5 (attention_bound); log and exp add a few 2^-24
+    return 1e-4 + 4e-7 * want.abs()
+
+
+def check_window(K, case, dtype, token_major):
+    B, N, Nk, Sq, Sk, D, window, sinks, lengths = case
+    q, k, v, dout = window_operands(B, N, Nk, Sq, Sk, D, dtype, token_major)
+    want = R.attention(q, k, v, D**-0.5, window, sinks, lengths, dout)
+    poison(q, Sk - Sq, lengths), poison(dout, Sk - Sq, lengths), poison(k, 0, lengths), poison(v, 0, lengths)
+    dq_, k_, v_, do_ = (same_memory(t) for t in (q, k, v, dout))
+    ln = device_lengths(lengths)
+    out, lse = K.window_attention(dq_, k_, v_, D**-0.5, window, sinks, ln)
+    assert out.stride() == dq_.stride() and out.dtype == dtype and lse.dtype == torch.float32
+    within(out, want["out"], R.attention_bound(want["out"], want["weight"], dtype), "out")
+    none = torch.isinf(want["lse"])
+    assert torch.equal(torch.isinf(lse.cpu()), none) and (out.cpu()[none] == 0).all()
+    live = ~none
+    within(lse.cpu()[live], want["lse"][live], lse_bound(want["lse"][live]), "lse")
+    grads = K.window_attention_backward(dq_, k_, v_, out, do_, lse, D**-0.5, window, sinks, ln)
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        assert got.dtype == dtype
+        within(got, want[name], R.attention_bound(want[name], want[name + "_weight"], dtype), name)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("token_major", [False, True])
+@pytest.mark.parametrize("case", WINDOW_CASES, ids=str)
+def test_window_attention(K, case, token_major, dtype):
+    announce(f"window_attention {case} token_major={token_major} {dtype}")
+    check_window(K, case, dtype, token_major)
