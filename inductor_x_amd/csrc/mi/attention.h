@@ -110,7 +110,10 @@ struct AttnElem<bf16_t> {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
   static __device__ __forceinline__ x4 read_tr(const __bf16* p) {
-    return __builtin_bit_cast(x4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) x4v*)(p)));
+    return read_tr_lds((__attribute__((address_space(3))) x4v*)(p));
+  }
+  static __device__ __forceinline__ x4 read_tr_lds(__attribute__((address_space(3))) x4v* p) {
+    return __builtin_bit_cast(x4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16(p));
   }
 };
 template <>
@@ -123,7 +126,10 @@ struct AttnElem<f16_t> {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
   static __device__ __forceinline__ x4 read_tr(const _Float16* p) {
-    return __builtin_bit_cast(x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) x4v*)(p)));
+    return read_tr_lds((__attribute__((address_space(3))) x4v*)(p));
+  }
+  static __device__ __forceinline__ x4 read_tr_lds(__attribute__((address_space(3))) x4v* p) {
+    return __builtin_bit_cast(x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16(p));
   }
 };
 

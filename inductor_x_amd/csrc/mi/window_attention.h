@@ -91,27 +91,45 @@ __device__ __forceinline__ void win_copy(const T* src, long long stride, int row
   }
 }
 
-// A operand along the rows of a tile: row `row`, d slice s, half g
-template <typename T, int DH>
-__device__ __forceinline__ typename AttnElem<T>::x8 win_row_frag(const T* tile, int row, int s, int g) {
-  return *reinterpret_cast<const typename AttnElem<T>::x8*>(tile + row * DH + 8 * ((2 * s + g) ^ win_swz<DH>(row)));
-}
-// Per-lane offsets of the transposing reads, one per block of 32 columns: in every group of 16 lanes, lane s points at
-// four consecutive d of row 4 g + s / 4 (+ 8 for the second read) and receives, for its own d, the four rows.
-template <int DH, int DB>
-__device__ __forceinline__ void win_tr_offsets(int (&off)[DB], int lane) {
+// Fragment addresses.  With the swizzle, the place of a fragment is the lane's base with a constant XORed into its chunk
+// bits and a constant added above them: two registers address every fragment of every tile, where one register per
+// distinct fragment (which is what the compiler makes of loop-invariant addresses) pushed accumulators into scratch.
+// `win_bases` gives the bases for a buffer and keeps the compiler from hoisting what follows from them.
+struct WinBases {
+  uint32_t row, tr;
+};
+// `lds`: the kernel's dynamic LDS, in which the buffers start.
+template <int DH>
+__device__ __forceinline__ WinBases win_lane_bases(unsigned char* lds, int lane) {
+  const int li = lane & 31, g = lane >> 5;
   const int sl = lane & 15, grp = lane >> 4;
-  const int row = 4 * (grp >> 1) + (sl >> 2);
-  const int c = 2 * (grp & 1) + ((sl & 3) >> 1);
-#pragma unroll
-  for (int db = 0; db < DB; ++db) off[db] = row * DH + 8 * ((4 * db + c) ^ win_swz<DH>(row)) + 4 * (sl & 1);
+  const int tr_row = 4 * (grp >> 1) + (sl >> 2);
+  const int tr_chunk = 2 * (grp & 1) + ((sl & 3) >> 1);
+  const uint32_t start = (uint32_t)(__attribute__((address_space(3))) unsigned char*)lds;
+  WinBases b;
+  b.row = start + li * DH * 2 + 16 * (g ^ win_swz<DH>(li));
+  b.tr = start + tr_row * DH * 2 + 16 * (tr_chunk ^ win_swz<DH>(tr_row)) + 8 * (sl & 1);
+  return b;
 }
-// A operand across the rows (the tile transposed): columns of block db via its offset, row slice t of 16
+__device__ __forceinline__ WinBases win_bases(WinBases lane_bases, uint32_t buffer) {
+  WinBases b{lane_bases.row + buffer, lane_bases.tr + buffer};
+  asm volatile("" : "+v"(b.row), "+v"(b.tr));
+  return b;
+}
+// A operand along the rows: row 32 block + lane % 32, d slice s, half lane / 32, of the tile `at` bytes into the buffer
 template <typename T, int DH>
-__device__ __forceinline__ typename AttnElem<T>::x8 win_tr_frag(const T* tile, int off, int t) {
+__device__ __forceinline__ typename AttnElem<T>::x8 win_row_frag(const WinBases& b, int at, int block, int s) {
+  return *(const __attribute__((address_space(3))) typename AttnElem<T>::x8*)((b.row ^ (32 * s)) + at + 64 * DH * block);
+}
+// A operand across the rows (the tile transposed): columns 32 db + lane % 32, row slice t of 16.  In every group of 16
+// lanes, lane s points at four consecutive d of row 4 g + s / 4 (+ 8 for the second read) and receives, for its own d,
+// the four rows: the order in which the accumulators of the first product hold them.
+template <typename T, int DH>
+__device__ __forceinline__ typename AttnElem<T>::x8 win_tr_frag(const WinBases& b, int at, int db, int t) {
   typedef AttnElem<T> E;
-  const typename E::x4 lo = E::read_tr(tile + 16 * t * DH + off);
-  const typename E::x4 hi = E::read_tr(tile + (16 * t + 8) * DH + (off ^ (8 * win_swz<DH>(8))));
+  typedef __attribute__((address_space(3))) typename E::x4v lds_x4;
+  const typename E::x4 lo = E::read_tr_lds((lds_x4*)((b.tr ^ (64 * db)) + at + 32 * DH * t));
+  const typename E::x4 hi = E::read_tr_lds((lds_x4*)((b.tr ^ (64 * db) ^ (16 * win_swz<DH>(8))) + at + 32 * DH * t + 16 * DH));
   typename E::x8 r;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
@@ -281,8 +299,7 @@ __device__ __forceinline__ void window_attention_fwd(const WindowFwdArgs& a) {
     win_copy<T, DH, kWinTile, kWinWaves>(K + static_cast<long long>(t) * kWinTile * a.ks.token, a.ks.token, length - t * kWinTile, s.dim, dst, wave, lane);
     win_copy<T, DH, kWinTile, kWinWaves>(V + static_cast<long long>(t) * kWinTile * a.vs.token, a.vs.token, length - t * kWinTile, s.dim, dst + TILE, wave, lane);
   };
-  int tr_off[DB];
-  win_tr_offsets<DH>(tr_off, lane);
+  const WinBases lane_bases = win_lane_bases<DH>(attn_lds, lane);
   float m = kWinFloor, l = 0.f;
   request(0);
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
@@ -291,14 +308,13 @@ __device__ __forceinline__ void window_attention_fwd(const WindowFwdArgs& a) {
     if (i + 1 < tiles.n) request(i + 1);
     const int t = tiles.at(i);
     if (me.active(t)) {
-      const T* Ks = buffers + (i & 1) * 2 * TILE;
-      const T* Vs = Ks + TILE;
+      const WinBases at = win_bases(lane_bases, (i & 1) * 4 * TILE);
       f32x16_t sacc[2];
       win_zero(sacc);
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int d = 0; d < DS; ++d) sacc[kb] = E::mfma(win_row_frag<T, DH>(Ks, 32 * kb + li, d, g), qf[d], sacc[kb]);
+        for (int d = 0; d < DS; ++d) sacc[kb] = E::mfma(win_row_frag<T, DH>(at, 0, kb, d), qf[d], sacc[kb]);
       if (!me.whole(t)) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
@@ -335,7 +351,7 @@ __device__ __forceinline__ void window_attention_fwd(const WindowFwdArgs& a) {
 #pragma unroll
       for (int k4 = 0; k4 < 4; ++k4)
 #pragma unroll
-        for (int db = 0; db < DB; ++db) oacc[db] = E::mfma(win_tr_frag<T, DH>(Vs, tr_off[db], k4), pf[k4], oacc[db]);
+        for (int db = 0; db < DB; ++db) oacc[db] = E::mfma(win_tr_frag<T, DH>(at, 2 * TILE, db, k4), pf[k4], oacc[db]);
     }
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the next tile has landed
     __syncthreads();

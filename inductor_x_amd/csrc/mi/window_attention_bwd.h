@@ -2,7 +2,9 @@
 // and dS = P * (dO V^T - D) over the visible pairs:
 //     dV = P^T dO        dK = scale * dS^T Q        dQ = scale * dS K        (dK, dV summed over the heads of a group)
 //
-//   statistics  (lse log2 e, D) per row; a row that does not exist gets 1e30 and 0, which makes its P zero.
+//   statistics  -lse / scale and -D per row, the values the accumulators of Q K^T and dO V^T start from, so that
+//               P = exp2(S' scale log2 e) and dS = P dP' need no subtraction; a row that does not exist gets -1e30
+//               and 0, which makes its P zero.
 //   dQ          blocks and key tiles of the forward: eight wavefronts of 32 queries of heads that share a key head.
 //   dK, dV      a wavefront owns 32 keys, a workgroup 256 of one key head, and walks the query tiles of 64 that see
 //               them through the window, head after head of the group.  The two gradients are separate halves of the
@@ -23,7 +25,7 @@ struct WindowBwdArgs {
   const void *q, *k, *v, *o, *dout;
   void *dq, *dk, *dv;
   const float* lse;  // [B, N, Sq]
-  float* stats;      // [B, N, Sq, 2]
+  float* stats;      // [2][B, N, Sq]: -lse / scale, -D
   float* slots;      // [B * Nk][n_slots][2][sink_rows][DH] (dK without its scale, dV); null without such keys
   WindowStride qs, ks, vs, os, dos, dqs, dks, dvs;
   int n_slots, sink_rows;  // sink_rows: keys below `sinks`, rounded up to 32
@@ -52,10 +54,8 @@ __device__ __forceinline__ void window_bwd_stats(const WindowBwdArgs& a) {
   }
   acc = wave_reduce<16>(acc, SumOp());
   if (row < rows && part == 0) {
-    Vec<float, 2> st;
-    st[0] = exists ? a.lse[row] * kWinLog2e : 1e30f;
-    st[1] = exists ? acc : 0.f;
-    store_vec<float, 2>(a.stats + 2 * row, st);
+    a.stats[row] = exists ? -a.lse[row] / s.scale : -1e30f;
+    a.stats[rows + row] = exists ? -acc : 0.f;
   }
 }
 
@@ -88,9 +88,9 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
   x8_t qf[DS], dof[DS];
   win_load_row<T>(qf, static_cast<const T*>(a.q) + w.b * a.qs.batch + me.head * a.qs.head + qi * a.qs.token, s.dim, g);
   win_load_row<T>(dof, static_cast<const T*>(a.dout) + w.b * a.dos.batch + me.head * a.dos.head + qi * a.dos.token, s.dim, g);
-  const Vec<float, 2> st = load_vec<float, 2>(a.stats + 2 * ((static_cast<size_t>(w.b) * s.heads + me.head) * s.Sq + qi));
-  const float m2 = st[0], delta = st[1];
   const float c2 = s.scale * kWinLog2e;
+  const float* st = a.stats + (static_cast<size_t>(w.b) * s.heads + me.head) * s.Sq + qi;
+  const float m2 = st[0] * c2, delta = st[static_cast<size_t>(s.batch) * s.heads * s.Sq];
   const int p = me.p_lo + li;
 
   const T* K = static_cast<const T*>(a.k) + w.b * a.ks.batch + w.kvh * a.ks.head;
@@ -102,12 +102,10 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
     win_copy<T, DH, kWinTile, kWinWaves>(K + static_cast<long long>(t) * kWinTile * a.ks.token, a.ks.token, length - t * kWinTile, s.dim, dst, wave, lane);
     win_copy<T, DH, kWinTile, kWinWaves>(V + static_cast<long long>(t) * kWinTile * a.vs.token, a.vs.token, length - t * kWinTile, s.dim, dst + TILE, wave, lane);
   };
-  int tr_off[DB];
-  win_tr_offsets<DH>(tr_off, lane);
+  const WinBases lane_bases = win_lane_bases<DH>(attn_lds, lane);
   auto compute = [&](int i, int t, auto mask_c) {
     constexpr bool MASK = decltype(mask_c)::value;
-    const T* Ks = buffers + (i & 1) * 2 * TILE;
-    const T* Vs = Ks + TILE;
+    const WinBases at = win_bases(lane_bases, (i & 1) * 4 * TILE);
     x8_t dsf[4];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
@@ -115,20 +113,20 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
       win_zero(sp);
 #pragma unroll
       for (int d = 0; d < DS; ++d) {
-        sp[0] = E::mfma(win_row_frag<T, DH>(Ks, 32 * kb + li, d, g), qf[d], sp[0]);
-        sp[1] = E::mfma(win_row_frag<T, DH>(Vs, 32 * kb + li, d, g), dof[d], sp[1]);
+        sp[0] = E::mfma(win_row_frag<T, DH>(at, 0, kb, d), qf[d], sp[0]);
+        sp[1] = E::mfma(win_row_frag<T, DH>(at, 2 * TILE, kb, d), dof[d], sp[1]);
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        float e = __builtin_amdgcn_exp2f(fmaf(sp[0][r], c2, -m2));
+        float e = __builtin_amdgcn_exp2f(fmaf(sp[0][r], c2, m2));
         if (MASK && !me.sees(p, t * kWinTile + 32 * kb + 8 * (r >> 2) + 4 * g + (r & 3))) e = 0.f;
-        dsf[2 * kb + (r >> 3)][r & 7] = static_cast<T>(e * (sp[1][r] - delta));
+        dsf[2 * kb + (r >> 3)][r & 7] = static_cast<T>(e * (sp[1][r] + delta));
       }
     }
 #pragma unroll
     for (int k4 = 0; k4 < 4; ++k4)
 #pragma unroll
-      for (int db = 0; db < DB; ++db) acc[db] = E::mfma(win_tr_frag<T, DH>(Ks, tr_off[db], k4), dsf[k4], acc[db]);
+      for (int db = 0; db < DB; ++db) acc[db] = E::mfma(win_tr_frag<T, DH>(at, 0, db, k4), dsf[k4], acc[db]);
   };
   request(0);
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
@@ -149,6 +147,8 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
 }
 
 // ---- dK (WHICH = 0) and dV (WHICH = 1): the pairs inside the window ----
+constexpr int kAhead = 2;  // matrix steps between an LDS fragment's read and its use
+
 template <typename T, int DH, int WHICH>
 __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
   constexpr bool DK = WHICH == 0;
@@ -181,10 +181,9 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
   win_load_row<T>(kf, static_cast<const T*>(a.k) + w.b * a.ks.batch + w.kvh * a.ks.head + kc * a.ks.token, s.dim, g);
   if constexpr (DK) win_load_row<T>(vf, static_cast<const T*>(a.v) + w.b * a.vs.batch + w.kvh * a.vs.head + kc * a.vs.token, s.dim, g);
   const float c2 = s.scale * kWinLog2e;
-  int tr_off[DB];
-  win_tr_offsets<DH>(tr_off, lane);
+  const WinBases lane_bases = win_lane_bases<DH>(attn_lds, lane);
 
-  Vec<float, 2> sst;
+  float sst;
   int next_h = 0, next_t = t_lo;  // head of the group and query tile of the next request
   auto request = [&](int i) {
     const int head = w.kvh * s.group + next_h;
@@ -194,11 +193,10 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
                                          query_end - static_cast<int>(q0), s.dim, dst, wave, lane);
     win_copy<T, DH, kWinTile, kWinWaves>(static_cast<const T*>(a.dout) + w.b * a.dos.batch + head * a.dos.head + q0 * a.dos.token, a.dos.token,
                                          query_end - static_cast<int>(q0), s.dim, dst + TILE, wave, lane);
-    if (threadIdx.x < kWinTile) {
-      const int q = static_cast<int>(q0) + threadIdx.x;
-      sst[0] = 1e30f;
-      sst[1] = 0.f;
-      if (q < s.Sq) sst = load_vec<float, 2>(a.stats + 2 * ((static_cast<size_t>(w.b) * s.heads + head) * s.Sq + q));
+    if (threadIdx.x < 2 * kWinTile) {  // the first wavefront fetches -lse / scale of the 64 rows, the second -D
+      const int q = static_cast<int>(q0) + lane;
+      sst = wave == 0 ? -1e30f : 0.f;
+      if (q < s.Sq) sst = a.stats[((static_cast<size_t>(wave) * s.batch + w.b) * s.heads + head) * s.Sq + q];
     }
     if (++next_t == t_lo + nt) {
       next_t = t_lo;
@@ -207,44 +205,69 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
   };
   // the requested tile has landed and its statistics go behind it
   auto finish = [&](int i) {
-    if (threadIdx.x < kWinTile) store_vec<float, 2>(reinterpret_cast<float*>(attn_lds + (i & 1) * BUF + 2 * TILE * 2) + 2 * threadIdx.x, sst);
+    if (threadIdx.x < 2 * kWinTile) reinterpret_cast<float*>(attn_lds + (i & 1) * BUF + 4 * TILE)[threadIdx.x] = sst;
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   };
-  auto compute = [&](int i, int t, auto mask_c) {
-    constexpr bool MASK = decltype(mask_c)::value;
-    const T* Qs = reinterpret_cast<const T*>(attn_lds + (i & 1) * BUF);
-    const T* dOs = Qs + TILE;
-    const float* st = reinterpret_cast<const float*>(dOs + TILE);
+  // One tile.  Its matrix steps (per query block the d slices of S and dP, then the updates) read their LDS fragments
+  // kAhead steps ahead, across the phases, with the order pinned by scheduling fences; `whole`: no pair is hidden.
+  auto compute = [&](int i, int t, bool whole) {
+    constexpr int N1 = 2 * DS, N2 = 4 * DB;
+    const WinBases at = win_bases(lane_bases, (i & 1) * BUF);
+    const float* st = reinterpret_cast<const float*>(attn_lds + (i & 1) * BUF + 4 * TILE);
     const int p0 = t * kWinTile + off;
-    x8_t bf[4];
-#pragma unroll
-    for (int qb = 0; qb < 2; ++qb) {
-      f32x16_t sp[DK ? 2 : 1];
-      win_zero(sp);
-#pragma unroll
-      for (int d = 0; d < DS; ++d) {
-        sp[0] = E::mfma(win_row_frag<T, DH>(Qs, 32 * qb + li, d, g), kf[d], sp[0]);
-        if constexpr (DK) sp[1] = E::mfma(win_row_frag<T, DH>(dOs, 32 * qb + li, d, g), vf[d], sp[1]);
+    x8_t bf[4], qa[N1], da[DK ? N1 : 1], ta[N2];
+    auto issue = [&](auto ic) {
+      constexpr int n = decltype(ic)::value;
+      if constexpr (n < N1) {
+        qa[n] = win_row_frag<T, DH>(at, 0, n / DS, n % DS);
+        if constexpr (DK) da[n] = win_row_frag<T, DH>(at, 2 * TILE, n / DS, n % DS);
+      } else if constexpr (n < N1 + N2) {
+        ta[n - N1] = win_tr_frag<T, DH>(at, DK ? 0 : 2 * TILE, (n - N1) % DB, (n - N1) / DB);
       }
+    };
+    static_for<kAhead>([&](auto ic) { issue(ic); });
+    f32x16_t sp[DK ? 2 : 1];
+    static_for<N1 + N2>([&](auto ic) {
+      constexpr int n = decltype(ic)::value;
+      issue(std::integral_constant<int, n + kAhead>{});
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (n < N1) {
+        constexpr int qb = n / DS, d = n % DS;
+        if constexpr (d == 0) {
 #pragma unroll
-      for (int rq = 0; rq < 4; ++rq) {
-        const int row = 32 * qb + 8 * rq + 4 * g;
-        const Vec<float, 4> sa = load_vec<float, 4>(st + 2 * row), sb = load_vec<float, 4>(st + 2 * row + 4);
-        const float m2[4] = {sa[0], sa[2], sb[0], sb[2]}, delta[4] = {sa[1], sa[3], sb[1], sb[3]};
+          for (int k = 0; k < (DK ? 2 : 1); ++k)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 4 * rq + e;
-          float x = __builtin_amdgcn_exp2f(fmaf(sp[0][r], c2, -m2[e]));
-          if (MASK && !(kj <= p0 + row + e && kj > p0 + row + e - s.window)) x = 0.f;
-          bf[2 * qb + (r >> 3)][r & 7] = static_cast<T>(DK ? x * (sp[DK ? 1 : 0][r] - delta[e]) : x);
+            for (int rq = 0; rq < 4; ++rq) {
+              const Vec<float, 4> v = load_vec<float, 4>(st + k * kWinTile + 32 * qb + 8 * rq + 4 * g);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sp[k][4 * rq + e] = v[e];
+            }
         }
+        sp[0] = E::mfma(qa[n], kf[d], sp[0]);
+        if constexpr (DK) sp[1] = E::mfma(da[n], vf[d], sp[1]);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (d == DS - 1) {
+          if (!whole) {
+            const int d0 = kj - (p0 + 32 * qb + 4 * g);  // row r sees the key if d0 <= its offset < d0 + window
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int o = 8 * (r >> 2) + (r & 3);
+              if (o < d0 || o - s.window >= d0) sp[0][r] = -__builtin_inff();
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float x = __builtin_amdgcn_exp2f(sp[0][r] * c2);
+            bf[2 * qb + (r >> 3)][r & 7] = static_cast<T>(DK ? x * sp[DK ? 1 : 0][r] : x);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+        constexpr int j = n - N1;
+        acc[j % DB] = E::mfma(ta[j], bf[j / DB], acc[j % DB]);
+        __builtin_amdgcn_sched_barrier(0);
       }
-    }
-    const T* tr = DK ? Qs : dOs;
-#pragma unroll
-    for (int q4 = 0; q4 < 4; ++q4)
-#pragma unroll
-      for (int db = 0; db < DB; ++db) acc[db] = E::mfma(win_tr_frag<T, DH>(tr, tr_off[db], q4), bf[q4], acc[db]);
+    });
   };
 
   if (steps > 0) {
@@ -256,12 +279,8 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
   for (int i = 0; i < steps; ++i) {
     if (i + 1 < steps) request(i + 1);
     const int p0 = t * kWinTile + off;  // positions p0 .. p0 + 63
-    if (exist > 0 && p0 + kWinTile > kw && p0 < kw + 32 - 1 + s.window) {
-      if (p0 >= kw + 31 && p0 + kWinTile - 1 < kw + s.window)
-        compute(i, t, attn_flag<false>{});
-      else
-        compute(i, t, attn_flag<true>{});
-    }
+    if (exist > 0 && p0 + kWinTile > kw && p0 < kw + 32 - 1 + s.window)
+      compute(i, t, p0 >= kw + 31 && p0 + kWinTile - 1 < kw + s.window);
     if (i + 1 < steps) finish(i + 1);
     __syncthreads();
     if (++t == t_lo + nt) t = t_lo;
@@ -311,8 +330,7 @@ __device__ __forceinline__ void window_bwd_sinks(const WindowBwdArgs& a) {
   win_load_row<T>(kf, static_cast<const T*>(a.k) + b * a.ks.batch + kvh * a.ks.head + kc * a.ks.token, s.dim, g);
   win_load_row<T>(vf, static_cast<const T*>(a.v) + b * a.vs.batch + kvh * a.vs.head + kc * a.vs.token, s.dim, g);
   const float c2 = s.scale * kWinLog2e;
-  int tr_off[DB];
-  win_tr_offsets<DH>(tr_off, lane);
+  const WinBases lane_bases = win_lane_bases<DH>(attn_lds, lane);
   f32x16_t dk[DB], dv[DB];
   win_zero(dk);
   win_zero(dv);
@@ -331,41 +349,37 @@ __device__ __forceinline__ void window_bwd_sinks(const WindowBwdArgs& a) {
     const int head = kvh * s.group + i / nt;
     const int q0 = (t_lo + i % nt) * kSinkTile;
     // statistics of the lane's sixteen rows, requested before the next tile's copies
-    float m2[16], delta[16];
+    f32x16_t sp[2];
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int q = min(q0 + 8 * (r >> 2) + 4 * g + (r & 3), s.Sq - 1);
-      const Vec<float, 2> st = load_vec<float, 2>(a.stats + 2 * ((static_cast<size_t>(b) * s.heads + head) * s.Sq + q));
-      m2[r] = st[0];
-      delta[r] = st[1];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) sp[k][r] = a.stats[((static_cast<size_t>(k) * s.batch + b) * s.heads + head) * s.Sq + q];
     }
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this tile has landed
     __builtin_amdgcn_sched_barrier(0);
     if (i + kSinkWaves < end) request(i + kSinkWaves, buf ^ 1);
-    const T* Qs = mine + buf * 2 * TILE;
-    const T* dOs = Qs + TILE;
-    f32x16_t sp[2];
-    win_zero(sp);
+    const WinBases at = win_bases(lane_bases, (wave * 4 + buf * 2) * TILE * 2);
 #pragma unroll
     for (int d = 0; d < DS; ++d) {
-      sp[0] = E::mfma(win_row_frag<T, DH>(Qs, li, d, g), kf[d], sp[0]);
-      sp[1] = E::mfma(win_row_frag<T, DH>(dOs, li, d, g), vf[d], sp[1]);
+      sp[0] = E::mfma(win_row_frag<T, DH>(at, 0, 0, d), kf[d], sp[0]);
+      sp[1] = E::mfma(win_row_frag<T, DH>(at, 2 * TILE, 0, d), vf[d], sp[1]);
     }
     x8_t pf[2], dsf[2];
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int q = q0 + 8 * (r >> 2) + 4 * g + (r & 3);
-      float x = __builtin_amdgcn_exp2f(fmaf(sp[0][r], c2, -m2[r]));
+      float x = __builtin_amdgcn_exp2f(sp[0][r] * c2);
       if (!(q < query_end && q + off - kj >= s.window && li < keys)) x = 0.f;
       pf[r >> 3][r & 7] = static_cast<T>(x);
-      dsf[r >> 3][r & 7] = static_cast<T>(x * (sp[1][r] - delta[r]));
+      dsf[r >> 3][r & 7] = static_cast<T>(x * sp[1][r]);
     }
 #pragma unroll
     for (int q2 = 0; q2 < 2; ++q2)
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
-        dv[db] = E::mfma(win_tr_frag<T, DH>(dOs, tr_off[db], q2), pf[q2], dv[db]);
-        dk[db] = E::mfma(win_tr_frag<T, DH>(Qs, tr_off[db], q2), dsf[q2], dk[db]);
+        dv[db] = E::mfma(win_tr_frag<T, DH>(at, 2 * TILE, db, q2), pf[q2], dv[db]);
+        dk[db] = E::mfma(win_tr_frag<T, DH>(at, 0, db, q2), dsf[q2], dk[db]);
       }
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the reads of this buffer are done before it is refilled
     __builtin_amdgcn_sched_barrier(0);

@@ -1078,7 +1078,7 @@ def window_attention_backward(
     if q.numel() == 0:
         return dq, dk.zero_(), dv.zero_()
     units, group = B * Nk, N // Nk
-    stats = torch.empty((B, N, Sq, 2), dtype=torch.float32, device=q.device)
+    stats = torch.empty((2, B, N, Sq), dtype=torch.float32, device=q.device)
     # queries that see the first keys from beyond their window: those at positions >= window
     far = min(sinks, Sk) if Sk > window else 0
     sink_rows, n_slots, slots = 0, 0, None
