@@ -20,12 +20,8 @@ using namespace mi;
   extern "C" __global__ __launch_bounds__(2 * DH) void window_attention_bwd_join_##TN##_d##DH(WindowBwdArgs args) { \
     window_bwd_join<T, DH>(args);                                                                                   \
   }
-#define WINDOW_BWD_TYPE(TN, T)                                                                                      \
-  extern "C" __global__ __launch_bounds__(256) void window_attention_bwd_stats_##TN(WindowBwdArgs args) {           \
-    window_bwd_stats<T>(args);                                                                                      \
-  }                                                                                                                 \
-  WINDOW_BWD(TN, T, 64)                                                                                             \
-  WINDOW_BWD(TN, T, 128)
 
-WINDOW_BWD_TYPE(bf16, bf16_t)
-WINDOW_BWD_TYPE(f16, f16_t)
+WINDOW_BWD(bf16, bf16_t, 64)
+WINDOW_BWD(bf16, bf16_t, 128)
+WINDOW_BWD(f16, f16_t, 64)
+WINDOW_BWD(f16, f16_t, 128)

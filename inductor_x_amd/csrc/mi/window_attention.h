@@ -164,8 +164,8 @@ __device__ __forceinline__ void win_zero(f32x16_t (&acc)[DB]) {
 
 // Transposed accumulators (lane = row, registers = columns) of a wavefront's 32 rows -> memory, through the
 // wavefront's own 32 x DH piece of LDS so that whole rows leave.  Rows below `exist` get the values times the lane's
-// factor, those from there to `rows` zeros.
-template <typename T, int DH, int DB>
+// factor, those from there to `rows` zeros.  REMAINDER stores what the rounding of that value lost instead.
+template <typename T, int DH, bool REMAINDER = false, int DB>
 __device__ __forceinline__ void win_store(T* dst, long long stride, const f32x16_t (&acc)[DB], float factor, T* stage,
                                           int lane, int exist, int rows, int dim) {
   typedef typename AttnElem<T>::x4 x4_t;
@@ -177,7 +177,13 @@ __device__ __forceinline__ void win_store(T* dst, long long stride, const f32x16
     for (int rq = 0; rq < 4; ++rq) {
       x4_t o4;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o4[e] = static_cast<T>(li < exist ? acc[db][4 * rq + e] * factor : 0.f);
+      for (int e = 0; e < 4; ++e) {
+        float x = li < exist ? acc[db][4 * rq + e] * factor : 0.f;
+        // the product is rounded to fp32 here: fused into a conversion or the subtraction it would round another
+        // way near a tie, and value and remainder would not belong together
+        asm volatile("" : "+v"(x));
+        o4[e] = static_cast<T>(REMAINDER ? x - static_cast<float>(static_cast<T>(x)) : x);
+      }
       *reinterpret_cast<x4_t*>(stage + li * DH + 8 * ((4 * db + rq) ^ (li % CH)) + 4 * g) = o4;
     }
   const int c = lane % CH;
@@ -250,6 +256,7 @@ __device__ __forceinline__ WindowWave window_wave(const WindowShape& s, const Wi
 struct WindowFwdArgs {
   const void *q, *k, *v;
   void* o;
+  void* low;   // may be null: what rounding o lost, laid out like o
   float* lse;  // [B, N, Sq]
   WindowStride qs, ks, vs, os;
   WindowShape shape;
@@ -269,7 +276,8 @@ __device__ __forceinline__ void window_attention_fwd(const WindowFwdArgs& a) {
   if (!w.any) return;
   const int length = s.length(w.b), query_end = s.query_end(w.b);
   const WindowWave me = window_wave(s, w, wave, query_end);
-  T* O = static_cast<T*>(a.o) + w.b * a.os.batch + me.head * a.os.head + me.q0 * a.os.token;
+  const long long o_at = w.b * a.os.batch + me.head * a.os.head + me.q0 * a.os.token;
+  T* O = static_cast<T*>(a.o) + o_at;
   float* lse = a.lse + (static_cast<size_t>(w.b) * s.heads + me.head) * s.Sq + me.q0;
   T* stage = reinterpret_cast<T*>(attn_lds) + wave * (32 * DH);
   f32x16_t oacc[DB];
@@ -277,6 +285,7 @@ __device__ __forceinline__ void window_attention_fwd(const WindowFwdArgs& a) {
   const int block_q0 = w.qb * per_block;
   if (block_q0 >= query_end) {  // nothing here exists
     win_store<T, DH>(O, a.os.token, oacc, 0.f, stage, lane, 0, me.rows, s.dim);
+    if (a.low != nullptr) win_store<T, DH>(static_cast<T*>(a.low) + o_at, a.os.token, oacc, 0.f, stage, lane, 0, me.rows, s.dim);
     if (g == 0 && li < me.rows) lse[li] = -__builtin_inff();
     return;
   }
@@ -358,6 +367,8 @@ __device__ __forceinline__ void window_attention_fwd(const WindowFwdArgs& a) {
   }
   l += __shfl_xor(l, 32, kWave);
   win_store<T, DH>(O, a.os.token, oacc, 1.0f / l, stage, lane, me.exist, me.rows, s.dim);
+  if (a.low != nullptr)
+    win_store<T, DH, true>(static_cast<T*>(a.low) + o_at, a.os.token, oacc, 1.0f / l, stage, lane, me.exist, me.rows, s.dim);
   if (g == 0 && li < me.rows)
     lse[li] = li < me.exist ? (m + __builtin_amdgcn_logf(l)) * kWinLn2 : -__builtin_inff();
 }

@@ -2,10 +2,12 @@
 // and dS = P * (dO V^T - D) over the visible pairs:
 //     dV = P^T dO        dK = scale * dS^T Q        dQ = scale * dS K        (dK, dV summed over the heads of a group)
 //
-//   statistics  -lse / scale and -D per row, the values the accumulators of Q K^T and dO V^T start from, so that
-//               P = exp2(S' scale log2 e) and dS = P dP' need no subtraction; a row that does not exist gets -1e30
-//               and 0, which makes its P zero.
-//   dQ          blocks and key tiles of the forward: eight wavefronts of 32 queries of heads that share a key head.
+//   dQ          blocks and key tiles of the forward: eight wavefronts of 32 queries of heads that share a key head.  It
+//               also forms the row statistics -lse / scale and -D, the values that the accumulators of Q K^T and
+//               dO V^T start from in the kernels after it, so that P = exp2(S' scale log2 e) and dS = P dP' need no
+//               subtraction there; a row that does not exist gets -1e30 and 0, which makes its P zero.
+//               D takes O with what its rounding lost, where the forward kept that: in rows that see few keys
+//               dO V^T and D nearly cancel, and the rounding of O would be the largest error of dS.
 //   dK, dV      a wavefront owns 32 keys, a workgroup 256 of one key head, and walks the query tiles of 64 that see
 //               them through the window, head after head of the group.  The two gradients are separate halves of the
 //               launch: with both a wavefront's accumulators and operands outgrow the 256 registers it has at two
@@ -22,7 +24,7 @@
 namespace mi {
 
 struct WindowBwdArgs {
-  const void *q, *k, *v, *o, *dout;
+  const void *q, *k, *v, *o, *low, *dout;  // low may be null
   void *dq, *dk, *dv;
   const float* lse;  // [B, N, Sq]
   float* stats;      // [2][B, N, Sq]: -lse / scale, -D
@@ -32,34 +34,9 @@ struct WindowBwdArgs {
   WindowShape shape;
 };
 
-// ---- statistics: 16 lanes per row ----
-template <typename T>
-__device__ __forceinline__ void window_bwd_stats(const WindowBwdArgs& a) {
-  typedef typename AttnElem<T>::x8 x8_t;
-  const WindowShape& s = a.shape;
-  const long long rows = static_cast<long long>(s.batch) * s.heads * s.Sq;
-  const long long row = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 4;
-  const int part = threadIdx.x & 15;
-  float acc = 0.f;
-  bool exists = false;
-  if (row < rows) {
-    const int i = row % s.Sq, head = row / s.Sq % s.heads, b = row / s.Sq / s.heads;
-    exists = i < s.query_end(b);
-    if (exists && 8 * part < s.dim) {
-      const x8_t o = *reinterpret_cast<const x8_t*>(static_cast<const T*>(a.o) + b * a.os.batch + head * a.os.head + i * a.os.token + 8 * part);
-      const x8_t d = *reinterpret_cast<const x8_t*>(static_cast<const T*>(a.dout) + b * a.dos.batch + head * a.dos.head + i * a.dos.token + 8 * part);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) acc = fmaf(static_cast<float>(o[e]), static_cast<float>(d[e]), acc);
-    }
-  }
-  acc = wave_reduce<16>(acc, SumOp());
-  if (row < rows && part == 0) {
-    a.stats[row] = exists ? -a.lse[row] / s.scale : -1e30f;
-    a.stats[rows + row] = exists ? -acc : 0.f;
-  }
-}
+constexpr int kAhead = 2;  // matrix steps between an LDS fragment's read and its use
 
-// ---- dQ ----
+// ---- dQ, and the row statistics for the kernels after it ----
 template <typename T, int DH>
 __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
   typedef AttnElem<T> E;
@@ -81,6 +58,11 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
   const int block_q0 = w.qb * per_block;
   if (block_q0 >= query_end) {
     win_store<T, DH>(dQ, a.dqs.token, acc, 0.f, stage, lane, 0, me.rows, s.dim);
+    if (g == 0 && li < me.rows) {
+      const size_t row = (static_cast<size_t>(w.b) * s.heads + me.head) * s.Sq + me.q0 + li;
+      a.stats[row] = -1e30f;
+      a.stats[static_cast<size_t>(s.batch) * s.heads * s.Sq + row] = 0.f;
+    }
     return;
   }
   const WindowTiles tiles = window_tiles(block_q0 + s.offset(), min(block_q0 + per_block, query_end) - 1 + s.offset(), s.window, s.sinks);
@@ -89,8 +71,33 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
   win_load_row<T>(qf, static_cast<const T*>(a.q) + w.b * a.qs.batch + me.head * a.qs.head + qi * a.qs.token, s.dim, g);
   win_load_row<T>(dof, static_cast<const T*>(a.dout) + w.b * a.dos.batch + me.head * a.dos.head + qi * a.dos.token, s.dim, g);
   const float c2 = s.scale * kWinLog2e;
-  const float* st = a.stats + (static_cast<size_t>(w.b) * s.heads + me.head) * s.Sq + qi;
-  const float m2 = st[0] * c2, delta = st[static_cast<size_t>(s.batch) * s.heads * s.Sq];
+  float m2, delta = 0.f;
+  {
+    const long long o_at = w.b * a.os.batch + me.head * a.os.head + qi * a.os.token;
+    x8_t of[DS];
+    auto add = [&]() {
+#pragma unroll
+      for (int d = 0; d < DS; ++d)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) delta = fmaf(-static_cast<float>(of[d][e]), static_cast<float>(dof[d][e]), delta);
+    };
+    win_load_row<T>(of, static_cast<const T*>(a.o) + o_at, s.dim, g);
+    add();
+    if (a.low != nullptr) {
+      win_load_row<T>(of, static_cast<const T*>(a.low) + o_at, s.dim, g);
+      add();
+    }
+    delta += __shfl_xor(delta, 32, kWave);
+    const size_t row = (static_cast<size_t>(w.b) * s.heads + me.head) * s.Sq + me.q0 + li;
+    const bool exists = li < me.exist;
+    m2 = exists ? -a.lse[row] : -1e30f;
+    if (!exists) delta = 0.f;
+    if (g == 0 && li < me.rows) {
+      a.stats[row] = exists ? m2 / s.scale : -1e30f;
+      a.stats[static_cast<size_t>(s.batch) * s.heads * s.Sq + row] = delta;
+    }
+    m2 *= kWinLog2e;
+  }
   const int p = me.p_lo + li;
 
   const T* K = static_cast<const T*>(a.k) + w.b * a.ks.batch + w.kvh * a.ks.head;
@@ -103,30 +110,56 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
     win_copy<T, DH, kWinTile, kWinWaves>(V + static_cast<long long>(t) * kWinTile * a.vs.token, a.vs.token, length - t * kWinTile, s.dim, dst + TILE, wave, lane);
   };
   const WinBases lane_bases = win_lane_bases<DH>(attn_lds, lane);
-  auto compute = [&](int i, int t, auto mask_c) {
-    constexpr bool MASK = decltype(mask_c)::value;
+  // One tile.  Its matrix steps (per key block the d slices of S and dP, then the updates) read their LDS fragments
+  // kAhead steps ahead, across the phases, with the order pinned by scheduling fences; `whole`: no pair is hidden.
+  auto compute = [&](int i, int t, bool whole) {
+    constexpr int N1 = 2 * DS, N2 = 4 * DB;
     const WinBases at = win_bases(lane_bases, (i & 1) * 4 * TILE);
-    x8_t dsf[4];
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      f32x16_t sp[2];
-      win_zero(sp);
-#pragma unroll
-      for (int d = 0; d < DS; ++d) {
-        sp[0] = E::mfma(win_row_frag<T, DH>(at, 0, kb, d), qf[d], sp[0]);
-        sp[1] = E::mfma(win_row_frag<T, DH>(at, 2 * TILE, kb, d), dof[d], sp[1]);
+    x8_t dsf[4], ka[N1], va[N1], ta[N2];
+    auto issue = [&](auto ic) {
+      constexpr int n = decltype(ic)::value;
+      if constexpr (n < N1) {
+        ka[n] = win_row_frag<T, DH>(at, 0, n / DS, n % DS);
+        va[n] = win_row_frag<T, DH>(at, 2 * TILE, n / DS, n % DS);
+      } else if constexpr (n < N1 + N2) {
+        ta[n - N1] = win_tr_frag<T, DH>(at, 0, (n - N1) % DB, (n - N1) / DB);
       }
+    };
+    static_for<kAhead>([&](auto ic) { issue(ic); });
+    f32x16_t sp[2];
+    static_for<N1 + N2>([&](auto ic) {
+      constexpr int n = decltype(ic)::value;
+      issue(std::integral_constant<int, n + kAhead>{});
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (n < N1) {
+        constexpr int kb = n / DS, d = n % DS;
+        if constexpr (d == 0) win_zero(sp);
+        sp[0] = E::mfma(ka[n], qf[d], sp[0]);
+        sp[1] = E::mfma(va[n], dof[d], sp[1]);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (d == DS - 1) {
+          if (!whole) {
+            const int first = t * kWinTile + 32 * kb + 4 * g;  // key of register 0
+            const int d1 = p - first, s1 = s.sinks - first;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        float e = __builtin_amdgcn_exp2f(fmaf(sp[0][r], c2, m2));
-        if (MASK && !me.sees(p, t * kWinTile + 32 * kb + 8 * (r >> 2) + 4 * g + (r & 3))) e = 0.f;
-        dsf[2 * kb + (r >> 3)][r & 7] = static_cast<T>(e * (sp[1][r] + delta));
+            for (int r = 0; r < 16; ++r) {
+              const int o = 8 * (r >> 2) + (r & 3);
+              if (o > d1 || (o <= d1 - s.window && o >= s1)) sp[0][r] = -__builtin_inff();
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float e = __builtin_amdgcn_exp2f(fmaf(sp[0][r], c2, m2));
+            dsf[2 * kb + (r >> 3)][r & 7] = static_cast<T>(e * (sp[1][r] + delta));
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+        constexpr int j = n - N1;
+        acc[j % DB] = E::mfma(ta[j], dsf[j / DB], acc[j % DB]);
+        __builtin_amdgcn_sched_barrier(0);
       }
-    }
-#pragma unroll
-    for (int k4 = 0; k4 < 4; ++k4)
-#pragma unroll
-      for (int db = 0; db < DB; ++db) acc[db] = E::mfma(win_tr_frag<T, DH>(at, 0, db, k4), dsf[k4], acc[db]);
+    });
   };
   request(0);
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
@@ -134,12 +167,7 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
   for (int i = 0; i < tiles.n; ++i) {
     if (i + 1 < tiles.n) request(i + 1);
     const int t = tiles.at(i);
-    if (me.active(t)) {
-      if (me.whole(t))
-        compute(i, t, attn_flag<false>{});
-      else
-        compute(i, t, attn_flag<true>{});
-    }
+    if (me.active(t)) compute(i, t, me.whole(t));
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the next tile has landed
     __syncthreads();
   }
@@ -147,8 +175,6 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
 }
 
 // ---- dK (WHICH = 0) and dV (WHICH = 1): the pairs inside the window ----
-constexpr int kAhead = 2;  // matrix steps between an LDS fragment's read and its use
-
 template <typename T, int DH, int WHICH>
 __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
   constexpr bool DK = WHICH == 0;

@@ -2,15 +2,16 @@
 
 The entry points of kernels.py (residual norm with an 8-bit result, rotary positions over several axes, attention with a
 sliding window and visible first tokens) registered in the package's operator library npu_graph with shape
-functions and gradients, so that torch.compile keeps them in its graph and autograd passes through them.  The functions
-of this module are what a model calls.
+functions, and wrapped with gradients: torch.compile keeps them in its graph and autograd passes through them.  The
+functions of this module are what a model calls; outside a compilation they call the kernels' entry points without
+the dispatcher.
 """
 from __future__ import annotations
 
 from typing import Optional, Sequence
 
 import torch
-from torch.library import register_autograd
+from torch.autograd import Function
 
 from . import kernels
 from .fusion_attention_graph import gpu_lib, meta_lib, npu_def
@@ -21,21 +22,29 @@ npu_def.define(
     "bool inverse=False) -> (Tensor, Tensor)"
 )
 npu_def.define(
-    "window_attention(Tensor q, Tensor k, Tensor v, float scale, int window, int sinks=0, Tensor? lengths=None) "
-    "-> (Tensor, Tensor)"
+    "window_attention(Tensor q, Tensor k, Tensor v, float scale, int window, int sinks=0, Tensor? lengths=None, "
+    "bool keep_low=False) -> (Tensor, Tensor, Tensor)"
 )
 npu_def.define(
     "window_attention_backward(Tensor q, Tensor k, Tensor v, Tensor out, Tensor dout, Tensor lse, float scale, "
-    "int window, int sinks=0, Tensor? lengths=None) -> (Tensor, Tensor, Tensor)"
+    "int window, int sinks=0, Tensor? lengths=None, Tensor? low=None) -> (Tensor, Tensor, Tensor)"
 )
 npu_def.define(
     "window_attention_decode(Tensor q, Tensor k_cache, Tensor v_cache, Tensor lengths, float scale, int window, "
     "int sinks=0) -> Tensor"
 )
 
+
+def _window_attention(q, k, v, scale, window, sinks=0, lengths=None, keep_low=False):
+    """kernels.window_attention with three outputs in any case: an empty `low` where it is not kept."""
+    if keep_low:
+        return kernels.window_attention(q, k, v, scale, window, sinks, lengths, True)
+    return (*kernels.window_attention(q, k, v, scale, window, sinks, lengths), q.new_empty(0))
+
+
 gpu_lib.impl("add_rmsnorm_quant", kernels.add_rmsnorm_quant)
 gpu_lib.impl("rotary_axes", kernels.rotary_axes)
-gpu_lib.impl("window_attention", kernels.window_attention)
+gpu_lib.impl("window_attention", _window_attention)
 gpu_lib.impl("window_attention_backward", kernels.window_attention_backward)
 gpu_lib.impl("window_attention_decode", kernels.window_attention_decode)
 
@@ -51,11 +60,12 @@ def _rotary_axes_meta(q, k, positions, inv_freq, sections=None, interleaved=Fals
     return torch.empty_like(q), torch.empty_like(k)
 
 
-def _window_attention_meta(q, k, v, scale, window, sinks=0, lengths=None):
-    return torch.empty_like(q), torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
+def _window_attention_meta(q, k, v, scale, window, sinks=0, lengths=None, keep_low=False):
+    return (torch.empty_like(q), torch.empty(q.shape[:3], dtype=torch.float32, device=q.device),
+            torch.empty_like(q) if keep_low else q.new_empty(0))
 
 
-def _window_attention_backward_meta(q, k, v, out, dout, lse, scale, window, sinks=0, lengths=None):
+def _window_attention_backward_meta(q, k, v, out, dout, lse, scale, window, sinks=0, lengths=None, low=None):
     return torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
 
 
@@ -70,60 +80,79 @@ meta_lib.impl("window_attention_backward", _window_attention_backward_meta)
 meta_lib.impl("window_attention_decode", _window_attention_decode_meta)
 
 
-def _rotary_context(ctx, inputs, output):
-    _, _, positions, inv_freq, sections, interleaved, inverse = inputs
-    ctx.save_for_backward(positions, inv_freq)
-    ctx.form = (sections, interleaved, inverse)
+def _ops():
+    """Where a call goes: the registered ops inside a compilation (and for shape-only tensors), the kernels outside."""
+    return torch.ops.npu_graph if torch.compiler.is_compiling() else kernels
 
 
-def _rotary_backward(ctx, dq, dk):
-    positions, inv_freq = ctx.saved_tensors
-    sections, interleaved, inverse = ctx.form
-    # a rotation's gradient is the rotation back; a gradient may arrive in any layout (a sum's is one number everywhere)
-    last = lambda t: t if t.stride(-1) == 1 else t.contiguous()  # noqa: E731
-    gq, gk = torch.ops.npu_graph.rotary_axes(last(dq), last(dk), positions, inv_freq, sections, interleaved, not inverse)
-    return gq, gk, None, None, None, None, None
+def _needs_grad(*tensors: torch.Tensor) -> bool:
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
 
 
-def _window_context(ctx, inputs, output):
-    q, k, v, scale, window, sinks, lengths = inputs
-    ctx.save_for_backward(q, k, v, output[0], output[1], lengths)
-    ctx.form = (scale, window, sinks)
-    ctx.mark_non_differentiable(output[1])
+def _fits(t: torch.Tensor) -> bool:
+    """Contiguous columns in 16-byte aligned rows, what the kernels take; a gradient may arrive in any layout (a
+    sum's is one number everywhere)."""
+    return (t.stride(-1) == 1 and all(t.stride(i) % 8 == 0 for i in range(t.dim() - 1) if t.shape[i] > 1)
+            and (torch.compiler.is_compiling() or t.data_ptr() % 16 == 0))
 
 
-def _window_backward(ctx, dout, _):
-    q, k, v, out, lse, lengths = ctx.saved_tensors
-    scale, window, sinks = ctx.form
-    rows = (dout.stride(i) for i in range(3) if dout.shape[i] > 1)
-    if dout.stride(3) != 1 or dout.data_ptr() % 16 or any(s % 8 for s in rows):
-        dout = dout.contiguous()
-    return (*torch.ops.npu_graph.window_attention_backward(q, k, v, out, dout, lse, scale, window, sinks, lengths),
-            None, None, None, None)
+class RotaryFunction(Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, inv_freq, sections, interleaved, inverse):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.form = (sections, interleaved, inverse)
+        return _ops().rotary_axes(q, k, positions, inv_freq, sections, interleaved, inverse)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        positions, inv_freq = ctx.saved_tensors
+        sections, interleaved, inverse = ctx.form
+        # a rotation's gradient is the rotation back
+        dq, dk = (t if t.stride(-1) == 1 else t.contiguous() for t in (dq, dk))
+        gq, gk = _ops().rotary_axes(dq, dk, positions, inv_freq, sections, interleaved, not inverse)
+        return gq, gk, None, None, None, None, None
 
 
-register_autograd("npu_graph::rotary_axes", _rotary_backward, setup_context=_rotary_context)
-register_autograd("npu_graph::window_attention", _window_backward, setup_context=_window_context)
+class WindowAttentionFunction(Function):
+    @staticmethod
+    def forward(ctx, q, k, v, scale, window, sinks, lengths):
+        out, lse, low = _ops().window_attention(q, k, v, scale, window, sinks, lengths, True)
+        ctx.save_for_backward(q, k, v, out, lse, low, lengths)
+        ctx.form = (scale, window, sinks)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, k, v, out, lse, low, lengths = ctx.saved_tensors
+        scale, window, sinks = ctx.form
+        if not _fits(dout):
+            dout = dout.contiguous()
+        dq, dk, dv = _ops().window_attention_backward(q, k, v, out, dout, lse, scale, window, sinks, lengths, low)
+        return dq, dk, dv, None, None, None, None
 
 
 def add_rmsnorm_quant(h: torch.Tensor, r: torch.Tensor, w: torch.Tensor, eps: float = 1e-6, group: int = 0):
     """(q, scales, h + r): kernels.add_rmsnorm_quant as a graph op.  Serving only: an 8-bit result has no gradient."""
-    return torch.ops.npu_graph.add_rmsnorm_quant(h, r, w, eps, group)
+    return _ops().add_rmsnorm_quant(h, r, w, eps, group)
 
 
 def rotary_axes(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
                 sections: Optional[Sequence[int]] = None, interleaved: bool = False, inverse: bool = False):
     """kernels.rotary_axes as a graph op with gradients for q and k."""
-    return torch.ops.npu_graph.rotary_axes(q, k, positions, inv_freq, sections, interleaved, inverse)
+    if _needs_grad(q, k):
+        return RotaryFunction.apply(q, k, positions, inv_freq, sections, interleaved, inverse)
+    return _ops().rotary_axes(q, k, positions, inv_freq, sections, interleaved, inverse)
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, window: int, sinks: int = 0,
                      lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The output of kernels.window_attention as a graph op with gradients for q, k and v."""
-    return torch.ops.npu_graph.window_attention(q, k, v, scale, window, sinks, lengths)[0]
+    if _needs_grad(q, k, v):
+        return WindowAttentionFunction.apply(q, k, v, scale, window, sinks, lengths)
+    return _ops().window_attention(q, k, v, scale, window, sinks, lengths)[0]
 
 
 def window_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
                             scale: float, window: int, sinks: int = 0) -> torch.Tensor:
     """kernels.window_attention_decode as a graph op (inference)."""
-    return torch.ops.npu_graph.window_attention_decode(q, k_cache, v_cache, lengths, scale, window, sinks)
+    return _ops().window_attention_decode(q, k_cache, v_cache, lengths, scale, window, sinks)

@@ -996,13 +996,13 @@ def _window_check(q, k, v, scale, window, sinks, lengths):
 def _window_fwd_launcher() -> CachingLauncher:
     cfgs = [LaunchConfig(f"window_attention_fwd_{t}_d{d}", 512, lds_bytes=4 * 64 * d * 2) for t in _ATTN_DTYPES.values() for d in (64, 128)]
     return CachingLauncher("window_attention_fwd", codecache.aot_source("window_attention_kernels.hip"),
-                           "PPPPP" + "q" * 12 + _WINDOW_SHAPE, cfgs, prefer_intree=True)
+                           "PPPPPP" + "q" * 12 + _WINDOW_SHAPE, cfgs, prefer_intree=True)
 
 
 def window_attention(
     q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, window: int, sinks: int = 0,
-    lengths: Optional[torch.Tensor] = None,
-) -> tuple[torch.Tensor, torch.Tensor]:
+    lengths: Optional[torch.Tensor] = None, keep_low: bool = False,
+) -> tuple[torch.Tensor, ...]:
     """Causal attention with a sliding window and first tokens that stay visible, heads may share keys: returns (out
     [B, N, Sq, D], lse fp32 [B, N, Sq]) for q [B, N, Sq, D] and k, v [B, Nk, Sk, D] (bf16 or fp16, N a multiple of Nk,
     Sq <= Sk, D a multiple of 8 up to 128; any strides with contiguous 16-byte aligned rows, so [B, S, N, D] tensors go in
@@ -1011,39 +1011,40 @@ def window_attention(
     The queries are the last Sq of Sk positions; position p sees the keys j <= p with p - j < window or
     j < sinks.  window >= Sk is plain causal attention.  lengths (int32 [B], on the device): positions from lengths[b] on
     do not exist (a right-padded batch): their keys are hidden and not read, their rows of out are zero and
-    of lse -inf.  lse is the natural logarithm of the sum of exp(score * scale).
+    of lse -inf.  lse is the natural logarithm of the sum of exp(score * scale).  keep_low adds a third tensor, what
+    rounding lost of out, which makes the gradients of rows that see few keys more exact (window_attention_backward).
     A NaN or infinity in an existing key or value row can also reach queries of the 63 positions before it, for
     which it is hidden but lies in the same tile."""
     dh, window, sinks = _window_check(q, k, v, scale, window, sinks, lengths)
     B, N, Sq, D = q.shape
     out = torch.empty_like(q)
+    low = torch.empty_like(q) if keep_low else None
     lse = torch.empty((B, N, Sq), dtype=torch.float32, device=q.device)
+    result = (out, lse, low) if keep_low else (out, lse)
     if q.numel() == 0:
-        return out, lse
+        return result
     shape = _window_shape(q, k, lengths, window, sinks, scale)
     blocks = cdiv(Sq, 256 >> shape[10]) * ((N // k.shape[1]) >> shape[10])
     l = _window_fwd_launcher()
     l._launch(
         _find(l, f"window_attention_fwd_{_ATTN_DTYPES[q.dtype]}_d{dh}"),
-        (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
-         *out.stride()[:3], *shape),
+        (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), low.data_ptr() if keep_low else 0, lse.data_ptr(), *q.stride()[:3],
+         *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], *shape),
         (_window_grid(B * k.shape[1], blocks), 1, 1), _stream(),
     )
-    return out, lse
+    return result
 
 
 @functools.lru_cache(maxsize=None)
 def _window_bwd_launchers() -> dict:
     src = codecache.aot_source("window_attention_bwd_kernels.hip")
-    sig = "P" * 11 + "q" * 24 + "ii" + _WINDOW_SHAPE
-    types = tuple(_ATTN_DTYPES.values())
+    sig = "P" * 12 + "q" * 24 + "ii" + _WINDOW_SHAPE
     mk = lambda which, block, lds: CachingLauncher(  # noqa: E731
         f"window_attention_bwd_{which}", src, sig,
-        [LaunchConfig(f"window_attention_bwd_{which}_{t}_d{d}", block(d), lds_bytes=lds(d)) for t in types for d in (64, 128)],
+        [LaunchConfig(f"window_attention_bwd_{which}_{t}_d{d}", block(d), lds_bytes=lds(d))
+         for t in _ATTN_DTYPES.values() for d in (64, 128)],
         prefer_intree=True)
     return {
-        "stats": CachingLauncher("window_attention_bwd_stats", src, sig,
-                                 [LaunchConfig(f"window_attention_bwd_stats_{t}", 256) for t in types], prefer_intree=True),
         "dq": mk("dq", lambda d: 512, lambda d: 4 * 64 * d * 2),
         "dkv": mk("dkv", lambda d: 512, lambda d: 2 * (2 * 64 * d * 2 + 512)),
         "sinks": mk("sinks", lambda d: 256, lambda d: 4 * 4 * 32 * d * 2),
@@ -1059,10 +1060,10 @@ def _sink_splits(units: int, key_blocks: int, tiles: int) -> int:
 
 def window_attention_backward(
     q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, dout: torch.Tensor, lse: torch.Tensor, scale: float,
-    window: int, sinks: int = 0, lengths: Optional[torch.Tensor] = None,
+    window: int, sinks: int = 0, lengths: Optional[torch.Tensor] = None, low: Optional[torch.Tensor] = None,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """Gradients (dq, dk, dv) of window_attention; out and lse are the forward's, dout [B, N, Sq, D] in the type of q
-    (strides as for q).  dk and dv are summed over the query heads that share a key head, in fp32 and in a fixed
+    """Gradients (dq, dk, dv) of window_attention; out, lse and (if kept) low are the forward's, dout [B, N, Sq, D] in the
+    type of q (strides as for q).  dk and dv are summed over the query heads that share a key head, in fp32 and in a fixed
     order.  Rows that do not exist get zeros, and what dout holds there is not read into anything else."""
     dh, window, sinks = _window_check(q, k, v, scale, window, sinks, lengths)
     _check_here(q, out, dout, lse)
@@ -1070,6 +1071,10 @@ def window_attention_backward(
         _require(t.shape == q.shape and t.dtype == q.dtype, "out and dout must match q")
         _require(t.stride(-1) == 1 and _aligned(t) and all(x % 8 == 0 for x, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1),
                  "columns must be contiguous, and rows 16-byte aligned")
+    if low is not None:
+        _check_here(q, low)
+        _require(low.shape == out.shape and low.dtype == out.dtype and low.stride() == out.stride() and _aligned(low),
+                 "low must be laid out like out")
     B, N, Sq, D = q.shape
     Nk, Sk = k.shape[1:3]
     _require(lse.shape == (B, N, Sq) and lse.dtype == torch.float32 and lse.is_contiguous(), "lse must be the forward's [B, N, Sq] fp32")
@@ -1087,7 +1092,7 @@ def window_attention_backward(
         n_slots = 1 + _sink_splits(units, sink_rows // 32, group * cdiv(min(Sq, Sk - window), 32))
         slots = torch.empty(units * n_slots * 2 * sink_rows * dh, dtype=torch.float32, device=q.device)
     shape = _window_shape(q, k, lengths, window, sinks, scale)
-    args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+    args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), low.data_ptr() if low is not None else 0, dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
             lse.data_ptr(), stats.data_ptr(), slots.data_ptr() if slots is not None else 0,
             *(x for t in (q, k, v, out, dout, dq, dk, dv) for x in t.stride()[:3]), n_slots, sink_rows, *shape)
     ls, st, ty = _window_bwd_launchers(), _stream(), _ATTN_DTYPES[q.dtype]
@@ -1095,12 +1100,11 @@ def window_attention_backward(
     def launch(which, name, grid):
         ls[which]._launch(_find(ls[which], f"window_attention_bwd_{which}_{name}"), args, grid, st)
 
-    launch("stats", ty, (cdiv(B * N * Sq * 16, 256), 1, 1))
+    launch("dq", f"{ty}_d{dh}", (_window_grid(units, cdiv(Sq, 256 >> shape[10]) * (group >> shape[10])), 1, 1))
     launch("dkv", f"{ty}_d{dh}", (_window_grid(units, cdiv(Sk, 256)), 2, 1))
     if far:
         launch("sinks", f"{ty}_d{dh}", (units * (sink_rows // 32) * (n_slots - 1), 1, 1))
         launch("join", f"{ty}_d{dh}", (units * far, 1, 1))
-    launch("dq", f"{ty}_d{dh}", (_window_grid(units, cdiv(Sq, 256 >> shape[10]) * (group >> shape[10])), 1, 1))
     return dq, dk, dv
 
 

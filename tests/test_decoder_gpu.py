@@ -319,6 +319,15 @@ def check_window(K, case, dtype, token_major):
     for name, got in zip(("dq", "dk", "dv"), grads):
         assert got.dtype == dtype
         within(got, want[name], R.attention_bound(want[name], want[name + "_weight"], dtype), name)
+    same, lse2, low = K.window_attention(dq_, k_, v_, D**-0.5, window, sinks, ln, keep_low=True)
+    assert torch.equal(same, out) and torch.equal(lse2, lse)
+    # out and its remainder together carry the roundings of the probabilities, and of the remainder: a step's step
+    h = R.half_step(dtype)
+    within(same.double().cpu() + low.double().cpu(), want["out"],
+           want["out"].abs() * h * h + want["weight"] * (h + 2e-4) + 1e-5, "out + low")
+    finer = K.window_attention_backward(dq_, k_, v_, out, do_, lse, D**-0.5, window, sinks, ln, low)
+    for name, got in zip(("dq", "dk", "dv"), finer):
+        within(got, want[name], R.attention_bound(want[name], want[name + "_weight"], dtype), name)
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
@@ -327,3 +336,45 @@ def check_window(K, case, dtype, token_major):
 def test_window_attention(K, case, token_major, dtype):
     announce(f"window_attention {case} token_major={token_major} {dtype}")
     check_window(K, case, dtype, token_major)
+
+
+def test_window_gradients_through_autograd():
+    announce("decoder.window_attention through autograd, strided gradient, against torch's own gradients in fp64")
+    from inductor_x_amd import decoder
+
+    B, N, Nk, S, D, window, sinks = 2, 4, 2, 150, 64, 40, 3
+    q, k, v, _ = window_operands(B, N, Nk, S, S, D, BF, True)
+    leaves = [same_memory(t).requires_grad_() for t in (q, k, v)]
+    out = decoder.window_attention(*leaves, 0.125, window, sinks)
+    out.sum().backward()  # a gradient of stride zero
+    want = R.attention(q, k, v, 0.125, window, sinks, None, torch.ones_like(q))
+    for leaf, name in zip(leaves, ("dq", "dk", "dv")):
+        within(leaf.grad, want[name], R.attention_bound(want[name], want[name + "_weight"], BF), name)
+    ref = [t.double().requires_grad_() for t in (q, k, v)]
+    see = R.visible(0, S, S, window, sinks, S)
+    s = (ref[0] @ ref[1].repeat_interleave(2, 1).transpose(-1, -2) * 0.125).masked_fill(~see, -math.inf)
+    (s.softmax(-1) @ ref[2].repeat_interleave(2, 1)).sum().backward()
+    for t, name in zip(ref, ("dq", "dk", "dv")):
+        assert (t.grad - want[name]).abs().max() < 1e-12
+
+
+def test_rotary_gradients_through_autograd():
+    announce("decoder.rotary_axes through autograd")
+    from inductor_x_amd import decoder
+
+    gen = torch.Generator().manual_seed(8)
+    q, k = torch.randn(2, 5, 3, 32, generator=gen), torch.randn(2, 5, 1, 32, generator=gen)
+    positions = torch.randint(0, 50, (2, 2, 5), generator=gen)
+    inv_freq = 100.0 ** (-torch.arange(12).double() / 12)
+    dq, dk = torch.randn(2, 5, 3, 32, generator=gen), torch.randn(2, 5, 1, 32, generator=gen)
+    leaves = [t.to(DEV).requires_grad_() for t in (q, k)]
+    outs = decoder.rotary_axes(*leaves, positions.to(DEV), inv_freq.to(DEV), [5, 7])
+    torch.autograd.backward(outs, [dq.to(DEV), dk.to(DEV)])
+    for x, g, leaf in ((q, dq, leaves[0]), (k, dk, leaves[1])):
+        ref = x.double().requires_grad_()
+        y = ref.clone()
+        angle = torch.cat([positions[0].double().unsqueeze(-1) * inv_freq[:5], positions[1].double().unsqueeze(-1) * inv_freq[5:]], -1).unsqueeze(2)
+        a, b = ref[..., :12], ref[..., 12:24]
+        y = torch.cat((a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin(), ref[..., 24:]), -1)
+        y.backward(g.double())
+        within(leaf.grad, ref.grad, 1e-5 + 1e-6 * ref.grad.abs(), "rotary gradient")

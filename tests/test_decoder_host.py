@@ -117,11 +117,80 @@ def test_decode_refusals():
 
 def test_shape_functions():
     m = lambda *s, dtype=BF: torch.empty(*s, dtype=dtype, device="meta")  # noqa: E731
-    q, scales, s = decoder.add_rmsnorm_quant(m(3, 5, 300), m(3, 5, 300), m(300), 1e-6, 128)
+    ops = torch.ops.npu_graph
+    q, scales, s = ops.add_rmsnorm_quant(m(3, 5, 300), m(3, 5, 300), m(300), 1e-6, 128)
     assert q.dtype == torch.float8_e4m3fn and q.shape == s.shape == (3, 5, 300) and scales.shape == (3, 5, 3)
-    a, b = decoder.rotary_axes(m(2, 3, 4, 64), m(2, 3, 1, 64), m(1, 2, 3, dtype=torch.int32), m(32, dtype=torch.float32))
+    a, b = ops.rotary_axes(m(2, 3, 4, 64), m(2, 3, 1, 64), m(1, 2, 3, dtype=torch.int32), m(32, dtype=torch.float32))
     assert a.shape == (2, 3, 4, 64) and b.shape == (2, 3, 1, 64)
-    assert decoder.window_attention_decode(m(2, 4, 64), m(2, 2, 9, 64), m(2, 2, 9, 64), m(2, dtype=torch.int32), 0.1, 4).shape == (2, 4, 64)
+    assert ops.window_attention_decode(m(2, 4, 64), m(2, 2, 9, 64), m(2, 2, 9, 64), m(2, dtype=torch.int32), 0.1, 4).shape == (2, 4, 64)
+    q4, kv = m(2, 9, 4, 64).transpose(1, 2), m(2, 2, 11, 64)
+    for keep in (False, True):
+        out, lse, low = ops.window_attention(q4, kv, kv, 0.1, 4, 1, None, keep)
+        assert out.shape == q4.shape and out.stride() == q4.stride() and lse.shape == (2, 4, 9) and lse.dtype == torch.float32
+        assert low.shape == (q4.shape if keep else (0,))
+    assert [t.shape for t in ops.window_attention_backward(q4, kv, kv, out, out, lse, 0.1, 4, 1, None, low)] == [q4.shape, kv.shape, kv.shape]
+
+
+def window_operands(B=2, N=4, Nk=2, Sq=8, Sk=16, D=64):
+    return torch.zeros(B, N, Sq, D, dtype=BF), torch.zeros(B, Nk, Sk, D, dtype=BF), torch.zeros(B, Nk, Sk, D, dtype=BF)
+
+
+def test_window_refusals():
+    q, k, v = window_operands()
+    n = torch.ones(2, dtype=torch.int32)
+    lse = torch.zeros(2, 4, 8)
+    with pytest.raises(Launched):
+        K.window_attention(q, k, v, 0.1, 4, 1, n)
+    with pytest.raises(Launched):
+        K.window_attention_backward(q, k, v, q, q, lse, 0.1, 4, 1, n)
+    for args, text in [
+        ((q[:, :, 0], k, v, 0.1, 4, 1), r"\[B, N, Sq, D\]"),
+        ((q, k, v[:, :, :8], 0.1, 4, 1), "share one"),
+        ((q, k.half(), v, 0.1, 4, 1), "share bf16"),
+        ((q.float(), k.float(), v.float(), 0.1, 4, 1), "share bf16"),
+        ((q[:, :3], k, v, 0.1, 4, 1), "multiple of the key heads"),
+        ((q[:, :0], k, v, 0.1, 4, 1), "multiple of the key heads"),
+        ((*window_operands(D=136), 0.1, 4, 1), "multiple of 8"),
+        ((*window_operands(D=60), 0.1, 4, 1), "multiple of 8"),
+        ((*window_operands(Sq=17), 0.1, 4, 1), "more queries than keys"),
+        ((q[:1], k, v, 0.1, 4, 1), "share batch"),
+        ((q, k, v, 0.1, 4, 1, n.long()), "int32"),
+        ((q, k, v, 0.1, 4, 1, n[:1]), "one value per sequence"),
+        ((q, k, v, float("inf"), 4, 1), "scale"),
+        ((q, k, v, -1.0, 4, 1), "scale"),
+        ((q, k, v, 0.1, 0, 1), "window"),
+        ((q, k, v, 0.1, 4, -1), "sinks"),
+        ((q, k, torch.zeros(2, 2, 16, 68, dtype=BF)[..., :64], 0.1, 4, 1), "16-byte aligned"),
+        ((torch.zeros(2 * 4 * 8 * 64 + 1, dtype=BF)[1:].view(2, 4, 8, 64), k, v, 0.1, 4, 1), "16-byte aligned"),
+        ((q, k.new_empty(1).expand(2, 2, 16, 64), v, 0.1, 4, 1), "contiguous"),
+    ]:
+        with pytest.raises(ValueError, match=text):
+            K.window_attention(*args)
+    for args, text in [
+        ((q, k, v, q, q.half(), lse, 0.1, 4, 1), "match q"),
+        ((q, k, v, q[:, :, :4], q, lse, 0.1, 4, 1), "match q"),
+        ((q, k, v, q, q.new_empty(1).expand(2, 4, 8, 64), lse, 0.1, 4, 1), "contiguous"),
+        ((q, k, v, q, q, lse.half(), 0.1, 4, 1), "lse"),
+        ((q, k, v, q, q, lse[:, :, :4], 0.1, 4, 1), "lse"),
+        ((q, k, v, q, q, lse, 0.1, 4, 1, None, q[:1]), "low"),
+    ]:
+        with pytest.raises(ValueError, match=text):
+            K.window_attention_backward(*args)
+    out, lse = K.window_attention(q[:0], k[:0], v[:0], 0.1, 4)
+    assert out.shape == (0, 4, 8, 64) and lse.shape == (0, 4, 8)
+    out, lse = K.window_attention(q[:, :, :0], k, v, 0.1, 4)
+    assert out.shape == (2, 4, 0, 64)
+    grads = K.window_attention_backward(q[:, :, :0], k, v, out, out, lse, 0.1, 4)
+    assert (grads[1] == 0).all() and (grads[2] == 0).all() and grads[1].shape == k.shape
+
+
+def test_heads_of_a_workgroup():
+    assert [K._largest_share(g) for g in (1, 2, 3, 4, 5, 6, 7, 8, 12, 16, 24, 40)] == [0, 1, 0, 2, 0, 1, 0, 3, 2, 3, 3, 3]
+    for units in (1, 8, 64, 1000):
+        for blocks in (1, 4):
+            for tiles in (1, 15, 100, 10000):
+                n = K._sink_splits(units, blocks, tiles)
+                assert n >= 1 and (n == 1 or tiles // n >= 16)
 
 
 def test_splits_of_a_decode():
