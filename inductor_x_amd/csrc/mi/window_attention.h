@@ -36,7 +36,7 @@ struct WindowStride {
   long long batch, head, token;
 };
 
-// Shared problem description; every kernel takes one as its last argument.
+// Problem description that every kernel takes behind its operands' pointers.
 struct WindowShape {
   const int* lengths;  // may be null: every position exists
   int batch, heads, kv_heads, group, Sq, Sk, dim, window, sinks, hb_shift, mixed;
@@ -258,8 +258,8 @@ struct WindowFwdArgs {
   void* o;
   void* low;   // may be null: what rounding o lost, laid out like o
   float* lse;  // [B, N, Sq]
-  WindowStride qs, ks, vs, os;
   WindowShape shape;
+  WindowStride qs, ks, vs, os;
 };
 
 template <typename T, int DH>

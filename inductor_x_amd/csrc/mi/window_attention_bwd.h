@@ -29,9 +29,9 @@ struct WindowBwdArgs {
   const float* lse;  // [B, N, Sq]
   float* stats;      // [2][B, N, Sq]: -lse / scale, -D
   float* slots;      // [B * Nk][n_slots][2][sink_rows][DH] (dK without its scale, dV); null without such keys
-  WindowStride qs, ks, vs, os, dos, dqs, dks, dvs;
-  int n_slots, sink_rows;  // sink_rows: keys below `sinks`, rounded up to 32
   WindowShape shape;
+  int n_slots, sink_rows;  // sink_rows: keys below `sinks`, rounded up to 32
+  WindowStride qs, ks, vs, os, dos, dqs, dks, dvs;
 };
 
 constexpr int kAhead = 2;  // matrix steps between an LDS fragment's read and its use

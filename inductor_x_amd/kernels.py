@@ -58,6 +58,46 @@ def _check_here(*tensors: torch.Tensor) -> None:
     _require(tensors[0].device.index == torch.cuda.current_device(), "tensors must live on the current GPU")
 
 
+# Launch plans of the decoder-layer operators.  Checking operands and choosing a launch costs more host time than the launch
+# itself, and a model calls with few distinct shapes: what follows from shapes, strides, types, alignment and the
+# arguments that are no tensors is settled once per such key.  Nothing about a tensor's contents or place is kept.
+_PLANS: dict = {}
+_MAX_PLANS = 4096
+
+
+def _plan(key, make, *args):
+    """The plan under `key`, made (and its operands checked) by make(*args) where there is none."""
+    plan = _PLANS.get(key)
+    if plan is None:
+        plan = make(*args)
+        if len(_PLANS) >= _MAX_PLANS:
+            _PLANS.clear()
+        _PLANS[key] = plan
+    return plan
+
+
+def _bind(l: CachingLauncher, symbol: str, constants, grid):
+    """enqueue(stream, *pointers) for a kernel of a family (launcher.Function.prepare).  A family's code object is loaded
+    on one GPU, the one that was current at its first use (one process per GPU)."""
+    home = l.__dict__.setdefault("_home", torch.cuda.current_device())
+    _require(home == torch.cuda.current_device(), f"this process runs {l.name} on GPU {home}")
+    cfg, fn = l.launchers[_find(l, symbol)]
+    return fn.prepare(l.signature, constants, grid, (cfg.block,), cfg.lds_bytes)
+
+
+def _form(t: Optional[torch.Tensor]):
+    """What a plan depends on in an operand."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device, t.data_ptr() & 15)
+
+
+def _stream_of(t: torch.Tensor) -> int:
+    """The current stream of the tensor's device, which has to be the current one."""
+    index = t.device.index
+    if index != torch._C._cuda_getDevice():
+        raise ValueError("tensors must live on the current GPU")
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 # ---------------------------------------------------------------------------
 # code objects (one per aot file), loaded lazily
 # ---------------------------------------------------------------------------
@@ -368,6 +408,16 @@ def add_rmsnorm_quant(
     all are zero, never below the smallest normal number.  A NaN or infinity in a row gives that row (every
     128 columns of it that it reaches) NaN, as the formula does.
     h, r: bf16 or fp16 of one shape with contiguous columns and evenly spaced rows; w one vector of the same type."""
+    enqueue, scales_shape = _plan(("norm", _form(h), _form(r), _form(w), eps, group), _norm_quant_plan, h, r, w, eps, group)
+    s = h.new_empty(h.shape)
+    q = torch.empty(h.shape, dtype=torch.float8_e4m3fn, device=h.device)
+    scales = torch.empty(scales_shape, dtype=torch.float32, device=h.device)
+    if enqueue is not None:
+        enqueue(_stream_of(h), h.data_ptr(), r.data_ptr(), w.data_ptr(), q.data_ptr(), scales.data_ptr(), s.data_ptr())
+    return q, scales, s
+
+
+def _norm_quant_plan(h, r, w, eps, group):
     _check_here(h, r, w)
     _require(h.dtype == r.dtype == w.dtype and h.dtype in _ATTN_DTYPES, "h, r, w must share bf16 or fp16")
     _require(h.shape == r.shape and h.dim() >= 1, "h and r must have the same shape")
@@ -375,26 +425,17 @@ def add_rmsnorm_quant(
     cols = h.shape[-1]
     _require(w.shape == (cols,) and (cols <= 1 or w.stride(0) == 1), "w must be a contiguous vector of the row length")
     _require(0 < cols <= 32768, "row length must lie in 1..32768")
-    groups = cdiv(cols, 128) if group else 1
-    s = torch.empty(h.shape, dtype=h.dtype, device=h.device)
-    q = torch.empty(h.shape, dtype=torch.float8_e4m3fn, device=h.device)
-    scales = torch.empty(h.shape[:-1] + (groups,), dtype=torch.float32, device=h.device)
+    scales_shape = h.shape[:-1] + (cdiv(cols, 128) if group else 1,)
     rows = h.numel() // cols
     if rows == 0:
-        return q, scales, s
+        return None, scales_shape
     _require(rows < 2**31, "too many rows")
-    hm, rm = _as_rows(h, "h"), _as_rows(r, "r")
-    hs, rs = hm.stride(0), rm.stride(0)
-    wide = (cols | hs | rs) % 8 == 0 and all(_aligned(t) for t in (h, r, w, s)) and _aligned(q, 8)
+    hs, rs = _as_rows(h, "h").stride(0), _as_rows(r, "r").stride(0)
+    # rows of 8 elements' multiples on 16-byte addresses move in 16-byte pieces, any others element by element
+    wide = (cols | hs | rs) % 8 == 0 and all(_aligned(t) for t in (h, r, w))
     b, t, i = next(v for v in _NORM_QUANT_VARIANTS if cols <= v[1] * v[2] * 8)
-    l = _norm_quant_launcher()
-    idx = _find(l, f"add_rmsnorm_quant_{_ATTN_DTYPES[h.dtype]}_b{b}_t{t}_i{i}{'_g128' if group else ''}{'' if wide else '_odd'}")
-    l._launch(
-        idx, (h.data_ptr(), r.data_ptr(), w.data_ptr(), q.data_ptr(), scales.data_ptr(), s.data_ptr(), rows, cols, hs, rs,
-              float(eps)),
-        (cdiv(rows, b // t), 1, 1), _stream(),
-    )
-    return q, scales, s
+    symbol = f"add_rmsnorm_quant_{_ATTN_DTYPES[h.dtype]}_b{b}_t{t}_i{i}{'_g128' if group else ''}{'' if wide else '_odd'}"
+    return _bind(_norm_quant_launcher(), symbol, (rows, cols, hs, rs, float(eps)), (cdiv(rows, b // t),)), scales_shape
 
 
 def _snap_split_plan(plan: SplitPlan, rows: int, cols: int) -> SplitPlan:
@@ -882,6 +923,16 @@ def rotary_axes(
     consecutive pairs each axis turns (default: all on one axis).  A pair is (column p, column p + P) of P pairs, or
     with interleaved=True (column 2 p, column 2 p + 1).  inverse turns back: the gradient of the rotation.
     Angles are formed in 64 bits, the products in 32, rounded once."""
+    sections = None if sections is None else tuple(sections)
+    enqueue = _plan(("rotary", _form(q), _form(k), _form(positions), _form(inv_freq), sections, interleaved, inverse),
+                    _rotary_plan, q, k, positions, inv_freq, sections, interleaved, inverse)
+    q_out, k_out = torch.empty_like(q), torch.empty_like(k)
+    if enqueue is not None:
+        enqueue(_stream_of(q), q.data_ptr(), q_out.data_ptr(), k.data_ptr(), k_out.data_ptr(), positions.data_ptr(), inv_freq.data_ptr())
+    return q_out, k_out
+
+
+def _rotary_plan(q, k, positions, inv_freq, sections, interleaved, inverse):
     _check_here(q, k, positions, inv_freq)
     _require(q.dtype == k.dtype and q.dtype in _ROTARY_DTYPES, "q and k must share bf16, fp16 or fp32")
     _require(q.dim() == 4 and k.dim() == 4, "q [B, S, N, D] and k [B, S, Nk, D]")
@@ -901,30 +952,25 @@ def rotary_axes(
     sections = [pairs] if sections is None else [int(x) for x in sections]
     _require(len(sections) == axes and min(sections) >= 0 and sum(sections) == pairs, "sections must give every axis its share of the pairs")
     ends = [sum(sections[: i + 1]) for i in range(axes - 1)] + [pairs] * (4 - axes)
-    q_out, k_out = torch.empty_like(q), torch.empty_like(k)
     if q.numel() + k.numel() == 0:
-        return q_out, k_out
+        return None
     tokens = B * S
     _require(tokens < 2**31 and N + k.shape[2] < 2**16, "extents must fit int32 indexing")
     vec = 16 // q.element_size()
     strides = []
-    for x in (q, q_out, k, k_out):
+    for x in (q, torch.empty_like(q), k, torch.empty_like(k)):  # operand and result
         _require(D <= 1 or x.stride(3) == 1, "columns of a head must be contiguous")
-        strides += [x.stride(0), x.stride(1), x.stride(2)]
+        strides += x.stride()[:3]
     step = vec if interleaved else 2 * vec
-    wide = (2 * pairs) % step == 0 and D % vec == 0 and all(x % vec == 0 for x in strides) and all(_aligned(x) for x in (q, q_out, k, k_out))
+    wide = (2 * pairs) % step == 0 and D % vec == 0 and all(x % vec == 0 for x in strides) and _aligned(q) and _aligned(k)
     # tokens per workgroup: as many as give every thread an angle, fewer where that would leave compute units idle
     per_block = max(1, min(256 // pairs, tokens // (2 * config.hardware().cu_count)))
-    l = _rotary_launcher()
-    i = _find(l, f"rotary_axes_{_ROTARY_DTYPES[q.dtype]}_{'beside' if interleaved else 'half'}{'' if wide else '_odd'}")
-    l._launch(
-        i,
-        (q.data_ptr(), q_out.data_ptr(), k.data_ptr(), k_out.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), *strides,
-         N, k.shape[2], positions.dtype == torch.int64, inv_freq.dtype == torch.float64, tokens, S, D, 2 * pairs,
+    return _bind(
+        _rotary_launcher(), f"rotary_axes_{_ROTARY_DTYPES[q.dtype]}_{'beside' if interleaved else 'half'}{'' if wide else '_odd'}",
+        (*strides, N, k.shape[2], positions.dtype == torch.int64, inv_freq.dtype == torch.float64, tokens, S, D, 2 * pairs,
          ends[0], ends[1], ends[2], per_block, -1.0 if inverse else 1.0),
-        (cdiv(tokens, per_block), 1, 1), _stream(),
+        (cdiv(tokens, per_block),),
     )
-    return q_out, k_out
 
 
 # ---------------------------------------------------------------------------
@@ -965,14 +1011,14 @@ def _largest_share(group: int) -> int:
 _WINDOW_SHAPE = "P" + "i" * 11 + "f"  # WindowShape of csrc/mi/window_attention.h
 
 
-def _window_shape(q, k, lengths, window, sinks, scale):
-    """The WindowShape members for these operands."""
+def _window_shape(q, k, window, sinks, scale):
+    """The members of WindowShape after `lengths` for these operands."""
     B, N, Sq, D = q.shape
     Nk, Sk = k.shape[1:3]
     # Where a die's eighth of the work is not whole key heads, its query blocks alternate between the long and the
     # short end; windows that are short against the sequence make all blocks alike, which then keep their order
     mixed = int((B * Nk) % 8 != 0 and 2 * window > Sk)
-    return (lengths.data_ptr() if lengths is not None else 0, B, N, Nk, N // Nk, Sq, Sk, D, window, sinks,
+    return (B, N, Nk, N // Nk, Sq, Sk, D, window, sinks,
             _largest_share(N // Nk), mixed, float(scale))
 
 
@@ -996,7 +1042,7 @@ def _window_check(q, k, v, scale, window, sinks, lengths):
 def _window_fwd_launcher() -> CachingLauncher:
     cfgs = [LaunchConfig(f"window_attention_fwd_{t}_d{d}", 512, lds_bytes=4 * 64 * d * 2) for t in _ATTN_DTYPES.values() for d in (64, 128)]
     return CachingLauncher("window_attention_fwd", codecache.aot_source("window_attention_kernels.hip"),
-                           "PPPPPP" + "q" * 12 + _WINDOW_SHAPE, cfgs, prefer_intree=True)
+                           "PPPPPP" + _WINDOW_SHAPE + "q" * 12, cfgs, prefer_intree=True)
 
 
 def window_attention(
@@ -1015,30 +1061,34 @@ def window_attention(
     rounding lost of out, which makes the gradients of rows that see few keys more exact (window_attention_backward).
     A NaN or infinity in an existing key or value row can also reach queries of the 63 positions before it, for
     which it is hidden but lies in the same tile."""
-    dh, window, sinks = _window_check(q, k, v, scale, window, sinks, lengths)
-    B, N, Sq, D = q.shape
+    enqueue = _plan(("window", _form(q), _form(k), _form(v), scale, window, sinks, _form(lengths)),
+                    _window_plan, q, k, v, scale, window, sinks, lengths)
     out = torch.empty_like(q)
     low = torch.empty_like(q) if keep_low else None
-    lse = torch.empty((B, N, Sq), dtype=torch.float32, device=q.device)
-    result = (out, lse, low) if keep_low else (out, lse)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
+    if enqueue is not None:
+        enqueue(_stream_of(q), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), low.data_ptr() if keep_low else 0,
+                lse.data_ptr(), lengths.data_ptr() if lengths is not None else 0)
+    return (out, lse, low) if keep_low else (out, lse)
+
+
+def _window_plan(q, k, v, scale, window, sinks, lengths):
+    dh, window, sinks = _window_check(q, k, v, scale, window, sinks, lengths)
     if q.numel() == 0:
-        return result
-    shape = _window_shape(q, k, lengths, window, sinks, scale)
-    blocks = cdiv(Sq, 256 >> shape[10]) * ((N // k.shape[1]) >> shape[10])
-    l = _window_fwd_launcher()
-    l._launch(
-        _find(l, f"window_attention_fwd_{_ATTN_DTYPES[q.dtype]}_d{dh}"),
-        (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), low.data_ptr() if keep_low else 0, lse.data_ptr(), *q.stride()[:3],
-         *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], *shape),
-        (_window_grid(B * k.shape[1], blocks), 1, 1), _stream(),
+        return None
+    shape = _window_shape(q, k, window, sinks, scale)
+    units, group, share = q.shape[0] * k.shape[1], q.shape[1] // k.shape[1], shape[9]
+    return _bind(
+        _window_fwd_launcher(), f"window_attention_fwd_{_ATTN_DTYPES[q.dtype]}_d{dh}",
+        (*shape, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *torch.empty_like(q).stride()[:3]),
+        (_window_grid(units, cdiv(q.shape[2], 256 >> share) * (group >> share)),),
     )
-    return result
 
 
 @functools.lru_cache(maxsize=None)
 def _window_bwd_launchers() -> dict:
     src = codecache.aot_source("window_attention_bwd_kernels.hip")
-    sig = "P" * 12 + "q" * 24 + "ii" + _WINDOW_SHAPE
+    sig = "P" * 12 + _WINDOW_SHAPE + "ii" + "q" * 24
     mk = lambda which, block, lds: CachingLauncher(  # noqa: E731
         f"window_attention_bwd_{which}", src, sig,
         [LaunchConfig(f"window_attention_bwd_{which}_{t}_d{d}", block(d), lds_bytes=lds(d))
@@ -1065,6 +1115,27 @@ def window_attention_backward(
     """Gradients (dq, dk, dv) of window_attention; out, lse and (if kept) low are the forward's, dout [B, N, Sq, D] in the
     type of q (strides as for q).  dk and dv are summed over the query heads that share a key head, in fp32 and in a fixed
     order.  Rows that do not exist get zeros, and what dout holds there is not read into anything else."""
+    launches, slots_size = _plan(
+        ("window backward", _form(q), _form(k), _form(v), _form(out), _form(dout), _form(lse), scale, window, sinks, _form(lengths),
+         _form(low)),
+        _window_backward_plan, q, k, v, out, dout, lse, scale, window, sinks, lengths, low)
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    if not launches:
+        return dq, dk.zero_(), dv.zero_()
+    # both halves of the statistics and the slots of the first keys in one piece of memory
+    rows = lse.numel()
+    work = torch.empty(2 * rows + slots_size, dtype=torch.float32, device=q.device)
+    at = work.data_ptr()
+    st = _stream_of(q)
+    pointers = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), low.data_ptr() if low is not None else 0, dout.data_ptr(),
+                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), lse.data_ptr(), at, at + 8 * rows if slots_size else 0,
+                lengths.data_ptr() if lengths is not None else 0)
+    for enqueue in launches:
+        enqueue(st, *pointers)
+    return dq, dk, dv
+
+
+def _window_backward_plan(q, k, v, out, dout, lse, scale, window, sinks, lengths, low):
     dh, window, sinks = _window_check(q, k, v, scale, window, sinks, lengths)
     _check_here(q, out, dout, lse)
     for t in (out, dout):
@@ -1079,33 +1150,24 @@ def window_attention_backward(
     Nk, Sk = k.shape[1:3]
     _require(lse.shape == (B, N, Sq) and lse.dtype == torch.float32 and lse.is_contiguous(), "lse must be the forward's [B, N, Sq] fp32")
     _require(q.stride(2) < _STRIDE_LIMIT and dout.stride(2) < _STRIDE_LIMIT, "tokens lie too far apart")
-    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
     if q.numel() == 0:
-        return dq, dk.zero_(), dv.zero_()
+        return (), 0
     units, group = B * Nk, N // Nk
-    stats = torch.empty((2, B, N, Sq), dtype=torch.float32, device=q.device)
     # queries that see the first keys from beyond their window: those at positions >= window
     far = min(sinks, Sk) if Sk > window else 0
-    sink_rows, n_slots, slots = 0, 0, None
+    sink_rows = 32 * cdiv(far, 32)
+    n_slots = 1 + _sink_splits(units, sink_rows // 32, group * cdiv(min(Sq, Sk - window), 32)) if far else 0
+    shape = _window_shape(q, k, window, sinks, scale)
+    share = shape[9]
+    strides = (x for t in (q, k, v, out, dout, torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)) for x in t.stride()[:3])
+    constants = (*shape, n_slots, sink_rows, *strides)
+    ls, name = _window_bwd_launchers(), f"{_ATTN_DTYPES[q.dtype]}_d{dh}"
+    bind = lambda which, grid: _bind(ls[which], f"window_attention_bwd_{which}_{name}", constants, grid)  # noqa: E731
+    launches = [bind("dq", (_window_grid(units, cdiv(Sq, 256 >> share) * (group >> share)),)),
+                bind("dkv", (_window_grid(units, cdiv(Sk, 256)), 2))]
     if far:
-        sink_rows = 32 * cdiv(far, 32)
-        n_slots = 1 + _sink_splits(units, sink_rows // 32, group * cdiv(min(Sq, Sk - window), 32))
-        slots = torch.empty(units * n_slots * 2 * sink_rows * dh, dtype=torch.float32, device=q.device)
-    shape = _window_shape(q, k, lengths, window, sinks, scale)
-    args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), low.data_ptr() if low is not None else 0, dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-            lse.data_ptr(), stats.data_ptr(), slots.data_ptr() if slots is not None else 0,
-            *(x for t in (q, k, v, out, dout, dq, dk, dv) for x in t.stride()[:3]), n_slots, sink_rows, *shape)
-    ls, st, ty = _window_bwd_launchers(), _stream(), _ATTN_DTYPES[q.dtype]
-
-    def launch(which, name, grid):
-        ls[which]._launch(_find(ls[which], f"window_attention_bwd_{which}_{name}"), args, grid, st)
-
-    launch("dq", f"{ty}_d{dh}", (_window_grid(units, cdiv(Sq, 256 >> shape[10]) * (group >> shape[10])), 1, 1))
-    launch("dkv", f"{ty}_d{dh}", (_window_grid(units, cdiv(Sk, 256)), 2, 1))
-    if far:
-        launch("sinks", f"{ty}_d{dh}", (units * (sink_rows // 32) * (n_slots - 1), 1, 1))
-        launch("join", f"{ty}_d{dh}", (units * far, 1, 1))
-    return dq, dk, dv
+        launches += [bind("sinks", (units * (sink_rows // 32) * (n_slots - 1),)), bind("join", (units * far,))]
+    return tuple(launches), units * n_slots * 2 * sink_rows * dh
 
 
 @functools.lru_cache(maxsize=None)
@@ -1136,6 +1198,21 @@ def window_attention_decode(
     the token sits at position lengths[b] - 1 and sees the keys j >= lengths[b] - window and j < sinks; values past
     the capacity count as the capacity.  A sequence of length 0 gets zeros.  What lies behind a sequence's
     length is not read."""
+    enqueue, join, part_size = _plan(
+        ("decode", _form(q), _form(k_cache), _form(v_cache), _form(lengths), scale, window, sinks),
+        _window_decode_plan, q, k_cache, v_cache, lengths, scale, window, sinks)
+    out = q.new_empty(q.shape)
+    if enqueue is None:
+        return out.zero_()
+    st = _stream_of(q)
+    part = torch.empty(part_size, dtype=torch.float32, device=q.device) if part_size else None
+    enqueue(st, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), part.data_ptr() if part_size else 0, lengths.data_ptr())
+    if part_size:
+        join(st, part.data_ptr(), out.data_ptr(), lengths.data_ptr())
+    return out
+
+
+def _window_decode_plan(q, k_cache, v_cache, lengths, scale, window, sinks):
     _check_here(q, k_cache, v_cache)
     _require(q.dim() == 3, "q must be [B, N, D]")
     dh, window, sinks = _window_operands(q, k_cache, v_cache, scale, window, sinks, "caches")
@@ -1143,35 +1220,23 @@ def window_attention_decode(
     B, N, D = q.shape
     Nk, capacity = k_cache.shape[1:3]
     _require(capacity < _WINDOW_LIMIT, "capacity must stay below 2**30")
-    out = torch.empty((B, N, D), dtype=q.dtype, device=q.device)
-    if B == 0:
-        return out
-    if capacity == 0:
-        return out.zero_()
+    if B == 0 or capacity == 0:
+        return None, None, 0
     group = N // Nk
     units = B * Nk * cdiv(group, 16)
     tiles = cdiv(min(window, capacity), 32) + cdiv(min(sinks, max(capacity - window, 0)), 32)
     splits = _decode_splits(units, tiles)
     _require(units * splits < 2**31, "too many heads and sequences for one launch")
-    part = torch.empty(B * N * splits * (dh + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
     main, join = _window_decode_launchers()
     name = f"{_ATTN_DTYPES[q.dtype]}_d{dh}"
-    st = _stream()
-    main._launch(
-        _find(main, f"window_decode_{name}"),
-        (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), part.data_ptr() if part is not None else 0,
-         lengths.data_ptr(), q.stride(0), q.stride(1), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
-         v_cache.stride(0), v_cache.stride(1), v_cache.stride(2), out.stride(0), out.stride(1), Nk, group, splits, capacity, D,
-         window, sinks, float(scale) * 1.4426950408889634),
-        (units * splits, 1, 1), st,
-    )
-    if part is not None:
-        join._launch(
-            _find(join, f"window_decode_join_{name}"),
-            (part.data_ptr(), out.data_ptr(), lengths.data_ptr(), N, splits, D, out.stride(0), out.stride(1)),
-            (B * N, 1, 1), st,
-        )
-    return out
+    enqueue = _bind(
+        main, f"window_decode_{name}",
+        (q.stride(0), q.stride(1), *k_cache.stride()[:3], *v_cache.stride()[:3], N * D, D, Nk, group, splits, capacity, D, window,
+         sinks, float(scale) * 1.4426950408889634),
+        (units * splits,))
+    if splits == 1:
+        return enqueue, None, 0
+    return enqueue, _bind(join, f"window_decode_join_{name}", (N, splits, D, N * D, D), (B * N,)), B * N * splits * (dh + 2)
 
 
 # ---------------------------------------------------------------------------

@@ -259,6 +259,34 @@ class Function:
                 f"HIP error {err} ({error_string(err)})"
             )
 
+    def prepare(self, signature: str, constants: Sequence, grid: Sequence[int], block: Sequence[int], lds_bytes: int = 0):
+        """enqueue(stream, *pointers) for a kernel whose parameters are leading pointers and then constants: what does
+        not change between calls of one shape (grid, constants in their packed form) is settled once."""
+        lead = len(signature) - len(constants)
+        if lead < 0 or set(signature[:lead]) - {"P"} or set(signature) - _VALID:
+            raise LauncherError(f"{self.name}: signature {signature!r} does not start with {lead} pointers")
+        tail = struct.Struct("@" + signature).pack(*([0] * lead), *constants)[8 * lead:]
+        pack = struct.Struct("@" + "P" * lead).pack
+        (gx, gy, gz), (bx, by, bz) = (tuple(grid) + (1, 1))[:3], (tuple(block) + (1, 1))[:3]
+        fast = self._fast.launch if self._fast is not None else None
+        handle, raw, name, lib = self._handle, self._raw_handle, self.name, self._lib
+
+        def enqueue(stream: int, *pointers: int) -> None:
+            segment = pack(*pointers) + tail
+            if launch_log is not None:
+                launch_log.append(name)
+            if fast is not None:
+                err = fast(raw, gx, gy, gz, bx, by, bz, lds_bytes, stream, segment)
+            else:
+                err = lib.mi_launch_packed(handle, gx, gy, gz, bx, by, bz, lds_bytes, ctypes.c_void_p(stream), segment, len(segment))
+            if err != 0:
+                raise LauncherError(
+                    f"launch of {name} grid=({gx},{gy},{gz}) block=({bx},{by},{bz}) lds={lds_bytes} failed: "
+                    f"HIP error {err} ({error_string(err)})"
+                )
+
+        return enqueue
+
     def launch_with_library_scratch(
         self,
         signature: str,

@@ -1,5 +1,5 @@
-"""Argument checks and shape functions of the decoder-layer operators, without a GPU: the device check and the launch are
-replaced, everything between them is the product's."""
+"""Argument checks and shape functions of the decoder-layer operators, without a GPU: the device check and the binding of a
+launch are replaced, everything between them is the product's."""
 import pytest
 import torch
 
@@ -14,14 +14,13 @@ class Launched(Exception):
 
 @pytest.fixture(autouse=True)
 def no_gpu(monkeypatch):
-    def launched(self, *a, **k):
-        raise Launched(self.name)
+    def bound(l, symbol, constants, grid):
+        raise Launched(symbol)
 
     monkeypatch.setattr(K, "_check_cuda", lambda *t: None)
     monkeypatch.setattr(K, "_check_here", lambda *t: None)
-    monkeypatch.setattr(K, "_stream", lambda: 0)
-    monkeypatch.setattr(K, "_find", lambda l, symbol: 0)
-    monkeypatch.setattr(K.CachingLauncher, "_launch", launched)
+    monkeypatch.setattr(K, "_bind", bound)
+    monkeypatch.setattr(K, "_PLANS", {})
 
 
 def test_tensors_on_the_host_are_refused(monkeypatch):
