@@ -6,7 +6,11 @@
 // A workgroup takes a few tokens.  Their sines and cosines are made once, in LDS, and serve all query and key
 // heads of the token.  The angle is formed and reduced in 64 bits as a number of turns (a position of 10^6 in
 // 32 bits would lose half the digits of the angle); from the fraction of a turn on, 32 bits hold the
-// rounding of the result.  Bound by memory: every element is read and written once.
+// rounding of the result.
+//
+// Bound by memory: every element is read and written once.  128 angles a workgroup (two tokens of 64 pairs) rather
+// than one a thread, for more workgroups in flight: 59 against 63 us at [4,4096,32+8,128]; results leave with the
+// streaming hint, 59 against 63 us there and 23 against 29 us at [3,2047,24+24,96].
 #pragma once
 
 #include "common.h"
@@ -65,7 +69,7 @@ __device__ __forceinline__ void rotary_axes(const RotaryTensor& q, const RotaryT
     T* __restrict__ out = static_cast<T*>(x.out) + b * x.out_batch + s * x.out_token + hd * x.out_head;
     if (j >= turned) {
       const int c = rotary + (j - turned) * VEC;
-      store_vec<T, VEC>(out + c, load_vec<T, VEC>(in + c));
+      store_vec<T, VEC, true>(out + c, load_vec<T, VEC>(in + c));
       continue;
     }
     const float* cs = cosine + tok * pairs + j * PAIRS;
@@ -79,7 +83,7 @@ __device__ __forceinline__ void rotary_axes(const RotaryTensor& q, const RotaryT
         o[2 * e] = from_f32<T>(a * cs[e] - d * sn[e]);
         o[2 * e + 1] = from_f32<T>(d * cs[e] + a * sn[e]);
       }
-      store_vec<T, VEC>(out + j * VEC, o);
+      store_vec<T, VEC, true>(out + j * VEC, o);
     } else {
       const int ca = INTERLEAVED ? 2 * j : j * VEC;
       const int cb = INTERLEAVED ? ca + 1 : ca + pairs;
@@ -91,8 +95,8 @@ __device__ __forceinline__ void rotary_axes(const RotaryTensor& q, const RotaryT
         oa[e] = from_f32<T>(a * cs[e] - d * sn[e]);
         ob[e] = from_f32<T>(d * cs[e] + a * sn[e]);
       }
-      store_vec<T, VEC>(out + ca, oa);
-      store_vec<T, VEC>(out + cb, ob);
+      store_vec<T, VEC, true>(out + ca, oa);
+      store_vec<T, VEC, true>(out + cb, ob);
     }
   }
 }

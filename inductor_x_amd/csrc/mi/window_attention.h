@@ -7,12 +7,11 @@
 // Positions from lengths[b] on do not exist (right padding): their keys are hidden and not read, their rows are
 // zero, lse -inf.
 //
-// Work of a workgroup: eight wavefronts of 32 queries on one key head.  They are HB = 1, 2, 4 or 8 query heads
-// that share the key head times 256 / HB consecutive queries, so that heads in a group read a key tile once
-// between them, and a block visits the keys of a window plus 256 / HB - 1 others instead of 255.  The key
-// tiles of 64 it visits are the tiles that hold sinks, then those from the window of its first query to the
-// position of its last; nothing between them is read, and no mask exists in memory: a wavefront compares
-// positions in the few tiles that are neither wholly visible nor wholly hidden to it.
+// Work of a workgroup: four wavefronts of 32 queries on one key head.  They are HB = 1, 2 or 4 query heads
+// that share the key head times 128 / HB consecutive queries, so that heads in a group read a key tile once
+// between them, and a block visits the keys of a window plus 128 / HB - 1 others, in tiles of 64 (window_keys).
+// No mask exists in memory: a wavefront compares positions in the few tiles that are neither wholly visible nor
+// wholly hidden to it.
 //
 // Operand layouts and the transposed products are those of attention.h.  Tiles travel memory -> LDS by direct
 // 16-byte loads, [64][DH] as they lie in memory with the chunks of a row swizzled; rows past the end and
@@ -23,7 +22,7 @@
 
 namespace mi {
 
-constexpr int kWinWaves = 8;
+constexpr int kWinWaves = 4;
 constexpr int kWinThreads = 64 * kWinWaves;
 constexpr int kWinRows = 32 * kWinWaves;  // (head, query) rows or keys of a workgroup
 constexpr int kWinTile = 64;              // keys (queries) of a tile
@@ -48,18 +47,22 @@ struct WindowShape {
   __device__ __forceinline__ int query_end(int b) const { return min(Sq, length(b) - offset()); }
 };
 
-// The key tiles a block visits: `front` tiles with sinks, then a run that starts `skip` tiles further on.
-struct WindowTiles {
-  int front, skip, n;
-  __device__ __forceinline__ int at(int i) const { return i < front ? i : i + skip; }
+// The keys a block visits, as one run of slots cut into tiles of 64: slots below `turn` are the first keys, slot u
+// from there on is key u - turn + lo, up to the position of the last query.  No tile is spent on the gap between them,
+// and the window starts at the very first key that a query of the block sees.  In a cache so long that a tile with
+// keys of both kinds would span 2^31 bytes, `turn` is rounded up to a whole tile.
+struct WindowKeys {
+  int sinks, lo, turn, n;  // n: tiles
+  __device__ __forceinline__ int jump() const { return lo - turn; }
 };
-__device__ __forceinline__ WindowTiles window_tiles(int p_lo, int p_hi, int window, int sinks) {
-  const int first = max(0, p_lo - window + 1) / kWinTile, last = p_hi / kWinTile;
-  WindowTiles t;
-  t.front = min((min(sinks, p_hi + 1) + kWinTile - 1) / kWinTile, first);
-  t.skip = first - t.front;
-  t.n = last - first + 1 + t.front;
-  return t;
+__device__ __forceinline__ WindowKeys window_keys(int p_lo, int p_hi, int window, int sinks, long long stride) {
+  WindowKeys k;
+  k.sinks = min(sinks, p_hi + 1);
+  k.lo = max(k.sinks, p_lo - window + 1);
+  const bool near = 2 * stride * (k.lo + kWinTile) < 0x7fffffffLL;
+  k.turn = near ? k.sinks : (k.sinks + kWinTile - 1) / kWinTile * kWinTile;
+  k.n = (k.turn + p_hi + 1 - k.lo + kWinTile - 1) / kWinTile;
+  return k;
 }
 
 // Chunk swizzle of a tile row: the 16-byte chunk c of row r lies at position c ^ win_swz(r).  One swizzle serves the
@@ -71,23 +74,41 @@ __device__ __forceinline__ int win_swz(int row) {
   return r0 | (r1 << 2) | (r2 << 1);
 }
 
-// ROWS rows of DH columns, memory -> LDS, by WAVES wavefronts.  `rows` of them exist (<= 0: none), `dim` columns hold data.
-// Byte offsets stay inside the tile: the caller's pointer is the tile's first row.
+// ROWS rows of DH columns, memory -> LDS, by WAVES wavefronts.  `rows` of them exist (<= 0: none), `dim` columns hold data,
+// the rest arrives as zeros.  Byte offsets stay inside the tile: the caller's pointer is the tile's first row.  Rows from
+// `turn` on lie `jump` rows further.
 template <typename T, int DH, int ROWS, int WAVES>
-__device__ __forceinline__ void win_copy(const T* src, long long stride, int rows, int dim, T* dst, int wave, int lane) {
+__device__ __forceinline__ void win_copy(const T* src, long long stride, int rows, int dim, T* dst, int wave, int lane,
+                                         int turn = ROWS, int jump = 0) {
   constexpr int CH = DH / 8;            // chunks of a row
   constexpr int PER = 64 / CH;          // rows of one instruction
   constexpr int N = ROWS / PER / WAVES;  // instructions of a wavefront
-  const int bytes = rows > 0 ? static_cast<int>((min(rows, ROWS) - 1) * stride * 2) + dim * 2 : 0;
+  const int step = 2 * static_cast<int>(stride);
+  const int bytes = rows > 0 ? (min(rows, ROWS) - 1 + jump) * step + dim * 2 : 0;
 #pragma unroll
   for (int u = 0; u < N; ++u) {
     const int blk = wave * N + u;
     const int row = blk * PER + lane / CH;
     const int chunk = (lane % CH) ^ win_swz<DH>(row);
-    const int voff = 8 * chunk < dim ? row * static_cast<int>(stride) * 2 + 16 * chunk : 0x7ffffff0;
+    const int at = row >= turn ? row + jump : row;
+    const int voff = 8 * chunk < dim ? at * step + 16 * chunk : 0x7ffffff0;
     __builtin_amdgcn_raw_ptr_buffer_load_lds(
         __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(src), 0, bytes, 0x00020000),
         (__attribute__((address_space(3))) void*)(dst + blk * 512), 16, voff, 0, 0, 0);
+  }
+}
+// Tile t of a block's keys: rows of the key or value matrix `src` that starts at key 0 and has `length` rows
+template <typename T, int DH>
+__device__ __forceinline__ void win_copy_keys(const T* src, long long stride, const WindowKeys& k, int t, int length, int dim, T* dst,
+                                              int wave, int lane) {
+  const int slot = t * kWinTile;
+  if (slot >= k.turn) {  // a path of its own: with the turn's selects in every tile a long prefill took 5 % longer
+    const int key = slot + k.jump();
+    win_copy<T, DH, kWinTile, kWinWaves>(src + key * stride, stride, length - key, dim, dst, wave, lane);
+  } else {
+    const bool both = slot + kWinTile > k.turn;
+    win_copy<T, DH, kWinTile, kWinWaves>(src + slot * stride, stride, length - slot - (both ? k.jump() : 0), dim, dst, wave, lane,
+                                     both ? k.turn - slot : kWinTile, both ? k.jump() : 0);
   }
 }
 
@@ -152,6 +173,16 @@ __device__ __forceinline__ void win_load_row(typename AttnElem<T>::x8 (&f)[DS], 
       for (int e = 0; e < 8; ++e) f[s][e] = static_cast<T>(0.f);
     }
   }
+}
+
+// maximum and sum over the two halves of a wavefront that hold a row, by a register swap
+__device__ __forceinline__ float win_half_max(float x) {
+  const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+}
+__device__ __forceinline__ float win_half_sum(float x) {
+  const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
 }
 
 template <int DB>
@@ -223,18 +254,33 @@ __device__ __forceinline__ WindowBlock window_block(const WindowShape& s, int bl
 struct WindowWave {
   int head, q0, exist, rows;  // first query, how many of the 32 exist, how many lie inside Sq
   int p_lo, p_hi;             // positions of the first and last that exist
-  int window, sinks;
-  // some query sees some key of the tile / every query sees every key
-  __device__ __forceinline__ bool active(int tile) const {
-    const int k = tile * kWinTile;
-    return exist > 0 && k <= p_hi && (k + kWinTile > p_lo - window + 1 || k < sinks);
+  int window;
+  // some query sees some key of tile t / every query sees every key
+  __device__ __forceinline__ bool active(const WindowKeys& k, int t) const {
+    const int slot = t * kWinTile, key = slot + k.jump();
+    const bool first = slot < k.sinks && slot <= p_hi;
+    const bool rest = slot + kWinTile > k.turn && key <= p_hi && key + kWinTile - 1 > p_lo - window;
+    return exist > 0 && (first || rest);
   }
-  __device__ __forceinline__ bool whole(int tile) const {
-    const int k = tile * kWinTile;
-    return k + kWinTile - 1 <= p_lo && (k > p_hi - window || k + kWinTile <= sinks);
+  __device__ __forceinline__ bool whole(const WindowKeys& k, int t) const {
+    const int slot = t * kWinTile, key = slot + k.jump();
+    if (slot >= k.turn) return key + kWinTile - 1 <= p_lo && key > p_hi - window;
+    return slot + kWinTile <= k.sinks && slot + kWinTile - 1 <= p_lo;
   }
-  // key `k` seen from position p
-  __device__ __forceinline__ bool sees(int p, int k) const { return k <= p && (k > p - window || k < sinks); }
+  // sets x[r] (key rows 8 (r / 4) + 4 g + r % 4 of the 32 slots from `slot` on) to -inf where position p does not see it
+  __device__ __forceinline__ void hide(const WindowKeys& k, int slot, int p, int g, f32x16_t& x) const {
+    const int near = p - (slot + k.jump() + 4 * g);  // offset o is behind p by near - o, if o is a window slot
+    const int far = near - window;
+    const int turn = k.turn - slot - 4 * g;
+    const int first = min(k.sinks, p + 1) - slot - 4 * g;  // first keys: offsets below it are seen
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int o = 8 * (r >> 2) + (r & 3);
+      // without short circuits: each would be a branch around two compares
+      const bool hidden = ((o < turn) & (o >= first)) | ((o >= turn) & ((o > near) | (o <= far)));
+      x[r] = hidden ? -__builtin_inff() : x[r];
+    }
+  }
 };
 __device__ __forceinline__ WindowWave window_wave(const WindowShape& s, const WindowBlock& w, int wave, int query_end) {
   WindowWave v;
@@ -246,7 +292,6 @@ __device__ __forceinline__ WindowWave window_wave(const WindowShape& s, const Wi
   v.p_lo = v.q0 + s.offset();
   v.p_hi = v.p_lo + v.exist - 1;
   v.window = s.window;
-  v.sinks = s.sinks;
   return v;
 }
 
@@ -291,7 +336,7 @@ __device__ __forceinline__ void window_attention_fwd(const WindowFwdArgs& a) {
   }
   const int p_lo = block_q0 + s.offset();
   const int p_hi = min(block_q0 + per_block, query_end) - 1 + s.offset();
-  const WindowTiles tiles = window_tiles(p_lo, p_hi, s.window, s.sinks);
+  const WindowKeys keys = window_keys(p_lo, p_hi, s.window, s.sinks, max(a.ks.token, a.vs.token));
 
   x8_t qf[DS];
   const int qi = min(me.q0 + li, s.Sq - 1);  // rows past the end work on a copy of the last row and are not stored
@@ -303,20 +348,18 @@ __device__ __forceinline__ void window_attention_fwd(const WindowFwdArgs& a) {
   const T* V = static_cast<const T*>(a.v) + w.b * a.vs.batch + w.kvh * a.vs.head;
   T* buffers = reinterpret_cast<T*>(attn_lds);  // two of K and V
   auto request = [&](int i) {
-    const int t = tiles.at(i);
     T* dst = buffers + (i & 1) * 2 * TILE;
-    win_copy<T, DH, kWinTile, kWinWaves>(K + static_cast<long long>(t) * kWinTile * a.ks.token, a.ks.token, length - t * kWinTile, s.dim, dst, wave, lane);
-    win_copy<T, DH, kWinTile, kWinWaves>(V + static_cast<long long>(t) * kWinTile * a.vs.token, a.vs.token, length - t * kWinTile, s.dim, dst + TILE, wave, lane);
+    win_copy_keys<T, DH>(K, a.ks.token, keys, i, length, s.dim, dst, wave, lane);
+    win_copy_keys<T, DH>(V, a.vs.token, keys, i, length, s.dim, dst + TILE, wave, lane);
   };
   const WinBases lane_bases = win_lane_bases<DH>(attn_lds, lane);
   float m = kWinFloor, l = 0.f;
   request(0);
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   __syncthreads();
-  for (int i = 0; i < tiles.n; ++i) {
-    if (i + 1 < tiles.n) request(i + 1);
-    const int t = tiles.at(i);
-    if (me.active(t)) {
+  for (int i = 0; i < keys.n; ++i) {
+    if (i + 1 < keys.n) request(i + 1);
+    if (me.active(keys, i)) {
       const WinBases at = win_bases(lane_bases, (i & 1) * 4 * TILE);
       f32x16_t sacc[2];
       win_zero(sacc);
@@ -324,19 +367,16 @@ __device__ __forceinline__ void window_attention_fwd(const WindowFwdArgs& a) {
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int d = 0; d < DS; ++d) sacc[kb] = E::mfma(win_row_frag<T, DH>(at, 0, kb, d), qf[d], sacc[kb]);
-      if (!me.whole(t)) {
+      if (!me.whole(keys, i)) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (!me.sees(p, t * kWinTile + 32 * kb + 8 * (r >> 2) + 4 * g + (r & 3))) sacc[kb][r] = -__builtin_inff();
+        for (int kb = 0; kb < 2; ++kb) me.hide(keys, i * kWinTile + 32 * kb, p, g, sacc[kb]);
       }
-      float mx = kWinFloor;
+      float mx = sacc[0][0];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sacc[kb][r] * scale2);
-      mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sacc[kb][r]);
+      mx = fmaxf(win_half_max(mx) * scale2, kWinFloor);
       const float m_new = mx > m + kAttnSlack ? mx : m;
       const float alpha = __builtin_amdgcn_exp2f(m - m_new);
       m = m_new;
@@ -365,7 +405,7 @@ __device__ __forceinline__ void window_attention_fwd(const WindowFwdArgs& a) {
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the next tile has landed
     __syncthreads();
   }
-  l += __shfl_xor(l, 32, kWave);
+  l = win_half_sum(l);
   win_store<T, DH>(O, a.os.token, oacc, 1.0f / l, stage, lane, me.exist, me.rows, s.dim);
   if (a.low != nullptr)
     win_store<T, DH, true>(static_cast<T*>(a.low) + o_at, a.os.token, oacc, 1.0f / l, stage, lane, me.exist, me.rows, s.dim);

@@ -2,13 +2,13 @@
 // and dS = P * (dO V^T - D) over the visible pairs:
 //     dV = P^T dO        dK = scale * dS^T Q        dQ = scale * dS K        (dK, dV summed over the heads of a group)
 //
-//   dQ          blocks and key tiles of the forward: eight wavefronts of 32 queries of heads that share a key head.  It
+//   dQ          blocks and key tiles of the forward: wavefronts of 32 queries of heads that share a key head.  It
 //               also forms the row statistics -lse / scale and -D, the values that the accumulators of Q K^T and
 //               dO V^T start from in the kernels after it, so that P = exp2(S' scale log2 e) and dS = P dP' need no
 //               subtraction there; a row that does not exist gets -1e30 and 0, which makes its P zero.
 //               D takes O with what its rounding lost, where the forward kept that: in rows that see few keys
 //               dO V^T and D nearly cancel, and the rounding of O would be the largest error of dS.
-//   dK, dV      a wavefront owns 32 keys, a workgroup 256 of one key head, and walks the query tiles of 64 that see
+//   dK, dV      a wavefront owns 32 keys, a workgroup 128 of one key head, and walks the query tiles of 64 that see
 //               them through the window, head after head of the group.  The two gradients are separate halves of the
 //               launch: with both a wavefront's accumulators and operands outgrow the 256 registers it has at two
 //               wavefronts per SIMD.
@@ -34,7 +34,8 @@ struct WindowBwdArgs {
   WindowStride qs, ks, vs, os, dos, dqs, dks, dvs;
 };
 
-constexpr int kAhead = 2;  // matrix steps between an LDS fragment's read and its use
+// Matrix steps between an LDS fragment's read and its use, in dK / dV and in dQ, which has no registers for two.
+constexpr int kAhead = 2, kAheadQ = 1;
 
 // ---- dQ, and the row statistics for the kernels after it ----
 template <typename T, int DH>
@@ -65,7 +66,8 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
     }
     return;
   }
-  const WindowTiles tiles = window_tiles(block_q0 + s.offset(), min(block_q0 + per_block, query_end) - 1 + s.offset(), s.window, s.sinks);
+  const WindowKeys keys = window_keys(block_q0 + s.offset(), min(block_q0 + per_block, query_end) - 1 + s.offset(), s.window, s.sinks,
+                                      max(a.ks.token, a.vs.token));
   const int qi = min(me.q0 + li, s.Sq - 1);
   x8_t qf[DS], dof[DS];
   win_load_row<T>(qf, static_cast<const T*>(a.q) + w.b * a.qs.batch + me.head * a.qs.head + qi * a.qs.token, s.dim, g);
@@ -87,7 +89,7 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
       win_load_row<T>(of, static_cast<const T*>(a.low) + o_at, s.dim, g);
       add();
     }
-    delta += __shfl_xor(delta, 32, kWave);
+    delta = win_half_sum(delta);
     const size_t row = (static_cast<size_t>(w.b) * s.heads + me.head) * s.Sq + me.q0 + li;
     const bool exists = li < me.exist;
     m2 = exists ? -a.lse[row] : -1e30f;
@@ -104,15 +106,14 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
   const T* V = static_cast<const T*>(a.v) + w.b * a.vs.batch + w.kvh * a.vs.head;
   T* buffers = reinterpret_cast<T*>(attn_lds);
   auto request = [&](int i) {
-    const int t = tiles.at(i);
     T* dst = buffers + (i & 1) * 2 * TILE;
-    win_copy<T, DH, kWinTile, kWinWaves>(K + static_cast<long long>(t) * kWinTile * a.ks.token, a.ks.token, length - t * kWinTile, s.dim, dst, wave, lane);
-    win_copy<T, DH, kWinTile, kWinWaves>(V + static_cast<long long>(t) * kWinTile * a.vs.token, a.vs.token, length - t * kWinTile, s.dim, dst + TILE, wave, lane);
+    win_copy_keys<T, DH>(K, a.ks.token, keys, i, length, s.dim, dst, wave, lane);
+    win_copy_keys<T, DH>(V, a.vs.token, keys, i, length, s.dim, dst + TILE, wave, lane);
   };
   const WinBases lane_bases = win_lane_bases<DH>(attn_lds, lane);
   // One tile.  Its matrix steps (per key block the d slices of S and dP, then the updates) read their LDS fragments
-  // kAhead steps ahead, across the phases, with the order pinned by scheduling fences; `whole`: no pair is hidden.
-  auto compute = [&](int i, int t, bool whole) {
+  // kAheadQ steps ahead, across the phases, with the order pinned by scheduling fences; `whole`: no pair is hidden.
+  auto compute = [&](int i, bool whole) {
     constexpr int N1 = 2 * DS, N2 = 4 * DB;
     const WinBases at = win_bases(lane_bases, (i & 1) * 4 * TILE);
     x8_t dsf[4], ka[N1], va[N1], ta[N2];
@@ -125,11 +126,11 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
         ta[n - N1] = win_tr_frag<T, DH>(at, 0, (n - N1) % DB, (n - N1) / DB);
       }
     };
-    static_for<kAhead>([&](auto ic) { issue(ic); });
+    static_for<kAheadQ>([&](auto ic) { issue(ic); });
     f32x16_t sp[2];
     static_for<N1 + N2>([&](auto ic) {
       constexpr int n = decltype(ic)::value;
-      issue(std::integral_constant<int, n + kAhead>{});
+      issue(std::integral_constant<int, n + kAheadQ>{});
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (n < N1) {
         constexpr int kb = n / DS, d = n % DS;
@@ -138,15 +139,7 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
         sp[1] = E::mfma(va[n], dof[d], sp[1]);
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (d == DS - 1) {
-          if (!whole) {
-            const int first = t * kWinTile + 32 * kb + 4 * g;  // key of register 0
-            const int d1 = p - first, s1 = s.sinks - first;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int o = 8 * (r >> 2) + (r & 3);
-              if (o > d1 || (o <= d1 - s.window && o >= s1)) sp[0][r] = -__builtin_inff();
-            }
-          }
+          if (!whole) me.hide(keys, i * kWinTile + 32 * kb, p, g, sp[0]);
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const float e = __builtin_amdgcn_exp2f(fmaf(sp[0][r], c2, m2));
@@ -164,10 +157,9 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
   request(0);
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   __syncthreads();
-  for (int i = 0; i < tiles.n; ++i) {
-    if (i + 1 < tiles.n) request(i + 1);
-    const int t = tiles.at(i);
-    if (me.active(t)) compute(i, t, me.whole(t));
+  for (int i = 0; i < keys.n; ++i) {
+    if (i + 1 < keys.n) request(i + 1);
+    if (me.active(keys, i)) compute(i, me.whole(keys, i));
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the next tile has landed
     __syncthreads();
   }
@@ -278,7 +270,7 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
               const int o = 8 * (r >> 2) + (r & 3);
-              if (o < d0 || o - s.window >= d0) sp[0][r] = -__builtin_inff();
+              sp[0][r] = (o < d0) | (o >= d0 + s.window) ? -__builtin_inff() : sp[0][r];
             }
           }
 #pragma unroll
@@ -396,7 +388,7 @@ __device__ __forceinline__ void window_bwd_sinks(const WindowBwdArgs& a) {
     for (int r = 0; r < 16; ++r) {
       const int q = q0 + 8 * (r >> 2) + 4 * g + (r & 3);
       float x = __builtin_amdgcn_exp2f(sp[0][r] * c2);
-      if (!(q < query_end && q + off - kj >= s.window && li < keys)) x = 0.f;
+      x = (q < query_end) & (q + off - kj >= s.window) & (li < keys) ? x : 0.f;
       pf[r >> 3][r & 7] = static_cast<T>(x);
       dsf[r >> 3][r & 7] = static_cast<T>(x * sp[1][r]);
     }

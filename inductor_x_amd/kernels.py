@@ -410,8 +410,8 @@ def add_rmsnorm_quant(
     h, r: bf16 or fp16 of one shape with contiguous columns and evenly spaced rows; w one vector of the same type."""
     enqueue, scales_shape = _plan(("norm", _form(h), _form(r), _form(w), eps, group), _norm_quant_plan, h, r, w, eps, group)
     s = h.new_empty(h.shape)
-    q = torch.empty(h.shape, dtype=torch.float8_e4m3fn, device=h.device)
-    scales = torch.empty(scales_shape, dtype=torch.float32, device=h.device)
+    q = h.new_empty(h.shape, dtype=torch.float8_e4m3fn)
+    scales = h.new_empty(scales_shape, dtype=torch.float32)
     if enqueue is not None:
         enqueue(_stream_of(h), h.data_ptr(), r.data_ptr(), w.data_ptr(), q.data_ptr(), scales.data_ptr(), s.data_ptr())
     return q, scales, s
@@ -963,8 +963,8 @@ def _rotary_plan(q, k, positions, inv_freq, sections, interleaved, inverse):
         strides += x.stride()[:3]
     step = vec if interleaved else 2 * vec
     wide = (2 * pairs) % step == 0 and D % vec == 0 and all(x % vec == 0 for x in strides) and _aligned(q) and _aligned(k)
-    # tokens per workgroup: as many as give every thread an angle, fewer where that would leave compute units idle
-    per_block = max(1, min(256 // pairs, tokens // (2 * config.hardware().cu_count)))
+    # tokens per workgroup: 128 angles' worth, fewer where that would leave compute units idle
+    per_block = max(1, min(128 // pairs, tokens // (2 * config.hardware().cu_count)))
     return _bind(
         _rotary_launcher(), f"rotary_axes_{_ROTARY_DTYPES[q.dtype]}_{'beside' if interleaved else 'half'}{'' if wide else '_odd'}",
         (*strides, N, k.shape[2], positions.dtype == torch.int64, inv_freq.dtype == torch.float64, tokens, S, D, 2 * pairs,
@@ -1003,9 +1003,12 @@ def _check_lengths(lengths, t):
              "lengths must be a contiguous int32 vector with one value per sequence")
 
 
+_WINDOW_ROWS = 128  # (head, query) rows or keys of a workgroup: four wavefronts of 32
+
+
 def _largest_share(group: int) -> int:
-    """log2 of the query heads of a group that a workgroup's eight wavefronts work on together."""
-    return next(e for e in (3, 2, 1, 0) if group % (1 << e) == 0)
+    """log2 of the query heads of a group that a workgroup's four wavefronts work on together."""
+    return next(e for e in (2, 1, 0) if group % (1 << e) == 0)
 
 
 _WINDOW_SHAPE = "P" + "i" * 11 + "f"  # WindowShape of csrc/mi/window_attention.h
@@ -1040,7 +1043,7 @@ def _window_check(q, k, v, scale, window, sinks, lengths):
 
 @functools.lru_cache(maxsize=None)
 def _window_fwd_launcher() -> CachingLauncher:
-    cfgs = [LaunchConfig(f"window_attention_fwd_{t}_d{d}", 512, lds_bytes=4 * 64 * d * 2) for t in _ATTN_DTYPES.values() for d in (64, 128)]
+    cfgs = [LaunchConfig(f"window_attention_fwd_{t}_d{d}", 256, lds_bytes=4 * 64 * d * 2) for t in _ATTN_DTYPES.values() for d in (64, 128)]
     return CachingLauncher("window_attention_fwd", codecache.aot_source("window_attention_kernels.hip"),
                            "PPPPPP" + _WINDOW_SHAPE + "q" * 12, cfgs, prefer_intree=True)
 
@@ -1076,12 +1079,13 @@ def _window_plan(q, k, v, scale, window, sinks, lengths):
     dh, window, sinks = _window_check(q, k, v, scale, window, sinks, lengths)
     if q.numel() == 0:
         return None
+    units, group = q.shape[0] * k.shape[1], q.shape[1] // k.shape[1]
     shape = _window_shape(q, k, window, sinks, scale)
-    units, group, share = q.shape[0] * k.shape[1], q.shape[1] // k.shape[1], shape[9]
+    share = shape[9]
     return _bind(
         _window_fwd_launcher(), f"window_attention_fwd_{_ATTN_DTYPES[q.dtype]}_d{dh}",
         (*shape, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *torch.empty_like(q).stride()[:3]),
-        (_window_grid(units, cdiv(q.shape[2], 256 >> share) * (group >> share)),),
+        (_window_grid(units, cdiv(q.shape[2], _WINDOW_ROWS >> share) * (group >> share)),),
     )
 
 
@@ -1089,23 +1093,22 @@ def _window_plan(q, k, v, scale, window, sinks, lengths):
 def _window_bwd_launchers() -> dict:
     src = codecache.aot_source("window_attention_bwd_kernels.hip")
     sig = "P" * 12 + _WINDOW_SHAPE + "ii" + "q" * 24
-    mk = lambda which, block, lds: CachingLauncher(  # noqa: E731
+    mk = lambda which, forms: CachingLauncher(  # noqa: E731
         f"window_attention_bwd_{which}", src, sig,
-        [LaunchConfig(f"window_attention_bwd_{which}_{t}_d{d}", block(d), lds_bytes=lds(d))
-         for t in _ATTN_DTYPES.values() for d in (64, 128)],
-        prefer_intree=True)
+        [LaunchConfig(f"window_attention_bwd_{which}_{t}_{form}", block, lds_bytes=lds)
+         for t in _ATTN_DTYPES.values() for form, block, lds in forms], prefer_intree=True)
     return {
-        "dq": mk("dq", lambda d: 512, lambda d: 4 * 64 * d * 2),
-        "dkv": mk("dkv", lambda d: 512, lambda d: 2 * (2 * 64 * d * 2 + 512)),
-        "sinks": mk("sinks", lambda d: 256, lambda d: 4 * 4 * 32 * d * 2),
-        "join": mk("join", lambda d: 2 * d, lambda d: 0),
+        "dq": mk("dq", [(f"d{d}", 256, 4 * 64 * d * 2) for d in (64, 128)]),
+        "dkv": mk("dkv", [(f"d{d}", 256, 2 * (2 * 64 * d * 2 + 512)) for d in (64, 128)]),
+        "sinks": mk("sinks", [(f"d{d}", 256, 4 * 4 * 32 * d * 2) for d in (64, 128)]),
+        "join": mk("join", [(f"d{d}", 2 * d, 0) for d in (64, 128)]),
     }
 
 
 def _sink_splits(units: int, key_blocks: int, tiles: int) -> int:
     """Shares into which the queries that see the first keys from beyond their window are cut: two workgroups for
-    each compute unit, and four tiles of 32 queries for each of a workgroup's four wavefronts."""
-    return max(1, min(cdiv(2 * config.hardware().cu_count, units * key_blocks), tiles // 16))
+    each compute unit, and at least a tile of 32 queries for each of a workgroup's four wavefronts."""
+    return max(1, min(cdiv(2 * config.hardware().cu_count, units * key_blocks), tiles // 4))
 
 
 def window_attention_backward(
@@ -1157,14 +1160,14 @@ def _window_backward_plan(q, k, v, out, dout, lse, scale, window, sinks, lengths
     far = min(sinks, Sk) if Sk > window else 0
     sink_rows = 32 * cdiv(far, 32)
     n_slots = 1 + _sink_splits(units, sink_rows // 32, group * cdiv(min(Sq, Sk - window), 32)) if far else 0
+    strides = tuple(x for t in (q, k, v, out, dout, torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)) for x in t.stride()[:3])
     shape = _window_shape(q, k, window, sinks, scale)
     share = shape[9]
-    strides = (x for t in (q, k, v, out, dout, torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)) for x in t.stride()[:3])
     constants = (*shape, n_slots, sink_rows, *strides)
     ls, name = _window_bwd_launchers(), f"{_ATTN_DTYPES[q.dtype]}_d{dh}"
     bind = lambda which, grid: _bind(ls[which], f"window_attention_bwd_{which}_{name}", constants, grid)  # noqa: E731
-    launches = [bind("dq", (_window_grid(units, cdiv(Sq, 256 >> share) * (group >> share)),)),
-                bind("dkv", (_window_grid(units, cdiv(Sk, 256)), 2))]
+    launches = [bind("dq", (_window_grid(units, cdiv(Sq, _WINDOW_ROWS >> share) * (group >> share)),)),
+                bind("dkv", (_window_grid(units, cdiv(Sk, _WINDOW_ROWS)), 2))]
     if far:
         launches += [bind("sinks", (units * (sink_rows // 32) * (n_slots - 1),)), bind("join", (units * far,))]
     return tuple(launches), units * n_slots * 2 * sink_rows * dh

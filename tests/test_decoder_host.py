@@ -184,12 +184,12 @@ def test_window_refusals():
 
 
 def test_heads_of_a_workgroup():
-    assert [K._largest_share(g) for g in (1, 2, 3, 4, 5, 6, 7, 8, 12, 16, 24, 40)] == [0, 1, 0, 2, 0, 1, 0, 3, 2, 3, 3, 3]
+    assert [K._largest_share(g) for g in (1, 2, 3, 4, 5, 6, 7, 8, 12, 16, 24, 40)] == [0, 1, 0, 2, 0, 1, 0, 2, 2, 2, 2, 2]
     for units in (1, 8, 64, 1000):
         for blocks in (1, 4):
             for tiles in (1, 15, 100, 10000):
                 n = K._sink_splits(units, blocks, tiles)
-                assert n >= 1 and (n == 1 or tiles // n >= 16)
+                assert n >= 1 and (n == 1 or tiles // n >= 4)
 
 
 def test_splits_of_a_decode():
