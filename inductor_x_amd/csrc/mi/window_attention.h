@@ -38,14 +38,16 @@ struct WindowStride {
 // Problem description that every kernel takes behind its operands' pointers.
 struct WindowShape {
   const int* lengths;  // may be null: every position exists
-  int batch, heads, kv_heads, group, Sq, Sk, dim, window, sinks, hb_shift, mixed;
-  float scale;
+  int batch, heads, kv_heads, group, Sq, Sk, dim, window, sinks, hb_shift;
+  float scale, scale2;  // scale2 = scale log2 e
 
   __device__ __forceinline__ int offset() const { return Sk - Sq; }
   __device__ __forceinline__ int length(int b) const { return lengths ? min(max(lengths[b], 0), Sk) : Sk; }
   // queries that exist (may be <= 0)
   __device__ __forceinline__ int query_end(int b) const { return min(Sq, length(b) - offset()); }
 };
+
+static_assert(sizeof(WindowShape) == 56, "the host packs it without padding");
 
 // The keys a block visits, as one run of slots cut into tiles of 64: slots below `turn` are the first keys, slot u
 // from there on is key u - turn + lo, up to the position of the last query.  No tile is spent on the gap between them,
@@ -185,6 +187,15 @@ __device__ __forceinline__ float win_half_sum(float x) {
   return __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
 }
 
+// keeps the computation of a fragment in its place: the compiler otherwise moves it to the fragment's use, behind the
+// products of the next block, and holds the fp32 scores until then
+template <typename X8>
+__device__ __forceinline__ void win_pin(X8& f) {
+  u32x4_t w = __builtin_bit_cast(u32x4_t, f);
+  asm volatile("" : "+v"(w));
+  f = __builtin_bit_cast(X8, w);
+}
+
 template <int DB>
 __device__ __forceinline__ void win_zero(f32x16_t (&acc)[DB]) {
 #pragma unroll
@@ -227,9 +238,8 @@ __device__ __forceinline__ void win_store(T* dst, long long stride, const f32x16
 }
 
 // Where a workgroup works.  Consecutive ids go round-robin to the eight dies, each with its own L2: a die takes a
-// contiguous eighth of the items, which run through one key head's query blocks before the next.  Blocks run from the
-// last to the first (a block without a full window before it is shorter); with `mixed` the two ends alternate, so that
-// any run of items has the same work also where a die's share is part of a head.
+// contiguous eighth of the items, which run through one key head's query blocks before the next, from the last to the
+// first (a block without a full window before it is shorter).
 struct WindowBlock {
   int b, kvh, qb, hg;
   bool any;
@@ -246,7 +256,7 @@ __device__ __forceinline__ WindowBlock window_block(const WindowShape& s, int bl
   w.kvh = unit % s.kv_heads;
   const int at = rest / parts;
   w.hg = rest % parts;
-  w.qb = s.mixed ? (at & 1 ? at >> 1 : blocks - 1 - (at >> 1)) : blocks - 1 - at;
+  w.qb = blocks - 1 - at;
   return w;
 }
 
@@ -342,7 +352,7 @@ __device__ __forceinline__ void window_attention_fwd(const WindowFwdArgs& a) {
   const int qi = min(me.q0 + li, s.Sq - 1);  // rows past the end work on a copy of the last row and are not stored
   win_load_row<T>(qf, static_cast<const T*>(a.q) + w.b * a.qs.batch + me.head * a.qs.head + qi * a.qs.token, s.dim, g);
   const int p = me.p_lo + li;
-  const float scale2 = s.scale * kWinLog2e;
+  const float scale2 = s.scale2;
 
   const T* K = static_cast<const T*>(a.k) + w.b * a.ks.batch + w.kvh * a.ks.head;
   const T* V = static_cast<const T*>(a.v) + w.b * a.vs.batch + w.kvh * a.vs.head;

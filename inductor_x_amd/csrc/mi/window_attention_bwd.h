@@ -34,8 +34,8 @@ struct WindowBwdArgs {
   WindowStride qs, ks, vs, os, dos, dqs, dks, dvs;
 };
 
-// Matrix steps between an LDS fragment's read and its use, in dK / dV and in dQ, which has no registers for two.
-constexpr int kAhead = 2, kAheadQ = 1;
+// Matrix steps between an LDS fragment's read and its use; one to four measured alike.
+constexpr int kAhead = 2;
 
 // ---- dQ, and the row statistics for the kernels after it ----
 template <typename T, int DH>
@@ -72,7 +72,7 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
   x8_t qf[DS], dof[DS];
   win_load_row<T>(qf, static_cast<const T*>(a.q) + w.b * a.qs.batch + me.head * a.qs.head + qi * a.qs.token, s.dim, g);
   win_load_row<T>(dof, static_cast<const T*>(a.dout) + w.b * a.dos.batch + me.head * a.dos.head + qi * a.dos.token, s.dim, g);
-  const float c2 = s.scale * kWinLog2e;
+  const float c2 = s.scale2;
   float m2, delta = 0.f;
   {
     const long long o_at = w.b * a.os.batch + me.head * a.os.head + qi * a.os.token;
@@ -112,7 +112,7 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
   };
   const WinBases lane_bases = win_lane_bases<DH>(attn_lds, lane);
   // One tile.  Its matrix steps (per key block the d slices of S and dP, then the updates) read their LDS fragments
-  // kAheadQ steps ahead, across the phases, with the order pinned by scheduling fences; `whole`: no pair is hidden.
+  // kAhead steps ahead, across the phases, with the order pinned by scheduling fences; `whole`: no pair is hidden.
   auto compute = [&](int i, bool whole) {
     constexpr int N1 = 2 * DS, N2 = 4 * DB;
     const WinBases at = win_bases(lane_bases, (i & 1) * 4 * TILE);
@@ -126,11 +126,11 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
         ta[n - N1] = win_tr_frag<T, DH>(at, 0, (n - N1) % DB, (n - N1) / DB);
       }
     };
-    static_for<kAheadQ>([&](auto ic) { issue(ic); });
+    static_for<kAhead>([&](auto ic) { issue(ic); });
     f32x16_t sp[2];
     static_for<N1 + N2>([&](auto ic) {
       constexpr int n = decltype(ic)::value;
-      issue(std::integral_constant<int, n + kAheadQ>{});
+      issue(std::integral_constant<int, n + kAhead>{});
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (n < N1) {
         constexpr int kb = n / DS, d = n % DS;
@@ -145,6 +145,8 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
             const float e = __builtin_amdgcn_exp2f(fmaf(sp[0][r], c2, m2));
             dsf[2 * kb + (r >> 3)][r & 7] = static_cast<T>(e * (sp[1][r] + delta));
           }
+          win_pin(dsf[2 * kb]);
+          win_pin(dsf[2 * kb + 1]);
           __builtin_amdgcn_sched_barrier(0);
         }
       } else {
@@ -198,7 +200,7 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
   x8_t kf[DS], vf[DK ? DS : 1];
   win_load_row<T>(kf, static_cast<const T*>(a.k) + w.b * a.ks.batch + w.kvh * a.ks.head + kc * a.ks.token, s.dim, g);
   if constexpr (DK) win_load_row<T>(vf, static_cast<const T*>(a.v) + w.b * a.vs.batch + w.kvh * a.vs.head + kc * a.vs.token, s.dim, g);
-  const float c2 = s.scale * kWinLog2e;
+  const float c2 = s.scale2;
   const WinBases lane_bases = win_lane_bases<DH>(attn_lds, lane);
 
   float sst;
@@ -278,6 +280,8 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
             const float x = __builtin_amdgcn_exp2f(sp[0][r] * c2);
             bf[2 * qb + (r >> 3)][r & 7] = static_cast<T>(DK ? x * sp[DK ? 1 : 0][r] : x);
           }
+          win_pin(bf[2 * qb]);
+          win_pin(bf[2 * qb + 1]);
           __builtin_amdgcn_sched_barrier(0);
         }
       } else {
@@ -299,6 +303,9 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
     const int p0 = t * kWinTile + off;  // positions p0 .. p0 + 63
     if (exist > 0 && p0 + kWinTile > kw && p0 < kw + 32 - 1 + s.window)
       compute(i, t, p0 >= kw + 31 && p0 + kWinTile - 1 < kw + s.window);
+    // one register set for the sums on both ways here: the compiler otherwise copies all of them in every tile
+#pragma unroll
+    for (int db = 0; db < DB; ++db) asm volatile("" : "+v"(acc[db]));
     if (i + 1 < steps) finish(i + 1);
     __syncthreads();
     if (++t == t_lo + nt) t = t_lo;
@@ -347,7 +354,7 @@ __device__ __forceinline__ void window_bwd_sinks(const WindowBwdArgs& a) {
   x8_t kf[DS], vf[DS];
   win_load_row<T>(kf, static_cast<const T*>(a.k) + b * a.ks.batch + kvh * a.ks.head + kc * a.ks.token, s.dim, g);
   win_load_row<T>(vf, static_cast<const T*>(a.v) + b * a.vs.batch + kvh * a.vs.head + kc * a.vs.token, s.dim, g);
-  const float c2 = s.scale * kWinLog2e;
+  const float c2 = s.scale2;
   const WinBases lane_bases = win_lane_bases<DH>(attn_lds, lane);
   f32x16_t dk[DB], dv[DB];
   win_zero(dk);

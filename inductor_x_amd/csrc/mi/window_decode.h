@@ -243,22 +243,31 @@ __device__ __forceinline__ void window_decode(const DecodeArgs& a) {
   }
 }
 
-// Joins the splits of one (sequence, head): a thread per column.
+constexpr int kDecodeSplits = 64;  // most shares the keys of a sequence are cut into
+
+// Joins the splits of one (sequence, head): a thread per split finds its weight, then a thread per column adds up.
 template <typename T, int DH>
 __device__ __forceinline__ void window_decode_join(const float* __restrict__ part, T* __restrict__ out,
                                                    const int* __restrict__ lengths, int heads, int splits, int dim,
                                                    long long out_batch, long long out_head) {
+  static_assert(DH >= kDecodeSplits, "a thread per split");
+  __shared__ float weight[kDecodeSplits], share[kDecodeSplits];
   const int b = blockIdx.x / heads, h = blockIdx.x % heads, d = threadIdx.x;
   const float* p = part + static_cast<size_t>(blockIdx.x) * splits * (DH + 2);
-  float top = -1e30f;
-  for (int s = 0; s < splits; ++s) top = fmaxf(top, p[s * (DH + 2) + DH]);
-  float sum = 0.f, acc = 0.f;
-  for (int s = 0; s < splits; ++s) {
-    const float f = __builtin_amdgcn_exp2f(p[s * (DH + 2) + DH] - top);
-    sum = fmaf(p[s * (DH + 2) + DH + 1], f, sum);
-    acc = fmaf(p[s * (DH + 2) + d], f, acc);
+  const int length = lengths[b];
+  if (d < kDecodeSplits) {  // the first wavefront
+    const bool mine = d < splits;
+    const float m = mine ? p[d * (DH + 2) + DH] : -1e30f;
+    const float l = mine ? p[d * (DH + 2) + DH + 1] : 0.f;
+    const float f = __builtin_amdgcn_exp2f(m - wave_reduce<kWave>(m, MaxOp()));
+    weight[d] = mine ? f : 0.f;
+    share[d] = wave_reduce<kWave>(l * f, SumOp());
   }
-  if (d < dim) out[b * out_batch + h * out_head + d] = static_cast<T>(lengths[b] > 0 ? acc / sum : 0.f);
+  __syncthreads();
+  float acc = 0.f;
+#pragma unroll 8
+  for (int s = 0; s < splits; ++s) acc = fmaf(p[s * (DH + 2) + d], weight[s], acc);
+  if (d < dim) out[b * out_batch + h * out_head + d] = static_cast<T>(length > 0 ? acc / share[0] : 0.f);
 }
 
 }  // namespace mi

@@ -1011,18 +1011,16 @@ def _largest_share(group: int) -> int:
     return next(e for e in (2, 1, 0) if group % (1 << e) == 0)
 
 
-_WINDOW_SHAPE = "P" + "i" * 11 + "f"  # WindowShape of csrc/mi/window_attention.h
+_WINDOW_SHAPE = "P" + "i" * 10 + "ff"  # WindowShape of csrc/mi/window_attention.h
 
 
 def _window_shape(q, k, window, sinks, scale):
     """The members of WindowShape after `lengths` for these operands."""
     B, N, Sq, D = q.shape
     Nk, Sk = k.shape[1:3]
-    # Where a die's eighth of the work is not whole key heads, its query blocks alternate between the long and the
-    # short end; windows that are short against the sequence make all blocks alike, which then keep their order
-    mixed = int((B * Nk) % 8 != 0 and 2 * window > Sk)
     return (B, N, Nk, N // Nk, Sq, Sk, D, window, sinks,
-            _largest_share(N // Nk), mixed, float(scale))
+            _largest_share(N // Nk), float(scale),
+            float(scale) * 1.4426950408889634)
 
 
 def _window_grid(units: int, blocks: int) -> int:
@@ -1038,6 +1036,9 @@ def _window_check(q, k, v, scale, window, sinks, lengths):
     _require(q.shape[0] * q.shape[1] * max(1, cdiv(k.shape[2], 32)) < 2**28, "too many heads and positions for one launch")
     if lengths is not None:
         _check_lengths(lengths, q)
+    # a window or first tokens that cover every key: plain causal attention
+    if window >= k.shape[2] or sinks >= k.shape[2]:
+        window, sinks = max(1, k.shape[2]), 0
     return dh, window, sinks
 
 
@@ -1186,9 +1187,11 @@ def _window_decode_launchers() -> tuple[CachingLauncher, CachingLauncher]:
 
 
 def _decode_splits(units: int, tiles: int) -> int:
-    """Shares the visible keys of a sequence are cut into: enough workgroups for the chip, and at least two tiles of
-    32 keys for each of a workgroup's four wavefronts."""
-    return max(1, min(cdiv(2 * config.hardware().cu_count, units), tiles // 8, 64))
+    """Shares the visible keys of a sequence (tiles of 32) are cut into: a workgroup for every compute unit, and at least
+    a tile for each of a workgroup's four wavefronts.  Measured, us with 1, 2, 4 ... shares: one sequence, window 1024,
+    8 key heads: 12.3, 10.9, 9.4, 7.6 (8); four sequences of 8192 keys, 2 key heads: 66.7, 39.6, 24.6, 15.9, 12.0, 10.2 (32),
+    14.1; eight of up to 8192, 8 key heads: 36.5, 26.8, 26.1 (4), 27.9, 32.7."""
+    return max(1, min(cdiv(config.hardware().cu_count, units), tiles // 4, 64))
 
 
 def window_attention_decode(

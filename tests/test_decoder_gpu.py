@@ -276,6 +276,7 @@ WINDOW_CASES = [
     (1, 4, 4, 700, 700, 128, 200, 2, None),
     (1, 4, 2, 517, 1030, 128, 64, 128, None),
     (1, 2, 1, 900, 900, 128, 300, 900, None),          # everything is a first key
+    (1, 2, 1, 900, 900, 64, 100, 701, None),           # first keys over eleven tiles
 ]
 
 

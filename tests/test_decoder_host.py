@@ -196,4 +196,4 @@ def test_splits_of_a_decode():
     for units in (1, 7, 64, 512, 5000):
         for tiles in (1, 3, 33, 129, 40000):
             n = K._decode_splits(units, tiles)
-            assert 1 <= n <= 64 and (n == 1 or tiles // n >= 8)
+            assert 1 <= n <= 64 and (n == 1 or (tiles // n >= 4 and n <= 1 + 256 // units))
