@@ -12,6 +12,7 @@ from typing import Optional, Sequence
 
 import torch
 from torch.autograd import Function
+from torch.library import register_autograd
 
 from . import kernels
 from .fusion_attention_graph import gpu_lib, meta_lib, npu_def
@@ -80,79 +81,109 @@ meta_lib.impl("window_attention_backward", _window_attention_backward_meta)
 meta_lib.impl("window_attention_decode", _window_attention_decode_meta)
 
 
-def _ops():
-    """Where a call goes: the registered ops inside a compilation (and for shape-only tensors), the kernels outside."""
-    return torch.ops.npu_graph if torch.compiler.is_compiling() else kernels
-
-
 def _needs_grad(*tensors: torch.Tensor) -> bool:
     return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
 
 
-def _fits(t: torch.Tensor) -> bool:
-    """Contiguous columns in 16-byte aligned rows, what the kernels take; a gradient may arrive in any layout (a
-    sum's is one number everywhere)."""
-    return (t.stride(-1) == 1 and all(t.stride(i) % 8 == 0 for i in range(t.dim() - 1) if t.shape[i] > 1)
-            and (torch.compiler.is_compiling() or t.data_ptr() % 16 == 0))
+# Gradients.  The same two steps (what the forward keeps, what the backward calls) serve the registered ops, which is how
+# a compilation sees them, and autograd functions over the kernels' entry points, which eager calls go through: the
+# dispatcher's way to a Python kernel and its gradient costs about 40 us of host time more, half of what a short text's
+# kernels run.
+def _rotary_context(ctx, inputs, output):
+    _, _, positions, inv_freq, sections, interleaved, inverse = inputs
+    ctx.save_for_backward(positions, inv_freq)
+    ctx.form = (sections, interleaved, inverse)
+
+
+def _rotary_gradient(ctx, call, dq, dk):
+    positions, inv_freq = ctx.saved_tensors
+    sections, interleaved, inverse = ctx.form
+    # a rotation's gradient is the rotation back
+    dq, dk = (t if t.stride(-1) == 1 else t.contiguous() for t in (dq, dk))
+    return (*call(dq, dk, positions, inv_freq, sections, interleaved, not inverse), None, None, None, None, None)
+
+
+def _window_context(ctx, inputs, output):
+    q, k, v, scale, window, sinks, lengths, keep_low = inputs
+    out, lse, low = output
+    ctx.save_for_backward(q, k, v, out, lse, low if keep_low else None, lengths)
+    ctx.form = (scale, window, sinks)
+    ctx.mark_non_differentiable(lse, low)
+    ctx.set_materialize_grads(False)
+
+
+def _window_gradient(ctx, call, dout):
+    q, k, v, out, lse, low, lengths = ctx.saved_tensors
+    if dout is None:
+        return (None,) * 8
+    scale, window, sinks = ctx.form
+    # contiguous columns in 16-byte aligned rows are what the kernels take; a gradient may arrive in any layout (a
+    # sum's is one number everywhere)
+    if dout.stride(3) != 1 or any(dout.stride(i) % 8 for i in range(3) if dout.shape[i] > 1) or dout.storage_offset() % 8:
+        dout = dout.contiguous()
+    return (*call(q, k, v, out, dout, lse, scale, window, sinks, lengths, low), None, None, None, None, None)
+
+
+register_autograd("npu_graph::rotary_axes", lambda ctx, dq, dk: _rotary_gradient(ctx, torch.ops.npu_graph.rotary_axes, dq, dk),
+                  setup_context=_rotary_context)
+register_autograd("npu_graph::window_attention",
+                  lambda ctx, dout, *_: _window_gradient(ctx, torch.ops.npu_graph.window_attention_backward, dout),
+                  setup_context=_window_context)
 
 
 class RotaryFunction(Function):
     @staticmethod
-    def forward(ctx, q, k, positions, inv_freq, sections, interleaved, inverse):
-        ctx.save_for_backward(positions, inv_freq)
-        ctx.form = (sections, interleaved, inverse)
-        return _ops().rotary_axes(q, k, positions, inv_freq, sections, interleaved, inverse)
+    def forward(ctx, *inputs):
+        output = kernels.rotary_axes(*inputs)
+        _rotary_context(ctx, inputs, output)
+        return output
 
     @staticmethod
     def backward(ctx, dq, dk):
-        positions, inv_freq = ctx.saved_tensors
-        sections, interleaved, inverse = ctx.form
-        # a rotation's gradient is the rotation back
-        dq, dk = (t if t.stride(-1) == 1 else t.contiguous() for t in (dq, dk))
-        gq, gk = _ops().rotary_axes(dq, dk, positions, inv_freq, sections, interleaved, not inverse)
-        return gq, gk, None, None, None, None, None
+        return _rotary_gradient(ctx, kernels.rotary_axes, dq, dk)
 
 
 class WindowAttentionFunction(Function):
     @staticmethod
-    def forward(ctx, q, k, v, scale, window, sinks, lengths):
-        out, lse, low = _ops().window_attention(q, k, v, scale, window, sinks, lengths, True)
-        ctx.save_for_backward(q, k, v, out, lse, low, lengths)
-        ctx.form = (scale, window, sinks)
-        return out
+    def forward(ctx, *inputs):
+        output = kernels.window_attention(*inputs)
+        _window_context(ctx, inputs, output)
+        return output
 
     @staticmethod
-    def backward(ctx, dout):
-        q, k, v, out, lse, low, lengths = ctx.saved_tensors
-        scale, window, sinks = ctx.form
-        if not _fits(dout):
-            dout = dout.contiguous()
-        dq, dk, dv = _ops().window_attention_backward(q, k, v, out, dout, lse, scale, window, sinks, lengths, low)
-        return dq, dk, dv, None, None, None, None
+    def backward(ctx, dout, *_):
+        return _window_gradient(ctx, kernels.window_attention_backward, dout)
 
 
 def add_rmsnorm_quant(h: torch.Tensor, r: torch.Tensor, w: torch.Tensor, eps: float = 1e-6, group: int = 0):
     """(q, scales, h + r): kernels.add_rmsnorm_quant as a graph op.  Serving only: an 8-bit result has no gradient."""
-    return _ops().add_rmsnorm_quant(h, r, w, eps, group)
+    if torch.compiler.is_compiling():
+        return torch.ops.npu_graph.add_rmsnorm_quant(h, r, w, eps, group)
+    return kernels.add_rmsnorm_quant(h, r, w, eps, group)
 
 
 def rotary_axes(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
                 sections: Optional[Sequence[int]] = None, interleaved: bool = False, inverse: bool = False):
     """kernels.rotary_axes as a graph op with gradients for q and k."""
-    if _needs_grad(q, k):
-        return RotaryFunction.apply(q, k, positions, inv_freq, sections, interleaved, inverse)
-    return _ops().rotary_axes(q, k, positions, inv_freq, sections, interleaved, inverse)
+    if torch.compiler.is_compiling():
+        return torch.ops.npu_graph.rotary_axes(q, k, positions, inv_freq, sections, interleaved, inverse)
+    call = RotaryFunction.apply if _needs_grad(q, k) else kernels.rotary_axes
+    return call(q, k, positions, inv_freq, sections, interleaved, inverse)
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, window: int, sinks: int = 0,
                      lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The output of kernels.window_attention as a graph op with gradients for q, k and v."""
-    if _needs_grad(q, k, v):
-        return WindowAttentionFunction.apply(q, k, v, scale, window, sinks, lengths)
-    return _ops().window_attention(q, k, v, scale, window, sinks, lengths)[0]
+    train = _needs_grad(q, k, v)
+    if torch.compiler.is_compiling():
+        return torch.ops.npu_graph.window_attention(q, k, v, scale, window, sinks, lengths, train)[0]
+    call = WindowAttentionFunction.apply if train else kernels.window_attention
+    return call(q, k, v, scale, window, sinks, lengths, train)[0]
 
 
 def window_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
                             scale: float, window: int, sinks: int = 0) -> torch.Tensor:
     """kernels.window_attention_decode as a graph op (inference)."""
-    return _ops().window_attention_decode(q, k_cache, v_cache, lengths, scale, window, sinks)
+    if torch.compiler.is_compiling():
+        return torch.ops.npu_graph.window_attention_decode(q, k_cache, v_cache, lengths, scale, window, sinks)
+    return kernels.window_attention_decode(q, k_cache, v_cache, lengths, scale, window, sinks)

@@ -379,3 +379,262 @@ def test_rotary_gradients_through_autograd():
         y = torch.cat((a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin(), ref[..., 24:]), -1)
         y.backward(g.double())
         within(leaf.grad, ref.grad, 1e-5 + 1e-6 * ref.grad.abs(), "rotary gradient")
+
+
+# ------------------------------------------------------------------------------------ calls of other kinds
+def test_window_attention_on_slices_and_broadcasts():
+    announce("window_attention on slices of one projection, on keys expanded over the batch")
+    from inductor_x_amd import decoder, kernels as K
+
+    B, S, N, Nk, D, window, sinks = 2, 190, 6, 2, 64, 50, 2
+    gen = torch.Generator().manual_seed(9)
+    qkv = torch.randn(B, S, N + 2 * Nk, D, generator=gen).to(BF)
+    dev = qkv.to(DEV).requires_grad_()
+    parts = lambda t: (t[:, :, :N].transpose(1, 2), t[:, :, N : N + Nk].transpose(1, 2), t[:, :, N + Nk :].transpose(1, 2))  # noqa: E731
+    dout = torch.randn(B, N, S, D, generator=gen).to(BF)
+    want = R.attention(*parts(qkv), 0.125, window, sinks, None, dout)
+    out = decoder.window_attention(*parts(dev), 0.125, window, sinks)
+    within(out, want["out"], R.attention_bound(want["out"], want["weight"], BF), "out")
+    out.backward(dout.to(DEV))
+    for got, name in zip(parts(dev.grad), ("dq", "dk", "dv")):
+        within(got, want[name], R.attention_bound(want[name], want[name + "_weight"], BF), name)
+    # one set of keys for the whole batch
+    q, k, v, dout = window_operands(3, 4, 2, 70, 70, D, BF, False)
+    k1, v1 = k[:1], v[:1]
+    want = R.attention(q, k1.expand(3, -1, -1, -1), v1.expand(3, -1, -1, -1), 0.125, 20, 1, None, dout)
+    leaves = [t.to(DEV).requires_grad_() for t in (q, k1, v1)]
+    out = decoder.window_attention(leaves[0], leaves[1].expand(3, -1, -1, -1), leaves[2].expand(3, -1, -1, -1), 0.125, 20, 1)
+    within(out, want["out"], R.attention_bound(want["out"], want["weight"], BF), "out, shared keys")
+    out.backward(dout.to(DEV))
+    for leaf, name in zip(leaves[1:], ("dk", "dv")):
+        # three gradients of 16 bits, added by autograd in 16 bits: two more roundings
+        total, size = want[name].sum(0, keepdim=True), want[name].abs().sum(0, keepdim=True)
+        bound = R.attention_bound(want[name], want[name + "_weight"], BF).sum(0, keepdim=True) + 2 * R.half_step(BF) * 1.02 * size
+        within(leaf.grad, total, bound, name + ", shared keys")
+
+
+def test_window_attention_far_rows():
+    announce("window_attention with keys whose byte offsets pass 2^31, forward and gradients")
+    from inductor_x_amd import kernels as K
+
+    Sk, Sq, window, sinks, D, heads = 1_150_000, 70, 100, 5, 128, 8
+    gen = torch.Generator().manual_seed(10)
+    base = torch.zeros(1, Sk, heads, D, dtype=BF, device=DEV)
+    head, tail = torch.randn(1, 8, heads, D, generator=gen).to(BF), torch.randn(1, 200, heads, D, generator=gen).to(BF)
+    base[:, :8], base[:, Sk - 200 :] = head.to(DEV), tail.to(DEV)
+    kv = base.transpose(1, 2)
+    q, dout = (torch.randn(1, heads, Sq, D, generator=gen).to(BF) for _ in range(2))
+    out, lse, low = K.window_attention(q.to(DEV), kv, kv, 0.09, window, sinks, keep_low=True)
+    # the same positions with the unseen middle cut out: 8 + 200 keys, the window never reaches the first
+    near = torch.cat((head, tail), 1).transpose(1, 2)
+    want = R.attention(q, near, near, 0.09, window, sinks, None, dout)
+    within(out, want["out"], R.attention_bound(want["out"], want["weight"], BF), "out")
+    dq, dk, dv = K.window_attention_backward(q.to(DEV), kv, kv, out, dout.to(DEV), lse, 0.09, window, sinks, None, low)
+    within(dq, want["dq"], R.attention_bound(want["dq"], want["dq_weight"], BF), "dq")
+    for got, name in ((dk, "dk"), (dv, "dv")):
+        assert not got[:, :, 8 : Sk - 200].any()
+        got = torch.cat((got[:, :, :8], got[:, :, Sk - 200 :]), 2)
+        within(got, want[name], R.attention_bound(want[name], want[name + "_weight"], BF), name)
+
+
+def test_many_small_sequences():
+    announce("70000 sequences of three tokens, 70000 caches")
+    from inductor_x_amd import kernels as K
+
+    gen = torch.Generator().manual_seed(11)
+    q, k, v, dout = window_operands(70000, 1, 1, 3, 3, 8, BF, False, seed=11)
+    d = [t.to(DEV) for t in (q, k, v, dout)]
+    out, lse, low = K.window_attention(*d[:3], 0.3, 2, 0, keep_low=True)
+    grads = K.window_attention_backward(*d[:3], out, d[3], lse, 0.3, 2, 0, None, low)
+    last = slice(69990, 70000)
+    want = R.attention(*(t[last] for t in (q, k, v)), 0.3, 2, 0, None, dout[last])
+    within(out[last], want["out"], R.attention_bound(want["out"], want["weight"], BF), "out")
+    for got, name in zip(grads, ("dq", "dk", "dv")):
+        within(got[last], want[name], R.attention_bound(want[name], want[name + "_weight"], BF), name)
+    got = K.window_attention_decode(q.to(DEV)[:, :, 2], d[1], d[2], torch.full((70000,), 3, dtype=torch.int32, device=DEV), 0.3, 2, 0)
+    within(got[last], want["out"][:, :, 2], R.attention_bound(want["out"], want["weight"], BF)[:, :, 2], "decode")
+
+
+def training_call(K, q, k, v, dout, window, sinks, lengths):
+    out, lse, low = K.window_attention(q, k, v, 0.1, window, sinks, lengths, True)
+    return (out, lse, *K.window_attention_backward(q, k, v, out, dout, lse, 0.1, window, sinks, lengths, low))
+
+
+def test_window_attention_repeats_captures_and_streams(K):
+    announce("window_attention: equal bits on every run, in a replayed graph, and on two streams at once")
+    gen = torch.Generator().manual_seed(12)
+    q, k, v, dout = (t.to(DEV) for t in window_operands(2, 8, 2, 500, 500, 128, BF, False, seed=12))
+    lengths = torch.tensor([500, 301], dtype=torch.int32, device=DEV)
+    call = lambda: training_call(K, q, k, v, dout, 90, 4, lengths)  # noqa: E731
+    first = call()
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(first, call()))
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]  # two graphs with workspaces of their own
+    held = []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            held.append(call())
+    for step in range(3):
+        q.copy_(torch.randn(q.shape, generator=gen).to(BF))
+        lengths.copy_(torch.tensor([500 - 100 * step, 37 + step], dtype=torch.int32))
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        want = call()
+        for got in held:
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), f"replay {step}"
+    other = [t.to(DEV) for t in window_operands(2, 8, 2, 500, 500, 128, BF, False, seed=13)]
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    results = []
+    for side, operands in zip(sides, ((q, k, v, dout), other)):
+        with torch.cuda.stream(side):
+            results.append([training_call(K, *operands, 90, 4, lengths) for _ in range(4)])
+    torch.cuda.synchronize()
+    for runs, operands in zip(results, ((q, k, v, dout), other)):
+        want = training_call(K, *operands, 90, 4, lengths)
+        for got in runs:
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_norm_and_rotary_captured(K):
+    announce("norm and rotary in one replayed graph")
+    gen = torch.Generator().manual_seed(14)
+    h, r, w = (t.to(DEV) for t in norm_operands(40, 512, BF))
+    at = torch.zeros(1, 40, dtype=torch.int32, device=DEV)
+    inv_freq = (100.0 ** (-torch.arange(32).float() / 32)).to(DEV)
+    call = lambda: (*K.add_rmsnorm_quant(h, r, w, group=128), *K.rotary_axes(h.view(1, 40, 8, 64), r.view(1, 40, 8, 64), at, inv_freq))  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = call()
+    for step in range(3):
+        h.copy_(torch.randn(40, 512, generator=gen).to(BF))
+        at.copy_(torch.randint(0, 10000, (1, 40), generator=gen))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a.float(), b.float()) for a, b in zip(held, call())), f"replay {step}"
+
+
+def test_plans_do_not_outlive_their_shapes(K):
+    announce("the same storage under other shapes, strides, types and alignments")
+    gen = torch.Generator().manual_seed(15)
+    raw = torch.randn(4096 * 3, generator=gen).to(BF).to(DEV)
+    w = torch.ones(4096, dtype=BF, device=DEV)
+    for rows, cols, offset in ((2, 512, 0), (4, 256, 0), (2, 512, 1), (2, 512, 8), (1, 1024, 0), (8, 128, 3)):
+        h = raw[offset : offset + rows * cols].view(rows, cols)
+        check_norm(K.add_rmsnorm_quant(h, h, w[:cols]), h.cpu(), h.cpu(), w[:cols].cpu(), 1e-6, 0)
+    part, whole = raw[:2048].view(2, 1024)[:, :512], raw[:1024].view(2, 512)
+    check_norm(K.add_rmsnorm_quant(part, whole, w[:512]), part.cpu(), whole.cpu(), w[:512].cpu(), 1e-6, 0)
+
+
+# ------------------------------------------------------------------------------------ used together
+class Layer(torch.nn.Module):
+    """The attention half of a decoder layer on these operators: norm with an 8-bit result, projections from it, rotary
+    positions over three axes, window attention, output projection."""
+
+    def __init__(self, width, heads, kv_heads, dim, window, sinks, gen):
+        super().__init__()
+        self.register_buffer("norm", torch.ones(width, dtype=BF, device=DEV))
+        w = torch.randn((heads + 2 * kv_heads) * dim, width, generator=gen) / math.sqrt(width)
+        scale = w.abs().amax(1, keepdim=True) / 448
+        self.register_buffer("wqkv", (w / scale).to(torch.float8_e4m3fn).to(DEV).t())
+        self.register_buffer("wqkv_scale", scale.t().contiguous().to(DEV))
+        self.register_buffer("wo", (torch.randn(heads * dim, width, generator=gen) / math.sqrt(heads * dim)).to(BF).to(DEV))
+        self.heads, self.kv_heads, self.dim, self.window, self.sinks = heads, kv_heads, dim, window, sinks
+        self.register_buffer("inv_freq", (10000.0 ** (-torch.arange(dim // 2, dtype=torch.float64) / (dim // 2))).float().to(DEV))
+
+    def projections(self, h, r, positions):
+        from inductor_x_amd import decoder
+
+        q8, scales, s = decoder.add_rmsnorm_quant(h, r, self.norm)
+        x = torch._scaled_mm(q8.flatten(0, 1), self.wqkv, scales.flatten(0, 1), self.wqkv_scale, out_dtype=BF)
+        q, k, v = x.view(*h.shape[:2], -1, self.dim).split([self.heads, self.kv_heads, self.kv_heads], 2)
+        q, k = decoder.rotary_axes(q, k, positions, self.inv_freq, [self.dim // 2 - 20, 10, 10])
+        return s, q, k, v
+
+    def forward(self, h, r, positions):
+        from inductor_x_amd import decoder
+
+        s, q, k, v = self.projections(h, r, positions)
+        out = decoder.window_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), self.dim**-0.5, self.window, self.sinks)
+        return s, torch.matmul(out.transpose(1, 2).flatten(-2), self.wo), k, v
+
+    def step(self, h, r, positions, k_cache, v_cache, lengths):
+        from inductor_x_amd import decoder
+
+        s, q, k, v = self.projections(h, r, positions)
+        at = (lengths - 1).long()
+        rows = torch.arange(h.shape[0], device=DEV)
+        k_cache[rows, at], v_cache[rows, at] = k[:, 0], v[:, 0]
+        out = decoder.window_attention_decode(q[:, 0], k_cache.transpose(1, 2), v_cache.transpose(1, 2), lengths, self.dim**-0.5,
+                                              self.window, self.sinks)
+        return s, torch.matmul(out.flatten(-2), self.wo)
+
+
+def layer_and_texts(B=2, S=75, width=256, window=20, sinks=3):
+    gen = torch.Generator().manual_seed(16)
+    layer = Layer(width, 8, 2, 64, window, sinks, gen)
+    h, r = (torch.randn(B, S, width, generator=gen).to(BF).to(DEV) for _ in range(2))
+    at = torch.arange(S).view(1, S).expand(B, S)
+    positions = torch.stack((at + 1000, at // 10, at % 10)).to(torch.int32).contiguous().to(DEV)
+    return layer, h, r, positions
+
+
+def test_decoding_follows_the_prefill():
+    announce("a layer's prefill against the same tokens decoded one by one over a cache")
+    layer, h, r, positions = layer_and_texts()
+    B, S = h.shape[:2]
+    s, out, k, v = layer(h, r, positions)
+    k_cache, v_cache = (torch.full((B, S + 30, 2, 64), float("nan"), dtype=BF, device=DEV) for _ in range(2))
+    for t in range(S):
+        lengths = torch.full((B,), t + 1, dtype=torch.int32, device=DEV)
+        s1, o1 = layer.step(h[:, t : t + 1], r[:, t : t + 1], positions[:, :, t : t + 1].contiguous(), k_cache, v_cache, lengths)
+        assert torch.equal(s1[:, 0], s[:, t])
+        # both attention outputs are within two roundings of the same value (probabilities, result) times the weight,
+        # below 1 for a mean of unit normals; the products then add 512 such errors over sqrt(512) weights of 1 / sqrt(512):
+        # at most 2 * 2 * 2^-8 * sqrt(512) = 0.35 if all had one sign, 0.016 * 3 as independent errors; their own
+        # roundings to 16 bits (inputs to and outputs of the projections in another order) are of the same size
+        assert (o1.float() - out[:, t].float()).abs().max() <= 0.35
+        assert (o1.float() - out[:, t].float()).norm() <= 0.03 * out[:, t].float().norm()
+    keep = torch.equal(k_cache[:, :S].isnan(), torch.zeros_like(k_cache[:, :S], dtype=torch.bool))
+    assert keep and k_cache[:, S:].isnan().all()  # rows behind the last token are left alone
+
+
+def test_layer_compiles_into_one_graph():
+    announce("a layer under torch.compile without a break, forward and decode, against its eager run")
+    import inductor_x_amd  # noqa: F401
+
+    layer, h, r, positions = layer_and_texts()
+    want = layer(h, r, positions)
+    got = torch.compile(layer, fullgraph=True)(h, r, positions)
+    for a, b in zip(got, want):
+        # the same kernels between products that the compiler may fuse with a conversion: rounding steps of bf16
+        assert a.shape == b.shape and (a.float() - b.float()).norm() <= 0.02 * b.float().norm()
+
+
+def test_gradients_compile():
+    announce("rotary and window attention with gradients under torch.compile")
+    from inductor_x_amd import decoder
+
+    B, S, N, Nk, D = 2, 60, 4, 2, 64
+    gen = torch.Generator().manual_seed(17)
+    q, k, v = (torch.randn(B, S, n, D, generator=gen).to(BF) for n in (N, Nk, Nk))
+    positions = torch.arange(S, dtype=torch.int32).view(1, 1, S).expand(1, B, S).contiguous().to(DEV)
+    inv_freq = (100.0 ** (-torch.arange(D // 2).float() / (D // 2))).to(DEV)
+    dout = torch.randn(B, N, S, D, generator=gen).to(BF).to(DEV)
+
+    def f(q, k, v):
+        q, k = decoder.rotary_axes(q, k, positions, inv_freq)
+        return decoder.window_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), 0.125, 16, 2)
+
+    results = []
+    for fn in (f, torch.compile(f, fullgraph=True)):
+        leaves = [t.to(DEV).requires_grad_() for t in (q, k, v)]
+        out = fn(*leaves)
+        out.backward(dout)
+        results.append([out.detach(), *(t.grad for t in leaves)])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)  # the same kernels on the same operands

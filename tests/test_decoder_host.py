@@ -197,3 +197,32 @@ def test_splits_of_a_decode():
         for tiles in (1, 3, 33, 129, 40000):
             n = K._decode_splits(units, tiles)
             assert 1 <= n <= 64 and (n == 1 or (tiles // n >= 4 and n <= 1 + 256 // units))
+
+
+def test_gradient_formulas_against_differences():
+    """The fp64 gradients that the kernels are held to, against central differences of the fp64 forward."""
+    from tests import decoder_reference as R
+
+    gen = torch.Generator().manual_seed(0)
+    q, k, v, dout = (torch.randn(2, n, s, 8, generator=gen, dtype=torch.float64) for n, s in ((4, 6), (2, 9), (2, 9), (4, 6)))
+    form = (0.4, 3, 2, [9, 7])
+    grads = R.attention(q, k, v, *form, dout)
+    loss = lambda: (R.attention(q, k, v, *form)["out"] * dout).sum().item()  # noqa: E731
+    for t, name in ((q, "dq"), (k, "dk"), (v, "dv")):
+        flat = t.view(-1)
+        for i in range(0, flat.numel(), 7):
+            at, step = flat[i].item(), 1e-5
+            flat[i] = at + step
+            up = loss()
+            flat[i] = at - step
+            down = loss()
+            flat[i] = at
+            # truncation of order step^2, cancellation of order 1e-16 / step
+            assert abs((up - down) / (2 * step) - grads[name].view(-1)[i].item()) < 1e-7, (name, i)
+    x = torch.randn(1, 3, 2, 12, generator=gen, dtype=torch.float64)
+    y = torch.randn(1, 3, 2, 12, generator=gen, dtype=torch.float64)
+    at, freq = torch.randint(0, 50, (2, 1, 3), generator=gen), torch.rand(5, generator=gen, dtype=torch.float64)
+    for beside in (False, True):
+        turned = R.rotary(x, at, freq, [2, 3], beside, False)
+        back = R.rotary(y, at, freq, [2, 3], beside, True)
+        assert abs((turned * y).sum() - (x * back).sum()) < 1e-12  # a linear map and its transpose
