@@ -9,12 +9,8 @@ using namespace mi;
   extern "C" __global__ __launch_bounds__(kWinThreads, 2) void window_attention_bwd_dq_##TN##_d##DH(WindowBwdArgs args) { \
     window_bwd_dq<T, DH>(args);                                                                                          \
   }                                                                                                                      \
-  /* gridDim.y = 2: dK, dV */                                                                                            \
-  extern "C" __global__ __launch_bounds__(kWinThreads, 2) void window_attention_bwd_dkv_##TN##_d##DH(WindowBwdArgs args) { \
-    if (blockIdx.y == 0)                                                                                                 \
-      window_bwd_dkv<T, DH, 0>(args);                                                                                    \
-    else                                                                                                                 \
-      window_bwd_dkv<T, DH, 1>(args);                                                                                    \
+  extern "C" __global__ __launch_bounds__(128 * kPairs, 2) void window_attention_bwd_dkv_##TN##_d##DH(WindowBwdArgs args) { \
+    window_bwd_dkv<T, DH>(args);                                                                                         \
   }                                                                                                                      \
   extern "C" __global__ __launch_bounds__(64 * kSinkWaves, 1) void window_attention_bwd_sinks_##TN##_d##DH(WindowBwdArgs args) { \
     window_bwd_sinks<T, DH>(args);                                                                                       \

@@ -168,10 +168,20 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
   win_store<T, DH>(dQ, a.dqs.token, acc, s.scale, stage, lane, me.exist, me.rows, s.dim);
 }
 
-// ---- dK (WHICH = 0) and dV (WHICH = 1): the pairs inside the window ----
-template <typename T, int DH, int WHICH>
+// ---- dK and dV: the pairs inside the window ----
+constexpr int kPairs = 4;                      // 32 keys each: two wavefronts, one for P and dV, one for dP and dK
+constexpr int kPairKeys = 32 * kPairs;
+constexpr int kPairBytes = kWinTile / 2 * 64 * 4;  // P of a tile in fp32, as its lanes hold it
+
+// All wavefronts meet; unlike __syncthreads this leaves copies into the other buffer under way.
+__device__ __forceinline__ void win_meet() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");  // writes to LDS have landed
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+template <typename T, int DH>
 __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
-  constexpr bool DK = WHICH == 0;
   typedef AttnElem<T> E;
   typedef typename E::x8 x8_t;
   constexpr int DS = DH / 16, DB = DH / 32, TILE = kWinTile * DH;
@@ -180,28 +190,28 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
   const WindowShape& s = a.shape;
   const int lane = threadIdx.x & 63, li = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const WindowBlock w = window_block(s, (s.Sk + kWinRows - 1) / kWinRows, 1);
+  const int pair = wave % kPairs;
+  const bool for_dk = wave >= kPairs;  // the two wavefronts of a pair share a SIMD
+  const WindowBlock w = window_block(s, (s.Sk + kPairKeys - 1) / kPairKeys, 1);
   if (!w.any) return;
   const int length = s.length(w.b), query_end = s.query_end(w.b), off = s.offset();
-  const int k0 = w.qb * kWinRows, kw = k0 + 32 * wave;
+  const int k0 = w.qb * kPairKeys, kw = k0 + 32 * pair;
   const int exist = min(32, length - kw), rows = min(32, s.Sk - kw);
-  const WindowStride& ds = DK ? a.dks : a.dvs;
-  T* out = static_cast<T*>(DK ? a.dk : a.dv) + w.b * ds.batch + w.kvh * ds.head + kw * ds.token;
-  T* stage = reinterpret_cast<T*>(attn_lds) + wave * (32 * DH);
   f32x16_t acc[DB];
   win_zero(acc);
 
   // query tiles that see a key of the block through the window
   const int t_lo = max(0, k0 - off) / kWinTile;
-  const int q_last = min(query_end - 1, min(k0 + kWinRows, length) - 2 + s.window - off);
+  const int q_last = min(query_end - 1, min(k0 + kPairKeys, length) - 2 + s.window - off);
   const int nt = k0 < length && q_last >= 0 ? max(0, q_last / kWinTile - t_lo + 1) : 0;
   const int steps = nt * s.group;
   const int kj = kw + li, kc = min(kj, s.Sk - 1);
-  x8_t kf[DS], vf[DK ? DS : 1];
-  win_load_row<T>(kf, static_cast<const T*>(a.k) + w.b * a.ks.batch + w.kvh * a.ks.head + kc * a.ks.token, s.dim, g);
-  if constexpr (DK) win_load_row<T>(vf, static_cast<const T*>(a.v) + w.b * a.vs.batch + w.kvh * a.vs.head + kc * a.vs.token, s.dim, g);
+  x8_t kf[DS];  // the lane's key for P, its value for dP
+  win_load_row<T>(kf, for_dk ? static_cast<const T*>(a.v) + w.b * a.vs.batch + w.kvh * a.vs.head + kc * a.vs.token
+                             : static_cast<const T*>(a.k) + w.b * a.ks.batch + w.kvh * a.ks.head + kc * a.ks.token, s.dim, g);
   const float c2 = s.scale2;
   const WinBases lane_bases = win_lane_bases<DH>(attn_lds, lane);
+  float* handed = reinterpret_cast<float*>(attn_lds + 2 * BUF + pair * kPairBytes) + 4 * lane;
 
   float sst;
   int next_h = 0, next_t = t_lo;  // head of the group and query tile of the next request
@@ -209,10 +219,10 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
     const int head = w.kvh * s.group + next_h;
     T* dst = reinterpret_cast<T*>(attn_lds + (i & 1) * BUF);
     const long long q0 = static_cast<long long>(next_t) * kWinTile;
-    win_copy<T, DH, kWinTile, kWinWaves>(static_cast<const T*>(a.q) + w.b * a.qs.batch + head * a.qs.head + q0 * a.qs.token, a.qs.token,
-                                         query_end - static_cast<int>(q0), s.dim, dst, wave, lane);
-    win_copy<T, DH, kWinTile, kWinWaves>(static_cast<const T*>(a.dout) + w.b * a.dos.batch + head * a.dos.head + q0 * a.dos.token, a.dos.token,
-                                         query_end - static_cast<int>(q0), s.dim, dst + TILE, wave, lane);
+    win_copy<T, DH, kWinTile, 2 * kPairs>(static_cast<const T*>(a.q) + w.b * a.qs.batch + head * a.qs.head + q0 * a.qs.token, a.qs.token,
+                                          query_end - static_cast<int>(q0), s.dim, dst, wave, lane);
+    win_copy<T, DH, kWinTile, 2 * kPairs>(static_cast<const T*>(a.dout) + w.b * a.dos.batch + head * a.dos.head + q0 * a.dos.token, a.dos.token,
+                                          query_end - static_cast<int>(q0), s.dim, dst + TILE, wave, lane);
     if (threadIdx.x < 2 * kWinTile) {  // the first wavefront fetches -lse / scale of the 64 rows, the second -D
       const int q = static_cast<int>(q0) + lane;
       sst = wave == 0 ? -1e30f : 0.f;
@@ -228,90 +238,108 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
     if (threadIdx.x < 2 * kWinTile) reinterpret_cast<float*>(attn_lds + (i & 1) * BUF + 4 * TILE)[threadIdx.x] = sst;
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   };
-  // One tile.  Its matrix steps (per query block the d slices of S and dP, then the updates) read their LDS fragments
-  // kAhead steps ahead, across the phases, with the order pinned by scheduling fences; `whole`: no pair is hidden.
-  auto compute = [&](int i, int t, bool whole) {
-    constexpr int N1 = 2 * DS, N2 = 4 * DB;
-    const WinBases at = win_bases(lane_bases, (i & 1) * BUF);
-    const float* st = reinterpret_cast<const float*>(attn_lds + (i & 1) * BUF + 4 * TILE);
-    const int p0 = t * kWinTile + off;
-    x8_t bf[4], qa[N1], da[DK ? N1 : 1], ta[N2];
-    auto issue = [&](auto ic) {
-      constexpr int n = decltype(ic)::value;
-      if constexpr (n < N1) {
-        qa[n] = win_row_frag<T, DH>(at, 0, n / DS, n % DS);
-        if constexpr (DK) da[n] = win_row_frag<T, DH>(at, 2 * TILE, n / DS, n % DS);
-      } else if constexpr (n < N1 + N2) {
-        ta[n - N1] = win_tr_frag<T, DH>(at, DK ? 0 : 2 * TILE, (n - N1) % DB, (n - N1) / DB);
-      }
-    };
-    static_for<kAhead>([&](auto ic) { issue(ic); });
-    f32x16_t sp[DK ? 2 : 1];
-    static_for<N1 + N2>([&](auto ic) {
-      constexpr int n = decltype(ic)::value;
-      issue(std::integral_constant<int, n + kAhead>{});
-      __builtin_amdgcn_sched_barrier(0);
-      if constexpr (n < N1) {
-        constexpr int qb = n / DS, d = n % DS;
-        if constexpr (d == 0) {
+  // the loop of one kind of wavefront; both kinds run it over the same tiles and meet at the same places
+  auto run = [&](auto for_dk_c) {
+    constexpr bool FOR_DK = decltype(for_dk_c)::value;
+    f32x16_t sp[2];  // S and then P, or dP, of the two blocks of 32 queries
+    x8_t bf[4];      // P or dS as operands
+    int t = t_lo;
+    for (int i = 0; i < steps; ++i) {
+      if (i + 1 < steps) request(i + 1);
+      const int p0 = t * kWinTile + off;  // positions p0 .. p0 + 63
+      const bool active = exist > 0 && p0 + kWinTile > kw && p0 < kw + 32 - 1 + s.window;
+      const WinBases at = win_bases(lane_bases, (i & 1) * BUF);
+      if (active) {
+        // sp = start values + (Q or dO) (K or V)^T, fragments kAhead steps ahead, the order pinned by scheduling fences
+        constexpr int N = 2 * DS, tile = FOR_DK ? 2 * TILE : 0;
+        x8_t qa[N];
+        static_for<kAhead>([&](auto ic) { qa[ic.value] = win_row_frag<T, DH>(at, tile, ic.value / DS, ic.value % DS); });
+        const float* st = reinterpret_cast<const float*>(attn_lds + (i & 1) * BUF + 4 * TILE) + (FOR_DK ? kWinTile : 0) + 4 * g;
 #pragma unroll
-          for (int k = 0; k < (DK ? 2 : 1); ++k)
+        for (int qb = 0; qb < 2; ++qb)
+#pragma unroll
+          for (int rq = 0; rq < 4; ++rq) {
+            const Vec<float, 4> v = load_vec<float, 4>(st + 32 * qb + 8 * rq);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sp[qb][4 * rq + e] = v[e];
+          }
+        static_for<N>([&](auto ic) {
+          constexpr int n = decltype(ic)::value;
+          if constexpr (n + kAhead < N) qa[n + kAhead] = win_row_frag<T, DH>(at, tile, (n + kAhead) / DS, (n + kAhead) % DS);
+          __builtin_amdgcn_sched_barrier(0);
+          sp[n / DS] = E::mfma(qa[n], kf[n % DS], sp[n / DS]);
+          __builtin_amdgcn_sched_barrier(0);
+        });
+        if constexpr (!FOR_DK) {
+          if (!(p0 >= kw + 31 && p0 + kWinTile - 1 < kw + s.window)) {
+#pragma unroll
+            for (int qb = 0; qb < 2; ++qb) {
+              const int d0 = kj - (p0 + 32 * qb + 4 * g);  // row r sees the key if d0 <= its offset < d0 + window
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                const int o = 8 * (r >> 2) + (r & 3);
+                sp[qb][r] = (o < d0) | (o >= d0 + s.window) ? -__builtin_inff() : sp[qb][r];
+              }
+            }
+          }
+#pragma unroll
+          for (int qb = 0; qb < 2; ++qb)
 #pragma unroll
             for (int rq = 0; rq < 4; ++rq) {
-              const Vec<float, 4> v = load_vec<float, 4>(st + k * kWinTile + 32 * qb + 8 * rq + 4 * g);
+              Vec<float, 4> v;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) sp[k][4 * rq + e] = v[e];
+              for (int e = 0; e < 4; ++e) {
+                v[e] = __builtin_amdgcn_exp2f(sp[qb][4 * rq + e] * c2);
+                bf[2 * qb + (rq >> 1)][4 * (rq & 1) + e] = static_cast<T>(v[e]);
+              }
+              store_vec<float, 4>(handed + 256 * (4 * qb + rq), v);
             }
         }
-        sp[0] = E::mfma(qa[n], kf[d], sp[0]);
-        if constexpr (DK) sp[1] = E::mfma(da[n], vf[d], sp[1]);
-        __builtin_amdgcn_sched_barrier(0);
-        if constexpr (d == DS - 1) {
-          if (!whole) {
-            const int d0 = kj - (p0 + 32 * qb + 4 * g);  // row r sees the key if d0 <= its offset < d0 + window
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int o = 8 * (r >> 2) + (r & 3);
-              sp[0][r] = (o < d0) | (o >= d0 + s.window) ? -__builtin_inff() : sp[0][r];
-            }
-          }
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float x = __builtin_amdgcn_exp2f(sp[0][r] * c2);
-            bf[2 * qb + (r >> 3)][r & 7] = static_cast<T>(DK ? x * sp[DK ? 1 : 0][r] : x);
-          }
-          win_pin(bf[2 * qb]);
-          win_pin(bf[2 * qb + 1]);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      } else {
-        constexpr int j = n - N1;
-        acc[j % DB] = E::mfma(ta[j], bf[j / DB], acc[j % DB]);
-        __builtin_amdgcn_sched_barrier(0);
       }
-    });
+      win_meet();  // P is handed over
+      if (active) {
+        if constexpr (FOR_DK) {
+#pragma unroll
+          for (int qb = 0; qb < 2; ++qb)
+#pragma unroll
+            for (int rq = 0; rq < 4; ++rq) {
+              const Vec<float, 4> v = load_vec<float, 4>(handed + 256 * (4 * qb + rq));
+#pragma unroll
+              for (int e = 0; e < 4; ++e) bf[2 * qb + (rq >> 1)][4 * (rq & 1) + e] = static_cast<T>(v[e] * sp[qb][4 * rq + e]);
+            }
+        }
+        // acc += (dO or Q)^T (P or dS)
+        constexpr int N = 4 * DB, tile = FOR_DK ? 0 : 2 * TILE;
+        x8_t ta[N];
+        static_for<kAhead>([&](auto ic) { ta[ic.value] = win_tr_frag<T, DH>(at, tile, ic.value % DB, ic.value / DB); });
+        static_for<N>([&](auto ic) {
+          constexpr int n = decltype(ic)::value;
+          if constexpr (n + kAhead < N) ta[n + kAhead] = win_tr_frag<T, DH>(at, tile, (n + kAhead) % DB, (n + kAhead) / DB);
+          __builtin_amdgcn_sched_barrier(0);
+          acc[n % DB] = E::mfma(ta[n], bf[n / DB], acc[n % DB]);
+          __builtin_amdgcn_sched_barrier(0);
+        });
+      }
+      // one register set for the sums on both ways here: the compiler otherwise copies all of them in every tile
+#pragma unroll
+      for (int db = 0; db < DB; ++db) asm volatile("" : "+v"(acc[db]));
+      if (i + 1 < steps) finish(i + 1);
+      __syncthreads();
+      if (++t == t_lo + nt) t = t_lo;
+    }
   };
-
   if (steps > 0) {
     request(0);
     finish(0);
   }
   __syncthreads();
-  int t = t_lo;
-  for (int i = 0; i < steps; ++i) {
-    if (i + 1 < steps) request(i + 1);
-    const int p0 = t * kWinTile + off;  // positions p0 .. p0 + 63
-    if (exist > 0 && p0 + kWinTile > kw && p0 < kw + 32 - 1 + s.window)
-      compute(i, t, p0 >= kw + 31 && p0 + kWinTile - 1 < kw + s.window);
-    // one register set for the sums on both ways here: the compiler otherwise copies all of them in every tile
-#pragma unroll
-    for (int db = 0; db < DB; ++db) asm volatile("" : "+v"(acc[db]));
-    if (i + 1 < steps) finish(i + 1);
-    __syncthreads();
-    if (++t == t_lo + nt) t = t_lo;
-  }
+  if (for_dk)
+    run(std::true_type());
+  else
+    run(std::false_type());
+  const int which = for_dk ? 0 : 1;
   if (a.slots != nullptr && kw < a.sink_rows) {  // kw and sink_rows are multiples of 32
-    float* slot = a.slots + ((static_cast<size_t>(w.b * s.kv_heads + w.kvh) * a.n_slots) * 2 + WHICH) * a.sink_rows * DH;
+    float* slot = a.slots + ((static_cast<size_t>(w.b * s.kv_heads + w.kvh) * a.n_slots) * 2 + which) * a.sink_rows * DH;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -322,7 +350,9 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
         store_vec<float, 4>(slot + static_cast<size_t>(kj) * DH + 32 * db + 8 * rq + 4 * g, v);
       }
   }
-  win_store<T, DH>(out, ds.token, acc, DK ? s.scale : 1.0f, stage, lane, exist, rows, s.dim);
+  const WindowStride& ds = for_dk ? a.dks : a.dvs;
+  T* out = static_cast<T*>(for_dk ? a.dk : a.dv) + w.b * ds.batch + w.kvh * ds.head + kw * ds.token;
+  win_store<T, DH>(out, ds.token, acc, for_dk ? s.scale : 1.0f, reinterpret_cast<T*>(attn_lds) + wave * (32 * DH), lane, exist, rows, s.dim);
 }
 
 // ---- dK and dV of the first keys from the queries beyond their window ----

@@ -1100,7 +1100,7 @@ def _window_bwd_launchers() -> dict:
          for t in _ATTN_DTYPES.values() for form, block, lds in forms], prefer_intree=True)
     return {
         "dq": mk("dq", [(f"d{d}", 256, 4 * 64 * d * 2) for d in (64, 128)]),
-        "dkv": mk("dkv", [(f"d{d}", 256, 2 * (2 * 64 * d * 2 + 512)) for d in (64, 128)]),
+        "dkv": mk("dkv", [(f"d{d}", 512, 2 * (2 * 64 * d * 2 + 512) + 4 * 8192) for d in (64, 128)]),
         "sinks": mk("sinks", [(f"d{d}", 256, 4 * 4 * 32 * d * 2) for d in (64, 128)]),
         "join": mk("join", [(f"d{d}", 2 * d, 0) for d in (64, 128)]),
     }
@@ -1168,7 +1168,7 @@ def _window_backward_plan(q, k, v, out, dout, lse, scale, window, sinks, lengths
     ls, name = _window_bwd_launchers(), f"{_ATTN_DTYPES[q.dtype]}_d{dh}"
     bind = lambda which, grid: _bind(ls[which], f"window_attention_bwd_{which}_{name}", constants, grid)  # noqa: E731
     launches = [bind("dq", (_window_grid(units, cdiv(Sq, _WINDOW_ROWS >> share) * (group >> share)),)),
-                bind("dkv", (_window_grid(units, cdiv(Sk, _WINDOW_ROWS)), 2))]
+                bind("dkv", (_window_grid(units, cdiv(Sk, _WINDOW_ROWS)),))]
     if far:
         launches += [bind("sinks", (units * (sink_rows // 32) * (n_slots - 1),)), bind("join", (units * far,))]
     return tuple(launches), units * n_slots * 2 * sink_rows * dh
