@@ -8,10 +8,13 @@
 //               subtraction there; a row that does not exist gets -1e30 and 0, which makes its P zero.
 //               D takes O with what its rounding lost, where the forward kept that: in rows that see few keys
 //               dO V^T and D nearly cancel, and the rounding of O would be the largest error of dS.
-//   dK, dV      a wavefront owns 32 keys, a workgroup 128 of one key head, and walks the query tiles of 64 that see
-//               them through the window, head after head of the group.  The two gradients are separate halves of the
-//               launch: with both a wavefront's accumulators and operands outgrow the 256 registers it has at two
-//               wavefronts per SIMD.
+//   dK, dV      32 keys are a pair of wavefronts, a workgroup four pairs, 128 keys of one key head; it walks the query
+//               tiles of 64 that see them through the window, head after head of the group.  One wavefront of a pair
+//               makes S and P and adds to dV; it hands P to the other through LDS, in fp32, lane to lane (both hold the
+//               same rows and keys), which has made dP meanwhile and adds to dK.  Neither holds more than one
+//               gradient's sums and one operand, each product is made once and each tile is copied once; two
+//               separate kernels (five products, two copies of each tile) took 670 us where this takes 567 us
+//               ([4,32/8,4096,128], window 1024: 850 TFLOP/s over the four products).
 //   first keys  the keys j < sinks are also seen by every query beyond their window, hundreds of tiles for a few keys.
 //               That part is a kernel of its own: a workgroup takes 32 such keys and a share of those queries, each
 //               wavefront streams its own tiles of 32 queries, and the sums go to fp32 slots; the dK / dV kernel

@@ -12,6 +12,7 @@ from typing import Optional, Sequence
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 from torch.library import register_autograd
 
 from . import kernels
@@ -140,7 +141,7 @@ class RotaryFunction(Function):
 
     @staticmethod
     def backward(ctx, dq, dk):
-        return _rotary_gradient(ctx, kernels.rotary_axes, dq, dk)
+        return _rotary_gradient(ctx, rotary_axes, dq, dk)  # a gradient of it can be asked for in turn
 
 
 class WindowAttentionFunction(Function):
@@ -151,6 +152,7 @@ class WindowAttentionFunction(Function):
         return output
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout, *_):
         return _window_gradient(ctx, kernels.window_attention_backward, dout)
 

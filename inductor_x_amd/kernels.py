@@ -980,6 +980,13 @@ _WINDOW_LIMIT = 2**30      # windows and lengths beyond mean "all"
 _STRIDE_LIMIT = 2**23      # elements between two tokens: byte offsets inside a tile fit 31 bits
 
 
+def _strides3(t: torch.Tensor) -> tuple:
+    """Batch, head and token stride of a [batch, head, token, column] tensor; the stride of a single token, which can be
+    anything, becomes one that the tile copies can step past the end with."""
+    b, h, s, _ = t.stride()
+    return b, h, (s if t.shape[2] > 1 else t.shape[3])
+
+
 def _window_operands(q, k, v, scale, window, sinks, what="k and v"):
     """Checks that the window attention entry points share; returns (DH, window, sinks)."""
     _require(q.dtype == k.dtype == v.dtype and q.dtype in _ATTN_DTYPES, "q, k, v must share bf16 or fp16")
@@ -991,7 +998,7 @@ def _window_operands(q, k, v, scale, window, sinks, what="k and v"):
     for t in (q, k, v):
         _require(t.stride(-1) == 1 and _aligned(t) and all(s % 8 == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1),
                  "columns must be contiguous, and rows 16-byte aligned")
-    _require(k.stride(2) < _STRIDE_LIMIT and v.stride(2) < _STRIDE_LIMIT, "tokens lie too far apart")
+    _require(_strides3(k)[2] < _STRIDE_LIMIT and _strides3(v)[2] < _STRIDE_LIMIT, "tokens lie too far apart")
     _require(scale > 0 and math.isfinite(scale), "scale must be positive and finite")
     _require(window >= 1 and sinks >= 0, "window must be at least 1 and sinks at least 0")
     return 64 if D <= 64 else 128, min(int(window), _WINDOW_LIMIT), min(int(sinks), _WINDOW_LIMIT)
@@ -1063,8 +1070,8 @@ def window_attention(
     do not exist (a right-padded batch): their keys are hidden and not read, their rows of out are zero and
     of lse -inf.  lse is the natural logarithm of the sum of exp(score * scale).  keep_low adds a third tensor, what
     rounding lost of out, which makes the gradients of rows that see few keys more exact (window_attention_backward).
-    A NaN or infinity in an existing key or value row can also reach queries of the 63 positions before it, for
-    which it is hidden but lies in the same tile."""
+    A NaN or infinity in the key or value row of a position that exists also reaches queries up to 95 positions away
+    from those that see it: it shares a tile with keys that they see."""
     enqueue = _plan(("window", _form(q), _form(k), _form(v), scale, window, sinks, _form(lengths)),
                     _window_plan, q, k, v, scale, window, sinks, lengths)
     out = torch.empty_like(q)
@@ -1085,7 +1092,7 @@ def _window_plan(q, k, v, scale, window, sinks, lengths):
     share = shape[9]
     return _bind(
         _window_fwd_launcher(), f"window_attention_fwd_{_ATTN_DTYPES[q.dtype]}_d{dh}",
-        (*shape, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *torch.empty_like(q).stride()[:3]),
+        (*shape, *_strides3(q), *_strides3(k), *_strides3(v), *_strides3(torch.empty_like(q))),
         (_window_grid(units, cdiv(q.shape[2], _WINDOW_ROWS >> share) * (group >> share)),),
     )
 
@@ -1153,15 +1160,16 @@ def _window_backward_plan(q, k, v, out, dout, lse, scale, window, sinks, lengths
     B, N, Sq, D = q.shape
     Nk, Sk = k.shape[1:3]
     _require(lse.shape == (B, N, Sq) and lse.dtype == torch.float32 and lse.is_contiguous(), "lse must be the forward's [B, N, Sq] fp32")
-    _require(q.stride(2) < _STRIDE_LIMIT and dout.stride(2) < _STRIDE_LIMIT, "tokens lie too far apart")
+    _require(_strides3(q)[2] < _STRIDE_LIMIT and _strides3(dout)[2] < _STRIDE_LIMIT, "tokens lie too far apart")
     if q.numel() == 0:
         return (), 0
     units, group = B * Nk, N // Nk
     # queries that see the first keys from beyond their window: those at positions >= window
     far = min(sinks, Sk) if Sk > window else 0
+    _require(units * far < 2**31, "too many heads and first keys for one launch")
     sink_rows = 32 * cdiv(far, 32)
     n_slots = 1 + _sink_splits(units, sink_rows // 32, group * cdiv(min(Sq, Sk - window), 32)) if far else 0
-    strides = tuple(x for t in (q, k, v, out, dout, torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)) for x in t.stride()[:3])
+    strides = tuple(x for t in (q, k, v, out, dout, torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)) for x in _strides3(t))
     shape = _window_shape(q, k, window, sinks, scale)
     share = shape[9]
     constants = (*shape, n_slots, sink_rows, *strides)
@@ -1237,7 +1245,7 @@ def _window_decode_plan(q, k_cache, v_cache, lengths, scale, window, sinks):
     name = f"{_ATTN_DTYPES[q.dtype]}_d{dh}"
     enqueue = _bind(
         main, f"window_decode_{name}",
-        (q.stride(0), q.stride(1), *k_cache.stride()[:3], *v_cache.stride()[:3], N * D, D, Nk, group, splits, capacity, D, window,
+        (q.stride(0), q.stride(1), *_strides3(k_cache), *_strides3(v_cache), N * D, D, Nk, group, splits, capacity, D, window,
          sinks, float(scale) * 1.4426950408889634),
         (units * splits,))
     if splits == 1:

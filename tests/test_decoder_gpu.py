@@ -530,6 +530,38 @@ def test_plans_do_not_outlive_their_shapes(K):
     check_norm(K.add_rmsnorm_quant(part, whole, w[:512]), part.cpu(), whole.cpu(), w[:512].cpu(), 1e-6, 0)
 
 
+def test_one_token_with_any_stride(K):
+    announce("single tokens whose stride is no multiple of anything")
+    gen = torch.Generator().manual_seed(18)
+    raw = torch.randn(4, 2 * 2 * 64 + 64, generator=gen).to(BF).to(DEV)
+    odd = lambda t: t[: 2 * 2 * 64].as_strided((2, 2, 1, 64), (128, 64, 7, 1))  # noqa: E731
+    q, k, v, dout = (odd(t) for t in raw)
+    want = R.attention(q.cpu(), k.cpu(), v.cpu(), 0.125, 5, 2, None, dout.cpu())
+    out, lse, low = K.window_attention(q, k, v, 0.125, 5, 2, keep_low=True)
+    within(out, want["out"], R.attention_bound(want["out"], want["weight"], BF), "out")
+    for got, name in zip(K.window_attention_backward(q, k, v, out, dout, lse, 0.125, 5, 2, None, low), ("dq", "dk", "dv")):
+        within(got, want[name], R.attention_bound(want[name], want[name + "_weight"], BF), name)
+    got = K.window_attention_decode(q[:, :, 0], k, v, torch.ones(2, dtype=torch.int32, device=DEV), 0.125, 5, 2)
+    within(got, want["out"][:, :, 0], R.attention_bound(want["out"], want["weight"], BF)[:, :, 0], "decode")
+
+
+def test_second_gradients():
+    announce("a gradient of the rotary gradient; window attention refuses one")
+    from inductor_x_amd import decoder
+
+    x = torch.randn(1, 3, 2, 8, device=DEV, requires_grad=True)
+    at, freq = torch.arange(3, dtype=torch.int32, device=DEV).view(1, 3), torch.tensor([1.0, 0.1], device=DEV)
+    y, _ = decoder.rotary_axes(x, x.detach(), at, freq)
+    g = torch.autograd.grad(y.square().sum() / 2, x, create_graph=True)[0]
+    # y is a rotation of x, so half its square sum has the gradient x, and x^3 summed over it the gradient 3 x^2
+    assert torch.allclose(torch.autograd.grad((g**3).sum(), x)[0], 3 * x.detach() ** 2, rtol=1e-4, atol=1e-5)
+    q = torch.randn(1, 2, 4, 8, dtype=BF, device=DEV, requires_grad=True)
+    out = decoder.window_attention(q, q, q, 0.3, 2)
+    first = torch.autograd.grad(out.float().square().sum(), q, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        first.float().square().sum().backward()
+
+
 # ------------------------------------------------------------------------------------ used together
 class Layer(torch.nn.Module):
     """The attention half of a decoder layer on these operators: norm with an 8-bit result, projections from it, rotary
