@@ -6,8 +6,11 @@
 //               also forms the row statistics -lse / scale and -D, the values that the accumulators of Q K^T and
 //               dO V^T start from in the kernels after it, so that P = exp2(S' scale log2 e) and dS = P dP' need no
 //               subtraction there; a row that does not exist gets -1e30 and 0, which makes its P zero.
-//               D takes O with what its rounding lost, where the forward kept that: in rows that see few keys
-//               dO V^T and D nearly cancel, and the rounding of O would be the largest error of dS.
+//               D takes O with what its rounding lost, where the forward kept that, and blocks with at most two key
+//               tiles add it up from P and dP: in rows that see few keys dO V^T and D nearly cancel, and the
+//               roundings of O, and of P in the forward, would be the largest errors of dS.
+//               P and dS are rounded to the operand type for the products they enter (half a step each; the
+//               products take 16 bits), everything else is fp32.
 //   dK, dV      32 keys are a pair of wavefronts, a workgroup four pairs, 128 keys of one key head; it walks the query
 //               tiles of 64 that see them through the window, head after head of the group.  One wavefront of a pair
 //               makes S and P and adds to dV; it hands P to the other through LDS, in fp32, lane to lane (both hold the
@@ -76,8 +79,12 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
   win_load_row<T>(qf, static_cast<const T*>(a.q) + w.b * a.qs.batch + me.head * a.qs.head + qi * a.qs.token, s.dim, g);
   win_load_row<T>(dof, static_cast<const T*>(a.dout) + w.b * a.dos.batch + me.head * a.dos.head + qi * a.dos.token, s.dim, g);
   const float c2 = s.scale2;
-  float m2, delta = 0.f;
-  {
+  const size_t row = (static_cast<size_t>(w.b) * s.heads + me.head) * s.Sq + me.q0 + li;
+  const bool exists = li < me.exist;
+  const float m2 = (exists ? -a.lse[row] : -1e30f) * kWinLog2e;
+  float delta = 0.f;  // -D
+  const bool few = keys.n <= 2;
+  if (!few) {
     const long long o_at = w.b * a.os.batch + me.head * a.os.head + qi * a.os.token;
     x8_t of[DS];
     auto add = [&]() {
@@ -92,16 +99,6 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
       win_load_row<T>(of, static_cast<const T*>(a.low) + o_at, s.dim, g);
       add();
     }
-    delta = win_half_sum(delta);
-    const size_t row = (static_cast<size_t>(w.b) * s.heads + me.head) * s.Sq + me.q0 + li;
-    const bool exists = li < me.exist;
-    m2 = exists ? -a.lse[row] : -1e30f;
-    if (!exists) delta = 0.f;
-    if (g == 0 && li < me.rows) {
-      a.stats[row] = exists ? m2 / s.scale : -1e30f;
-      a.stats[static_cast<size_t>(s.batch) * s.heads * s.Sq + row] = delta;
-    }
-    m2 *= kWinLog2e;
   }
   const int p = me.p_lo + li;
 
@@ -160,10 +157,36 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
     });
   };
   request(0);
+  if (keys.n == 2) request(1);
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   __syncthreads();
+  if (few) {
+    // every key of the block is at hand: D = sum of P dP itself, free of the roundings that P and O took in the forward
+    for (int i = 0; i < keys.n; ++i) {
+      if (!me.active(keys, i)) continue;
+      const WinBases at = win_bases(lane_bases, (i & 1) * 4 * TILE);
+#pragma nounroll
+      for (int kb = 0; kb < 2; ++kb) {
+        f32x16_t sp[2];
+        win_zero(sp);
+#pragma unroll
+        for (int d = 0; d < DS; ++d) {
+          sp[0] = E::mfma(win_row_frag<T, DH>(at, 0, kb, d), qf[d], sp[0]);
+          sp[1] = E::mfma(win_row_frag<T, DH>(at, 2 * TILE, kb, d), dof[d], sp[1]);
+        }
+        me.hide(keys, i * kWinTile + 32 * kb, p, g, sp[0]);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) delta = fmaf(-__builtin_amdgcn_exp2f(fmaf(sp[0][r], c2, m2)), sp[1][r], delta);
+      }
+    }
+  }
+  delta = exists ? win_half_sum(delta) : 0.f;
+  if (g == 0 && li < me.rows) {
+    a.stats[row] = exists ? m2 / s.scale2 : -1e30f;
+    a.stats[static_cast<size_t>(s.batch) * s.heads * s.Sq + row] = delta;
+  }
   for (int i = 0; i < keys.n; ++i) {
-    if (i + 1 < keys.n) request(i + 1);
+    if (i + 1 < keys.n && !few) request(i + 1);
     if (me.active(keys, i)) compute(i, me.whole(keys, i));
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the next tile has landed
     __syncthreads();
