@@ -7,7 +7,10 @@
 // collected in the same sweep as the sum of squares and a row costs one workgroup reduction, its elements
 // stay in registers and memory is touched once.  A thread holds ITERS pieces of eight consecutive
 // columns, so 128 columns are 16 neighbouring lanes and their maximum four DPP steps.
-// Bound by memory: 7 bytes an element.
+//
+// Bound by memory, 7 bytes an element.  [16384, 4096] bf16 with 128-column scales, three input sets in turn: 85 us a call,
+// 5.5 TB/s (a plain copy of 4 GiB reaches 4.7); one input set replayed: 77 us.  A few rows cost the launch: 3.5 us.
+// The element-wise form for rows off the 16-byte grid takes 134 us where the wide one takes 40 ([8192, 4095] and 4096).
 #pragma once
 
 #include "common.h"

@@ -10,7 +10,8 @@
 //
 // Bound by memory: every element is read and written once.  128 angles a workgroup (two tokens of 64 pairs) rather
 // than one a thread, for more workgroups in flight: 59 against 63 us at [4,4096,32+8,128]; results leave with the
-// streaming hint, 59 against 63 us there and 23 against 29 us at [3,2047,24+24,96].
+// streaming hint, 59 against 63 us there (5.7 TB/s) and 23 against 29 us at [3,2047,24+24,96].  The element-wise form for
+// heads off the 16-byte grid takes 158 us where the wide one takes 50 (126 and 128 columns, one input set replayed).
 #pragma once
 
 #include "common.h"

@@ -13,6 +13,13 @@
 // No mask exists in memory: a wavefront compares positions in the few tiles that are neither wholly visible nor
 // wholly hidden to it.
 //
+// Measured on MI355X (bf16, 32 query heads on 8 key heads, 128 columns): 4096 queries at the end of 32768 keys, window
+// 8192, 128 first keys: 541 us, 1032 TFLOP/s over the visible pairs, 89 % of what a large library product reaches
+// (1165); 8192 queries, window 1024: 163 us, 795 TFLOP/s.  The matrix pipe is busy 51 % and 42 % of the cycles: beside it
+// run 6 (8) vector instructions per product, and every product reads one operand from LDS.  In short windows a block's
+// first loads and last stores are the rest, which the second workgroup of the CU covers in part.  A two-phase software
+// pipeline like attention_v5.h's was 4 % faster in rows of thousands of keys and 25 % slower in windows of 256.
+//
 // Operand layouts and the transposed products are those of attention.h.  Tiles travel memory -> LDS by direct
 // 16-byte loads, [64][DH] as they lie in memory with the chunks of a row swizzled; rows past the end and
 // columns past the head dimension arrive as zeros (bounds of the buffer descriptor).
