@@ -18,10 +18,12 @@
 //               gradient's sums and one operand, each product is made once and each tile is copied once; two
 //               separate kernels (five products, two copies of each tile) took 670 us where this takes 567 us
 //               ([4,32/8,4096,128], window 1024: 850 TFLOP/s over the four products).
-//   first keys  the keys j < sinks are also seen by every query beyond their window, hundreds of tiles for a few keys.
-//               That part is a kernel of its own: a workgroup takes 32 such keys and a share of those queries, each
-//               wavefront streams its own tiles of 32 queries, and the sums go to fp32 slots; the dK / dV kernel
-//               puts its part of these keys in slot 0 and a last kernel adds the slots in order and rounds once.
+//   first keys  the keys j < sinks are also seen by every query beyond their window, hundreds of tiles for a few keys
+//               in a long text.  There that part is a kernel of its own: a workgroup takes 32 such keys and a share of
+//               those queries, each wavefront streams its own tiles of 32 queries, and the sums go to fp32 slots; the
+//               dK / dV kernel puts its part of these keys in slot 0 and a last kernel adds the slots in order and
+//               rounds once.  Where those queries are few, or the first keys many, the dK / dV kernel walks them
+//               itself (the host's rule has both sides measured).
 // No atomics: results do not depend on the order of execution.
 #pragma once
 
@@ -34,7 +36,7 @@ struct WindowBwdArgs {
   void *dq, *dk, *dv;
   const float* lse;  // [B, N, Sq]
   float* stats;      // [2][B, N, Sq]: -lse / scale, -D
-  float* slots;      // [B * Nk][n_slots][2][sink_rows][DH] (dK without its scale, dV); null without such keys
+  float* slots;      // [B * Nk][n_slots][2][sink_rows][DH] (dK without its scale, dV); null: no kernel for first keys
   WindowShape shape;
   int n_slots, sink_rows;  // sink_rows: keys below `sinks`, rounded up to 32
   WindowStride qs, ks, vs, os, dos, dqs, dks, dvs;
@@ -226,9 +228,11 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
   f32x16_t acc[DB];
   win_zero(acc);
 
-  // query tiles that see a key of the block through the window
+  // query tiles that see a key of the block: through the window, or all from its first key on where the block holds
+  // first keys and there is no kernel for them
   const int t_lo = max(0, k0 - off) / kWinTile;
-  const int q_last = min(query_end - 1, min(k0 + kPairKeys, length) - 2 + s.window - off);
+  const int sinks = a.slots == nullptr ? s.sinks : 0;
+  const int q_last = min(query_end - 1, k0 < sinks ? query_end : min(k0 + kPairKeys, length) - 2 + s.window - off);
   const int nt = k0 < length && q_last >= 0 ? max(0, q_last / kWinTile - t_lo + 1) : 0;
   const int steps = nt * s.group;
   const int kj = kw + li, kc = min(kj, s.Sk - 1);
@@ -273,7 +277,7 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
     for (int i = 0; i < steps; ++i) {
       if (i + 1 < steps) request(i + 1);
       const int p0 = t * kWinTile + off;  // positions p0 .. p0 + 63
-      const bool active = exist > 0 && p0 + kWinTile > kw && p0 < kw + 32 - 1 + s.window;
+      const bool active = exist > 0 && p0 + kWinTile > kw && (p0 < kw + 32 - 1 + s.window || kw < sinks);
       const WinBases at = win_bases(lane_bases, (i & 1) * BUF);
       if (active) {
         // sp = start values + (Q or dO) (K or V)^T, fragments kAhead steps ahead, the order pinned by scheduling fences
@@ -297,14 +301,15 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
           __builtin_amdgcn_sched_barrier(0);
         });
         if constexpr (!FOR_DK) {
-          if (!(p0 >= kw + 31 && p0 + kWinTile - 1 < kw + s.window)) {
+          if (!(p0 >= kw + 31 && (p0 + kWinTile - 1 < kw + s.window || kw + 32 <= sinks))) {
 #pragma unroll
             for (int qb = 0; qb < 2; ++qb) {
-              const int d0 = kj - (p0 + 32 * qb + 4 * g);  // row r sees the key if d0 <= its offset < d0 + window
+              // row r sees the key if d0 <= its offset < d1
+              const int d0 = kj - (p0 + 32 * qb + 4 * g), d1 = kj < sinks ? kWinTile : d0 + s.window;
 #pragma unroll
               for (int r = 0; r < 16; ++r) {
                 const int o = 8 * (r >> 2) + (r & 3);
-                sp[qb][r] = (o < d0) | (o >= d0 + s.window) ? -__builtin_inff() : sp[qb][r];
+                sp[qb][r] = (o < d0) | (o >= d1) ? -__builtin_inff() : sp[qb][r];
               }
             }
           }

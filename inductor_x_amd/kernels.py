@@ -1164,8 +1164,15 @@ def _window_backward_plan(q, k, v, out, dout, lse, scale, window, sinks, lengths
     if q.numel() == 0:
         return (), 0
     units, group = B * Nk, N // Nk
-    # queries that see the first keys from beyond their window: those at positions >= window
-    far = min(sinks, Sk) if Sk > window else 0
+    # queries at positions >= window see the first keys from beyond their window.  Where they are few, the blocks of dK and
+    # dV that hold those keys walk them too (at most 8 steps of 64 rows more than any other block takes), and where the
+    # first keys are a quarter of the keys or more, so that many blocks share them; else they have a kernel of their own,
+    # split over the queries, and a join.  Measured, us with the kernel and without: [1,8/8,512,128] window 128 (6 steps
+    # more) 51 and 43, [3,8/8,777,128] (9) 56 and 52, [1,8/8,1536,128] (20) 55 and 70; [2,32/8,384,128] (8) 71 and 66,
+    # [2,32/8,448,128] (12) 73 and 75, [2,32/8,777,128] (36) 95 and 125; [2,32/8,4096,128] with 4, 512 and 1024 first keys
+    # 226 and 670, 507 and 620, 808 and 683, [1,8/8,2048,128] 58 and 87, 94 and 87, 123 and 100
+    merged = group * (cdiv(Sq, 64) - cdiv(window + _WINDOW_ROWS, 64)) <= 8 or 4 * sinks >= Sk
+    far = min(sinks, Sk) if Sk > window and not merged else 0
     _require(units * far < 2**31, "too many heads and first keys for one launch")
     sink_rows = 32 * cdiv(far, 32)
     n_slots = 1 + _sink_splits(units, sink_rows // 32, group * cdiv(min(Sq, Sk - window), 32)) if far else 0

@@ -277,6 +277,12 @@ WINDOW_CASES = [
     (1, 4, 2, 517, 1030, 128, 64, 128, None),
     (1, 2, 1, 900, 900, 128, 300, 900, None),          # everything is a first key
     (1, 2, 1, 900, 900, 64, 100, 701, None),           # first keys over eleven tiles
+    # gradients of the first keys from queries far beyond their window, a kernel of their own
+    (2, 8, 2, 777, 777, 128, 64, 4, [777, 300]),
+    (2, 5, 1, 400, 400, 64, 33, 2, [400, 30]),         # the second sequence ends inside the first window
+    (1, 6, 3, 600, 1500, 80, 100, 33, [1400]),
+    (1, 1, 1, 1200, 1200, 96, 200, 1, None),
+    (1, 2, 1, 900, 900, 64, 100, 200, None),           # seven blocks of first keys
 ]
 
 
