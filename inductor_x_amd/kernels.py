@@ -69,6 +69,10 @@ def _plan(key, make, *args):
     """The plan under `key`, made (and its operands checked) by make(*args) where there is none."""
     plan = _PLANS.get(key)
     if plan is None:
+        # a tensor in the key would be found again by its identity, whatever its value had become
+        for x in key:
+            for y in x if isinstance(x, tuple) else (x,):
+                _require(not isinstance(y, torch.Tensor), "arguments that are no operands must be plain numbers, not tensors")
         plan = make(*args)
         if len(_PLANS) >= _MAX_PLANS:
             _PLANS.clear()

@@ -504,6 +504,42 @@ def test_window_attention_repeats_captures_and_streams(K):
             assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_training_step_captured():
+    announce("rotary and window attention with their gradients in a replayed graph")
+    from inductor_x_amd import decoder
+
+    gen = torch.Generator().manual_seed(21)
+    B, S, N, Nk, D = 2, 300, 4, 2, 64
+    leaves = [torch.randn(B, S, n, D, generator=gen).to(BF).to(DEV).requires_grad_() for n in (N, Nk, Nk)]
+    dout = torch.randn(B, N, S, D, generator=gen).to(BF).to(DEV)
+    positions = torch.arange(S, device=DEV).expand(B, S).contiguous()
+    inv_freq = 100.0 ** (-torch.arange(D // 2, device=DEV).double() / D)
+    lengths = torch.tensor([300, 111], dtype=torch.int32, device=DEV)
+
+    def step():
+        q, k = decoder.rotary_axes(leaves[0], leaves[1], positions, inv_freq)
+        out = decoder.window_attention(q.transpose(1, 2), k.transpose(1, 2), leaves[2].transpose(1, 2), 0.125, 70, 3, lengths)
+        return (out.detach(), *torch.autograd.grad(out, leaves, dout))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()  # loads the code; its graph of gradients is gone when it returns
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for i in range(4):
+        with torch.no_grad():
+            for t in (*leaves, dout):
+                t.copy_(torch.randn(t.shape, generator=gen).to(BF))
+        lengths.copy_(torch.tensor([300 - 90 * i, 1 + i], dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, step())), f"replay {i}"
+
+
 def test_norm_and_rotary_captured(K):
     announce("norm and rotary in one replayed graph")
     gen = torch.Generator().manual_seed(14)

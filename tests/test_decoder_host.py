@@ -183,6 +183,43 @@ def test_window_refusals():
     assert (grads[1] == 0).all() and (grads[2] == 0).all() and grads[1].shape == k.shape
 
 
+def test_plain_arguments_are_no_tensors():
+    """A plan is found by its arguments: a tensor among them could change its value behind the plan's back."""
+    q, k, v = window_operands()
+    n = torch.ones(2, dtype=torch.int32)
+    h, w = torch.zeros(4, 256, dtype=BF), torch.ones(256, dtype=BF)
+    turn = torch.zeros(2, 3, 4, 64, dtype=BF), torch.zeros(2, 3, 2, 64, dtype=BF), torch.zeros(2, 2, 3, dtype=torch.int32), torch.ones(32)
+    for call in (lambda: K.window_attention(q, k, v, torch.tensor(0.1), 4),
+                 lambda: K.window_attention(q, k, v, 0.1, torch.tensor(4)),
+                 lambda: K.window_attention_backward(q, k, v, q, q, torch.zeros(2, 4, 8), 0.1, 4, torch.tensor(1)),
+                 lambda: K.window_attention_decode(q[:, :, 0].contiguous(), k, v, n, torch.tensor(0.1), 4),
+                 lambda: K.add_rmsnorm_quant(h, h, w, torch.tensor(1e-6)),
+                 lambda: K.rotary_axes(*turn, torch.tensor([20, 12]))):
+        with pytest.raises(ValueError, match="plain numbers"):
+            call()
+
+
+def test_first_keys_have_a_kernel_of_their_own_or_not(monkeypatch):
+    """Which kernels a backward pass consists of."""
+    bound = []
+    monkeypatch.setattr(K, "_bind", lambda l, symbol, constants, grid: bound.append(symbol) or (lambda *a: None))
+    monkeypatch.setattr(K, "_stream_of", lambda t: 0)
+
+    def kernels(B, N, Nk, Sq, Sk, window, sinks):
+        del bound[:]
+        q, k, v = window_operands(B, N, Nk, Sq, Sk)
+        K.window_attention_backward(q, k, v, q, q, torch.zeros(B, N, Sq), 0.1, window, sinks)
+        return len(bound)
+
+    assert kernels(1, 4, 4, 832, 832, 256, 4) == 2     # 7 tiles of queries more than a window's
+    assert kernels(1, 4, 4, 897, 897, 256, 4) == 4     # 9
+    assert kernels(1, 4, 1, 897, 897, 512, 4) == 4     # 5, of four heads
+    assert kernels(1, 4, 4, 897, 897, 256, 0) == 2     # no first keys
+    assert kernels(1, 4, 4, 897, 897, 256, 225) == 2   # a quarter of the keys
+    assert kernels(1, 4, 1, 256, 5000, 64, 4) == 2     # 1, of four heads
+    assert kernels(1, 4, 4, 897, 897, 897, 4) == 2     # none beyond the window
+
+
 def test_heads_of_a_workgroup():
     assert [K._largest_share(g) for g in (1, 2, 3, 4, 5, 6, 7, 8, 12, 16, 24, 40)] == [0, 1, 0, 2, 0, 1, 0, 2, 2, 2, 2, 2]
     for units in (1, 8, 64, 1000):
