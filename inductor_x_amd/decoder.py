@@ -12,7 +12,6 @@ from typing import Optional, Sequence
 
 import torch
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 from torch.library import register_autograd
 
 from . import kernels
@@ -86,10 +85,10 @@ def _needs_grad(*tensors: torch.Tensor) -> bool:
     return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
 
 
-# Gradients.  The same two steps (what the forward keeps, what the backward calls) serve the registered ops, which is how
-# a compilation sees them, and autograd functions over the kernels' entry points, which eager calls go through: the
-# dispatcher's way to a Python kernel and its gradient costs about 40 us of host time more, half of what a short text's
-# kernels run.
+# Gradients.  A compilation sees those of the registered ops.  Eager calls go through autograd functions over the kernels'
+# entry points: the dispatcher's way to a Python kernel and its gradient costs about 40 us of host time more, half of
+# what a short text's kernels run.  Rotary's function is here and shares its two steps (what the forward keeps, what
+# the backward calls) with the op; window attention's is csrc/mi_ops.cpp's.
 def _rotary_context(ctx, inputs, output):
     _, _, positions, inv_freq, sections, interleaved, inverse = inputs
     ctx.save_for_backward(positions, inv_freq)
@@ -144,19 +143,6 @@ class RotaryFunction(Function):
         return _rotary_gradient(ctx, rotary_axes, dq, dk)  # a gradient of it can be asked for in turn
 
 
-class WindowAttentionFunction(Function):
-    @staticmethod
-    def forward(ctx, *inputs):
-        output = kernels.window_attention(*inputs)
-        _window_context(ctx, inputs, output)
-        return output
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout, *_):
-        return _window_gradient(ctx, kernels.window_attention_backward, dout)
-
-
 def add_rmsnorm_quant(h: torch.Tensor, r: torch.Tensor, w: torch.Tensor, eps: float = 1e-6, group: int = 0):
     """(q, scales, h + r): kernels.add_rmsnorm_quant as a graph op.  Serving only: an 8-bit result has no gradient."""
     if torch.compiler.is_compiling():
@@ -179,8 +165,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     train = _needs_grad(q, k, v)
     if torch.compiler.is_compiling():
         return torch.ops.npu_graph.window_attention(q, k, v, scale, window, sinks, lengths, train)[0]
-    call = WindowAttentionFunction.apply if train else kernels.window_attention
-    return call(q, k, v, scale, window, sinks, lengths, train)[0]
+    if train:
+        return kernels.window_attention_with_gradients(q, k, v, scale, window, sinks, lengths)
+    return kernels.window_attention(q, k, v, scale, window, sinks, lengths)[0]
 
 
 def window_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,

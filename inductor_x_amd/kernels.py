@@ -17,7 +17,7 @@ from typing import Optional
 
 import torch
 
-from . import codecache, config
+from . import codecache, config, launcher
 from .hip_heuristics import (
     CachingLauncher,
     LaunchConfig,
@@ -59,47 +59,47 @@ def _check_here(*tensors: torch.Tensor) -> None:
 
 
 # Launch plans of the decoder-layer operators.  Checking operands and choosing a launch costs more host time than the launch
-# itself, and a model calls with few distinct shapes: what follows from shapes, strides, types, alignment and the
-# arguments that are no tensors is settled once per such key.  Nothing about a tensor's contents or place is kept.
-_PLANS: dict = {}
-_MAX_PLANS = 4096
+# itself, and a model calls with few distinct shapes: what follows from shapes, strides, types, devices, alignment and the
+# arguments that are no tensors is settled once per such key by the functions named _..._plan, and csrc/mi_ops.cpp answers
+# the calls.  A plan is (launches, outputs, returned): kernels with the places of their pointers among operands
+# and outputs (-1: null), what to allocate, and how many of the outputs are results (the others are workspaces).
+@functools.lru_cache(maxsize=None)
+def _operators():
+    """call(operator, *arguments), after telling the native side which function makes each operator's plans."""
+    ops = launcher.load_operators()
+    makers = {"NORM": (_norm_quant_plan, (0, 1, 2)), "ROTARY": (_rotary_plan, (0, 1, 2, 3)), "WINDOW": (_window_plan, (0, 1, 2, 6)),
+              "WINDOW_BACKWARD": (_window_backward_plan, (0, 1, 2, 3, 4, 5, 9, 10)), "DECODE": (_window_decode_plan, (0, 1, 2, 3))}
+    assert tuple(makers) == _OPERATOR_NAMES
+    numbers = [ops.operator(*entry) for entry in makers.values()]
+    assert numbers == list(range(len(makers)))
+    ops.window(_WINDOW, _WINDOW_BACKWARD)
+    return ops
 
 
-def _plan(key, make, *args):
-    """The plan under `key`, made (and its operands checked) by make(*args) where there is none."""
-    plan = _PLANS.get(key)
-    if plan is None:
-        # a tensor in the key would be found again by its identity, whatever its value had become
-        for x in key:
-            for y in x if isinstance(x, tuple) else (x,):
-                _require(not isinstance(y, torch.Tensor), "arguments that are no operands must be plain numbers, not tensors")
-        plan = make(*args)
-        if len(_PLANS) >= _MAX_PLANS:
-            _PLANS.clear()
-        _PLANS[key] = plan
-    return plan
+_OPERATOR_NAMES = ("NORM", "ROTARY", "WINDOW", "WINDOW_BACKWARD", "DECODE")
+_NORM, _ROTARY, _WINDOW, _WINDOW_BACKWARD, _DECODE = range(5)
 
 
 def _bind(l: CachingLauncher, symbol: str, constants, grid):
-    """enqueue(stream, *pointers) for a kernel of a family (launcher.Function.prepare).  A family's code object is loaded
+    """What a plan keeps of a launch but its pointers (launcher.Function.describe).  A family's code object is loaded
     on one GPU, the one that was current at its first use (one process per GPU)."""
     home = l.__dict__.setdefault("_home", torch.cuda.current_device())
     _require(home == torch.cuda.current_device(), f"this process runs {l.name} on GPU {home}")
     cfg, fn = l.launchers[_find(l, symbol)]
-    return fn.prepare(l.signature, constants, grid, (cfg.block,), cfg.lds_bytes)
+    return fn.describe(l.signature, constants, grid, (cfg.block,), cfg.lds_bytes)
 
 
-def _form(t: Optional[torch.Tensor]):
-    """What a plan depends on in an operand."""
-    return None if t is None else (t.shape, t.stride(), t.dtype, t.device, t.data_ptr() & 15)
+def _output(shape, dtype: torch.dtype, zero: bool = False) -> tuple:
+    """A contiguous output of a plan."""
+    shape, strides = tuple(shape), [1]
+    for n in shape[:0:-1]:
+        strides.append(strides[-1] * max(n, 1))
+    return shape, tuple(strides[::-1][: len(shape)]), dtype, zero
 
 
-def _stream_of(t: torch.Tensor) -> int:
-    """The current stream of the tensor's device, which has to be the current one."""
-    index = t.device.index
-    if index != torch._C._cuda_getDevice():
-        raise ValueError("tensors must live on the current GPU")
-    return torch._C._cuda_getCurrentRawStream(index)
+def _output_like(t: torch.Tensor, zero: bool = False) -> tuple:
+    """An output of a plan in the layout that torch.empty_like gives."""
+    return tuple(t.shape), torch.empty_like(t).stride(), t.dtype, zero
 
 
 # ---------------------------------------------------------------------------
@@ -412,13 +412,7 @@ def add_rmsnorm_quant(
     all are zero, never below the smallest normal number.  A NaN or infinity in a row gives that row (every
     128 columns of it that it reaches) NaN, as the formula does.
     h, r: bf16 or fp16 of one shape with contiguous columns and evenly spaced rows; w one vector of the same type."""
-    enqueue, scales_shape = _plan(("norm", _form(h), _form(r), _form(w), eps, group), _norm_quant_plan, h, r, w, eps, group)
-    s = h.new_empty(h.shape)
-    q = h.new_empty(h.shape, dtype=torch.float8_e4m3fn)
-    scales = h.new_empty(scales_shape, dtype=torch.float32)
-    if enqueue is not None:
-        enqueue(_stream_of(h), h.data_ptr(), r.data_ptr(), w.data_ptr(), q.data_ptr(), scales.data_ptr(), s.data_ptr())
-    return q, scales, s
+    return _operators().call(_NORM, h, r, w, eps, group)
 
 
 def _norm_quant_plan(h, r, w, eps, group):
@@ -431,15 +425,16 @@ def _norm_quant_plan(h, r, w, eps, group):
     _require(0 < cols <= 32768, "row length must lie in 1..32768")
     scales_shape = h.shape[:-1] + (cdiv(cols, 128) if group else 1,)
     rows = h.numel() // cols
+    outputs = (_output(h.shape, torch.float8_e4m3fn), _output(scales_shape, torch.float32), _output(h.shape, h.dtype))
     if rows == 0:
-        return None, scales_shape
+        return (), outputs, 3
     _require(rows < 2**31, "too many rows")
     hs, rs = _as_rows(h, "h").stride(0), _as_rows(r, "r").stride(0)
     # rows of 8 elements' multiples on 16-byte addresses move in 16-byte pieces, any others element by element
     wide = (cols | hs | rs) % 8 == 0 and all(_aligned(t) for t in (h, r, w))
     b, t, i = next(v for v in _NORM_QUANT_VARIANTS if cols <= v[1] * v[2] * 8)
     symbol = f"add_rmsnorm_quant_{_ATTN_DTYPES[h.dtype]}_b{b}_t{t}_i{i}{'_g128' if group else ''}{'' if wide else '_odd'}"
-    return _bind(_norm_quant_launcher(), symbol, (rows, cols, hs, rs, float(eps)), (cdiv(rows, b // t),)), scales_shape
+    return ((*_bind(_norm_quant_launcher(), symbol, (rows, cols, hs, rs, float(eps)), (cdiv(rows, b // t),)), range(6)),), outputs, 3
 
 
 def _snap_split_plan(plan: SplitPlan, rows: int, cols: int) -> SplitPlan:
@@ -928,12 +923,7 @@ def rotary_axes(
     with interleaved=True (column 2 p, column 2 p + 1).  inverse turns back: the gradient of the rotation.
     Angles are formed in 64 bits, the products in 32, rounded once."""
     sections = None if sections is None else tuple(sections)
-    enqueue = _plan(("rotary", _form(q), _form(k), _form(positions), _form(inv_freq), sections, interleaved, inverse),
-                    _rotary_plan, q, k, positions, inv_freq, sections, interleaved, inverse)
-    q_out, k_out = torch.empty_like(q), torch.empty_like(k)
-    if enqueue is not None:
-        enqueue(_stream_of(q), q.data_ptr(), q_out.data_ptr(), k.data_ptr(), k_out.data_ptr(), positions.data_ptr(), inv_freq.data_ptr())
-    return q_out, k_out
+    return _operators().call(_ROTARY, q, k, positions, inv_freq, sections, interleaved, inverse)
 
 
 def _rotary_plan(q, k, positions, inv_freq, sections, interleaved, inverse):
@@ -956,8 +946,9 @@ def _rotary_plan(q, k, positions, inv_freq, sections, interleaved, inverse):
     sections = [pairs] if sections is None else [int(x) for x in sections]
     _require(len(sections) == axes and min(sections) >= 0 and sum(sections) == pairs, "sections must give every axis its share of the pairs")
     ends = [sum(sections[: i + 1]) for i in range(axes - 1)] + [pairs] * (4 - axes)
+    outputs = (_output_like(q), _output_like(k))
     if q.numel() + k.numel() == 0:
-        return None
+        return (), outputs, 2
     tokens = B * S
     _require(tokens < 2**31 and N + k.shape[2] < 2**16, "extents must fit int32 indexing")
     vec = 16 // q.element_size()
@@ -969,12 +960,13 @@ def _rotary_plan(q, k, positions, inv_freq, sections, interleaved, inverse):
     wide = (2 * pairs) % step == 0 and D % vec == 0 and all(x % vec == 0 for x in strides) and _aligned(q) and _aligned(k)
     # tokens per workgroup: 128 angles' worth, fewer where that would leave compute units idle
     per_block = max(1, min(128 // pairs, tokens // (2 * config.hardware().cu_count)))
-    return _bind(
+    launch = _bind(
         _rotary_launcher(), f"rotary_axes_{_ROTARY_DTYPES[q.dtype]}_{'beside' if interleaved else 'half'}{'' if wide else '_odd'}",
         (*strides, N, k.shape[2], positions.dtype == torch.int64, inv_freq.dtype == torch.float64, tokens, S, D, 2 * pairs,
          ends[0], ends[1], ends[2], per_block, -1.0 if inverse else 1.0),
         (cdiv(tokens, per_block),),
     )
+    return ((*launch, (0, 4, 1, 5, 2, 3)),), outputs, 2
 
 
 # ---------------------------------------------------------------------------
@@ -1076,29 +1068,23 @@ def window_attention(
     rounding lost of out, which makes the gradients of rows that see few keys more exact (window_attention_backward).
     A NaN or infinity in the key or value row of a position that exists also reaches queries up to 95 positions away
     from those that see it: it shares a tile with keys that they see."""
-    enqueue = _plan(("window", _form(q), _form(k), _form(v), scale, window, sinks, _form(lengths)),
-                    _window_plan, q, k, v, scale, window, sinks, lengths)
-    out = torch.empty_like(q)
-    low = torch.empty_like(q) if keep_low else None
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
-    if enqueue is not None:
-        enqueue(_stream_of(q), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), low.data_ptr() if keep_low else 0,
-                lse.data_ptr(), lengths.data_ptr() if lengths is not None else 0)
-    return (out, lse, low) if keep_low else (out, lse)
+    return _operators().call(_WINDOW, q, k, v, scale, window, sinks, lengths, keep_low)
 
 
-def _window_plan(q, k, v, scale, window, sinks, lengths):
+def _window_plan(q, k, v, scale, window, sinks, lengths, keep_low):
     dh, window, sinks = _window_check(q, k, v, scale, window, sinks, lengths)
+    outputs = (_output_like(q), _output(q.shape[:3], torch.float32)) + ((_output_like(q),) if keep_low else ())
     if q.numel() == 0:
-        return None
+        return (), outputs, len(outputs)
     units, group = q.shape[0] * k.shape[1], q.shape[1] // k.shape[1]
     shape = _window_shape(q, k, window, sinks, scale)
     share = shape[9]
-    return _bind(
+    launch = _bind(
         _window_fwd_launcher(), f"window_attention_fwd_{_ATTN_DTYPES[q.dtype]}_d{dh}",
         (*shape, *_strides3(q), *_strides3(k), *_strides3(v), *_strides3(torch.empty_like(q))),
         (_window_grid(units, cdiv(q.shape[2], _WINDOW_ROWS >> share) * (group >> share)),),
     )
+    return ((*launch, (0, 1, 2, 4, 6 if keep_low else -1, 5, 3)),), outputs, len(outputs)
 
 
 @functools.lru_cache(maxsize=None)
@@ -1130,24 +1116,16 @@ def window_attention_backward(
     """Gradients (dq, dk, dv) of window_attention; out, lse and (if kept) low are the forward's, dout [B, N, Sq, D] in the
     type of q (strides as for q).  dk and dv are summed over the query heads that share a key head, in fp32 and in a fixed
     order.  Rows that do not exist get zeros, and what dout holds there is not read into anything else."""
-    launches, slots_size = _plan(
-        ("window backward", _form(q), _form(k), _form(v), _form(out), _form(dout), _form(lse), scale, window, sinks, _form(lengths),
-         _form(low)),
-        _window_backward_plan, q, k, v, out, dout, lse, scale, window, sinks, lengths, low)
-    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
-    if not launches:
-        return dq, dk.zero_(), dv.zero_()
-    # both halves of the statistics and the slots of the first keys in one piece of memory
-    rows = lse.numel()
-    work = torch.empty(2 * rows + slots_size, dtype=torch.float32, device=q.device)
-    at = work.data_ptr()
-    st = _stream_of(q)
-    pointers = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), low.data_ptr() if low is not None else 0, dout.data_ptr(),
-                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), lse.data_ptr(), at, at + 8 * rows if slots_size else 0,
-                lengths.data_ptr() if lengths is not None else 0)
-    for enqueue in launches:
-        enqueue(st, *pointers)
-    return dq, dk, dv
+    return _operators().call(_WINDOW_BACKWARD, q, k, v, out, dout, lse, scale, window, sinks, lengths, low)
+
+
+def window_attention_with_gradients(
+    q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, window: int, sinks: int = 0,
+    lengths: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """The output of window_attention with window_attention_backward as its gradient for autograd (keep_low included); the
+    gradient itself has none and says so when one is asked for."""
+    return _operators().window_attention_with_gradients(q, k, v, scale, window, sinks, lengths)
 
 
 def _window_backward_plan(q, k, v, out, dout, lse, scale, window, sinks, lengths, low):
@@ -1166,7 +1144,7 @@ def _window_backward_plan(q, k, v, out, dout, lse, scale, window, sinks, lengths
     _require(lse.shape == (B, N, Sq) and lse.dtype == torch.float32 and lse.is_contiguous(), "lse must be the forward's [B, N, Sq] fp32")
     _require(_strides3(q)[2] < _STRIDE_LIMIT and _strides3(dout)[2] < _STRIDE_LIMIT, "tokens lie too far apart")
     if q.numel() == 0:
-        return (), 0
+        return (), (_output_like(q), _output_like(k, zero=True), _output_like(v, zero=True)), 3
     units, group = B * Nk, N // Nk
     # queries at positions >= window see the first keys from beyond their window.  Where they are few, the blocks of dK and
     # dV that hold those keys walk them too (at most 8 steps of 64 rows more than any other block takes), and where the
@@ -1180,6 +1158,7 @@ def _window_backward_plan(q, k, v, out, dout, lse, scale, window, sinks, lengths
     _require(units * far < 2**31, "too many heads and first keys for one launch")
     sink_rows = 32 * cdiv(far, 32)
     n_slots = 1 + _sink_splits(units, sink_rows // 32, group * cdiv(min(Sq, Sk - window), 32)) if far else 0
+    results = [_output_like(t) for t in (q, k, v)]
     strides = tuple(x for t in (q, k, v, out, dout, torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)) for x in _strides3(t))
     shape = _window_shape(q, k, window, sinks, scale)
     share = shape[9]
@@ -1188,9 +1167,12 @@ def _window_backward_plan(q, k, v, out, dout, lse, scale, window, sinks, lengths
     bind = lambda which, grid: _bind(ls[which], f"window_attention_bwd_{which}_{name}", constants, grid)  # noqa: E731
     launches = [bind("dq", (_window_grid(units, cdiv(Sq, _WINDOW_ROWS >> share) * (group >> share)),)),
                 bind("dkv", (_window_grid(units, cdiv(Sk, _WINDOW_ROWS)),))]
+    outputs = [*results, _output((2, B, N, Sq), torch.float32)]
     if far:
         launches += [bind("sinks", (units * (sink_rows // 32) * (n_slots - 1),)), bind("join", (units * far,))]
-    return tuple(launches), units * n_slots * 2 * sink_rows * dh
+        outputs.append(_output((units, n_slots, 2, sink_rows, dh), torch.float32))
+    pointers = (0, 1, 2, 3, 7, 4, 8, 9, 10, 5, 11, 12 if far else -1, 6)
+    return tuple((*launch, pointers) for launch in launches), tuple(outputs), 3
 
 
 @functools.lru_cache(maxsize=None)
@@ -1223,18 +1205,7 @@ def window_attention_decode(
     the token sits at position lengths[b] - 1 and sees the keys j >= lengths[b] - window and j < sinks; values past
     the capacity count as the capacity.  A sequence of length 0 gets zeros.  What lies behind a sequence's
     length is not read."""
-    enqueue, join, part_size = _plan(
-        ("decode", _form(q), _form(k_cache), _form(v_cache), _form(lengths), scale, window, sinks),
-        _window_decode_plan, q, k_cache, v_cache, lengths, scale, window, sinks)
-    out = q.new_empty(q.shape)
-    if enqueue is None:
-        return out.zero_()
-    st = _stream_of(q)
-    part = torch.empty(part_size, dtype=torch.float32, device=q.device) if part_size else None
-    enqueue(st, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), part.data_ptr() if part_size else 0, lengths.data_ptr())
-    if part_size:
-        join(st, part.data_ptr(), out.data_ptr(), lengths.data_ptr())
-    return out
+    return _operators().call(_DECODE, q, k_cache, v_cache, lengths, scale, window, sinks)
 
 
 def _window_decode_plan(q, k_cache, v_cache, lengths, scale, window, sinks):
@@ -1246,7 +1217,7 @@ def _window_decode_plan(q, k_cache, v_cache, lengths, scale, window, sinks):
     Nk, capacity = k_cache.shape[1:3]
     _require(capacity < _WINDOW_LIMIT, "capacity must stay below 2**30")
     if B == 0 or capacity == 0:
-        return None, None, 0
+        return (), (_output(q.shape, q.dtype, zero=True),), 1
     group = N // Nk
     units = B * Nk * cdiv(group, 16)
     tiles = cdiv(min(window, capacity), 32) + cdiv(min(sinks, max(capacity - window, 0)), 32)
@@ -1254,14 +1225,16 @@ def _window_decode_plan(q, k_cache, v_cache, lengths, scale, window, sinks):
     _require(units * splits < 2**31, "too many heads and sequences for one launch")
     main, join = _window_decode_launchers()
     name = f"{_ATTN_DTYPES[q.dtype]}_d{dh}"
-    enqueue = _bind(
+    launch = _bind(
         main, f"window_decode_{name}",
         (q.stride(0), q.stride(1), *_strides3(k_cache), *_strides3(v_cache), N * D, D, Nk, group, splits, capacity, D, window,
          sinks, float(scale) * 1.4426950408889634),
         (units * splits,))
+    result = _output(q.shape, q.dtype)
     if splits == 1:
-        return enqueue, None, 0
-    return enqueue, _bind(join, f"window_decode_join_{name}", (N, splits, D, N * D, D), (B * N,)), B * N * splits * (dh + 2)
+        return ((*launch, (0, 1, 2, 4, -1, 3)),), (result,), 1
+    second = _bind(join, f"window_decode_join_{name}", (N, splits, D, N * D, D), (B * N,))
+    return ((*launch, (0, 1, 2, 4, 5, 3)), (*second, (5, 4, 3))), (result, _output((B, N, splits, dh + 2), torch.float32)), 1
 
 
 # ---------------------------------------------------------------------------

@@ -141,6 +141,33 @@ def _load_fastcall(lib: ctypes.CDLL):
     return _fast
 
 
+OPS_PATH = os.path.join(_HERE, "_mi_ops.so")
+_ops = None
+
+
+def load_operators():
+    """The host side of the decoder-layer operators (csrc/mi_ops.cpp), bound to the loaded library."""
+    global _ops
+    lib = load_library()
+    with _lib_lock:
+        if _ops is None:
+            import importlib.machinery
+            import importlib.util
+
+            if not os.path.exists(OPS_PATH):
+                raise LauncherError(f"{OPS_PATH} not found: build it first (python -c 'import __graft_entry__ as g; g.build()')")
+            loader = importlib.machinery.ExtensionFileLoader("_mi_ops", OPS_PATH)
+            mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("_mi_ops", loader))
+            loader.exec_module(mod)
+            mod.bind(ctypes.cast(lib.mi_launch_packed, ctypes.c_void_p).value, _launch_failed, globals())
+            _ops = mod
+        return _ops
+
+
+def _launch_failed(name: str, grid: tuple, block: tuple, lds_bytes: int, err: int) -> None:
+    raise LauncherError(f"launch of {name} grid={grid} block={block} lds={lds_bytes} failed: HIP error {err} ({error_string(err)})")
+
+
 def error_string(err: int) -> str:
     return load_library().mi_error_string(err).decode()
 
@@ -259,33 +286,15 @@ class Function:
                 f"HIP error {err} ({error_string(err)})"
             )
 
-    def prepare(self, signature: str, constants: Sequence, grid: Sequence[int], block: Sequence[int], lds_bytes: int = 0):
-        """enqueue(stream, *pointers) for a kernel whose parameters are leading pointers and then constants: what does
-        not change between calls of one shape (grid, constants in their packed form) is settled once."""
+    def describe(self, signature: str, constants: Sequence, grid: Sequence[int], block: Sequence[int], lds_bytes: int = 0) -> tuple:
+        """(function, grid + block + LDS bytes, constants in their packed form, name) of a kernel whose parameters are leading
+        pointers and then constants: what a plan of csrc/mi_ops.cpp keeps of a launch."""
         lead = len(signature) - len(constants)
         if lead < 0 or set(signature[:lead]) - {"P"} or set(signature) - _VALID:
             raise LauncherError(f"{self.name}: signature {signature!r} does not start with {lead} pointers")
         tail = struct.Struct("@" + signature).pack(*([0] * lead), *constants)[8 * lead:]
-        pack = struct.Struct("@" + "P" * lead).pack
-        (gx, gy, gz), (bx, by, bz) = (tuple(grid) + (1, 1))[:3], (tuple(block) + (1, 1))[:3]
-        fast = self._fast.launch if self._fast is not None else None
-        handle, raw, name, lib = self._handle, self._raw_handle, self.name, self._lib
-
-        def enqueue(stream: int, *pointers: int) -> None:
-            segment = pack(*pointers) + tail
-            if launch_log is not None:
-                launch_log.append(name)
-            if fast is not None:
-                err = fast(raw, gx, gy, gz, bx, by, bz, lds_bytes, stream, segment)
-            else:
-                err = lib.mi_launch_packed(handle, gx, gy, gz, bx, by, bz, lds_bytes, ctypes.c_void_p(stream), segment, len(segment))
-            if err != 0:
-                raise LauncherError(
-                    f"launch of {name} grid=({gx},{gy},{gz}) block=({bx},{by},{bz}) lds={lds_bytes} failed: "
-                    f"HIP error {err} ({error_string(err)})"
-                )
-
-        return enqueue
+        dims = (*(tuple(grid) + (1, 1))[:3], *(tuple(block) + (1, 1))[:3], lds_bytes)
+        return self._raw_handle, dims, tail, self.name
 
     def launch_with_library_scratch(
         self,

@@ -540,6 +540,22 @@ def test_training_step_captured():
         assert all(torch.equal(a, b) for a, b in zip(held, step())), f"replay {i}"
 
 
+def test_launches_are_logged(K):
+    announce("the symbols of a call's launches, with gradients too")
+    from inductor_x_amd import decoder, launcher
+
+    q, k, v, dout = (t.to(DEV) for t in window_operands(1, 4, 2, 450, 450, 64, BF, False, seed=14))
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    launcher.launch_log = []
+    try:
+        decoder.window_attention(*leaves, 0.1, 64, 4).backward(dout)
+        K.window_attention_decode(q.detach()[:, :, 0], k.detach(), v.detach(), torch.full((1,), 450, dtype=torch.int32, device=DEV), 0.1, 64)
+    finally:
+        log, launcher.launch_log = launcher.launch_log, None
+    kinds = ["fwd", "bwd_dq", "bwd_dkv", "bwd_sinks", "bwd_join"]
+    assert log == [f"window_attention_{x}_bf16_d64" for x in kinds] + ["window_decode_bf16_d64"]
+
+
 def test_norm_and_rotary_captured(K):
     announce("norm and rotary in one replayed graph")
     gen = torch.Generator().manual_seed(14)

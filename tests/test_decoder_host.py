@@ -1,5 +1,6 @@
 """Argument checks and shape functions of the decoder-layer operators, without a GPU: the device check and the binding of a
 launch are replaced, everything between them is the product's."""
+import numpy as np
 import pytest
 import torch
 
@@ -20,7 +21,9 @@ def no_gpu(monkeypatch):
     monkeypatch.setattr(K, "_check_cuda", lambda *t: None)
     monkeypatch.setattr(K, "_check_here", lambda *t: None)
     monkeypatch.setattr(K, "_bind", bound)
-    monkeypatch.setattr(K, "_PLANS", {})
+    K._operators().forget()
+    yield
+    K._operators().forget()
 
 
 def test_tensors_on_the_host_are_refused(monkeypatch):
@@ -199,16 +202,42 @@ def test_plain_arguments_are_no_tensors():
             call()
 
 
+def test_arguments_of_other_kinds():
+    q, k, v = window_operands()
+    for scale in (np.float32(0.1), np.float64(0.1), 1):
+        with pytest.raises(Launched):
+            K.window_attention(q, k, v, scale, np.int64(4), True)
+    for call in (lambda: K.window_attention(q, k, v, "0.1", 4), lambda: K.window_attention(q, k, v, None, 4),
+                 lambda: K.window_attention_with_gradients(q, k, v, "0.1", 4), lambda: K.window_attention_with_gradients(q, k, None, 0.1, 4),
+                 lambda: K.window_attention_with_gradients(q, k, v, 0.1, 4, 1, [8, 8])):
+        with pytest.raises((TypeError, ValueError)):
+            call()
+    with pytest.raises(ValueError, match="plain numbers"):
+        K.window_attention_with_gradients(q, k, v, torch.tensor(0.1), 4)
+    with pytest.raises(ValueError, match="scale"):  # a refusal passes through the native side unchanged
+        K.window_attention_with_gradients(q, k, v, -1.0, 4)
+    with pytest.raises(Launched):
+        K.window_attention_with_gradients(q, k, v, 0.1, 4)
+
+
+def test_more_shapes_than_plans_are_kept():
+    q = torch.empty(0, 4, 1, 64, dtype=BF)
+    for n in range(1, 4200):  # no sequences: results and no launch
+        kv = torch.empty(0, 2, n, 64, dtype=BF)
+        out, lse = K.window_attention(q, kv, kv, 0.1, n)
+        assert out.shape == q.shape and lse.shape == q.shape[:3]
+
+
 def test_first_keys_have_a_kernel_of_their_own_or_not(monkeypatch):
     """Which kernels a backward pass consists of."""
     bound = []
-    monkeypatch.setattr(K, "_bind", lambda l, symbol, constants, grid: bound.append(symbol) or (lambda *a: None))
-    monkeypatch.setattr(K, "_stream_of", lambda t: 0)
+    monkeypatch.setattr(K, "_bind", lambda l, symbol, constants, grid: bound.append(symbol) or (0, (1,) * 6 + (0,), b"", symbol))
 
     def kernels(B, N, Nk, Sq, Sk, window, sinks):
         del bound[:]
         q, k, v = window_operands(B, N, Nk, Sq, Sk)
-        K.window_attention_backward(q, k, v, q, q, torch.zeros(B, N, Sq), 0.1, window, sinks)
+        with pytest.raises(ValueError, match="current GPU"):  # nothing is enqueued for tensors of the host
+            K.window_attention_backward(q, k, v, q, q, torch.zeros(B, N, Sq), 0.1, window, sinks)
         return len(bound)
 
     assert kernels(1, 4, 4, 832, 832, 256, 4) == 2     # 7 tiles of queries more than a window's
