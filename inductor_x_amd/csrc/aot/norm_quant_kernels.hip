@@ -1,5 +1,5 @@
 // Instantiations of the residual add + RMS norm with an 8-bit result (norm_quant.h): element type, threads per
-// row and pieces per thread, one scale per row or per 128 columns, wide or element-wise access.
+// row and pieces per thread, one scale per row or per 128 columns, aligned or unaligned access.
 #include "../mi/norm_quant.h"
 
 using namespace mi;
@@ -16,6 +16,8 @@ using namespace mi;
   NORM_QUANT(TN, T, BLOCK, TPR, ITERS, , false, _odd, false)   \
   NORM_QUANT(TN, T, BLOCK, TPR, ITERS, _g128, true, _odd, false)
 #define NORM_QUANT_SIZES(TN, T)            \
+  NORM_QUANT_FORMS(TN, T, 256, 16, 1)      \
+  NORM_QUANT_FORMS(TN, T, 256, 32, 1)      \
   NORM_QUANT_FORMS(TN, T, 256, 64, 1)      \
   NORM_QUANT_FORMS(TN, T, 256, 64, 2)      \
   NORM_QUANT_FORMS(TN, T, 256, 256, 1)     \

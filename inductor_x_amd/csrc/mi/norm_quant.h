@@ -10,7 +10,9 @@
 //
 // Bound by memory, 7 bytes an element.  [16384, 4096] bf16 with 128-column scales, three input sets in turn: 85 us a call,
 // 5.5 TB/s (a plain copy of 4 GiB reaches 4.7); one input set replayed: 77 us.  A few rows cost the launch: 3.5 us.
-// The element-wise form for rows off the 16-byte grid takes 134 us where the wide one takes 40 ([8192, 4095] and 4096).
+// Rows off the 16-byte grid move in the same pieces by unaligned accesses and only a row's last columns one by one: 57 us
+// where the aligned form takes 43 ([8192, 4095] and 4096; 142 with every element on its own).  A row of up to 128 or
+// 256 columns takes 16 or 32 lanes: [65536, 128] 12 us, 30 with a wavefront a row; [65536, 256] 20 and 31.
 #pragma once
 
 #include "common.h"
@@ -52,7 +54,7 @@ __device__ __forceinline__ float e4m3_scale(float largest) {
 }
 
 // GROUPED: a scale for every 128 columns (the last group may be short), otherwise one per row.
-// WIDE: rows are 16-byte aligned and a multiple of eight columns long; otherwise elements move one by one.
+// WIDE: rows are 16-byte aligned and a multiple of eight columns long.
 template <typename T, int BLOCK, int TPR, int ITERS, bool GROUPED, bool WIDE>
 __device__ __forceinline__ void add_rmsnorm_quant(const T* __restrict__ h, const T* __restrict__ r,
                                                   const T* __restrict__ w, uint8_t* __restrict__ q,
@@ -81,6 +83,10 @@ __device__ __forceinline__ void add_rmsnorm_quant(const T* __restrict__ h, const
         rv = load_vec<T, VEC, true>(r + at * r_stride + c);
         wv = load_vec<T, VEC>(w + c);
       }
+    } else if (n >= VEC) {
+      __builtin_memcpy(&hv, h + at * h_stride + c, sizeof(hv));
+      __builtin_memcpy(&rv, r + at * r_stride + c, sizeof(rv));
+      __builtin_memcpy(&wv, w + c, sizeof(wv));
     } else {
 #pragma unroll
       for (int k = 0; k < VEC; ++k)
@@ -104,6 +110,8 @@ __device__ __forceinline__ void add_rmsnorm_quant(const T* __restrict__ h, const
     }
     if (WIDE) {
       if (n > 0) store_vec<T, VEC, true>(s_out + at * cols + c, sv);
+    } else if (n >= VEC) {
+      __builtin_memcpy(s_out + at * cols + c, &sv, sizeof(sv));
     } else {
 #pragma unroll
       for (int k = 0; k < VEC; ++k)
@@ -136,8 +144,10 @@ __device__ __forceinline__ void add_rmsnorm_quant(const T* __restrict__ h, const
         v[1] = word[1];
         store_vec<uint32_t, 2, true>(reinterpret_cast<uint32_t*>(q + at * cols + c), v);
       }
+    } else if (live && c + VEC <= cols) {
+      __builtin_memcpy(q + at * cols + c, word, sizeof(word));
     } else {
-      const int n = live ? min(VEC, cols - c) : 0;
+      const int n = live ? cols - c : 0;
 #pragma unroll
       for (int k = 0; k < VEC; ++k)
         if (k < n) q[at * cols + c + k] = static_cast<uint8_t>(word[k / 4] >> (8 * (k & 3)));

@@ -377,7 +377,7 @@ def add_rmsnorm(
     return out, s
 
 
-_NORM_QUANT_VARIANTS = [(256, 64, 1), (256, 64, 2), (256, 256, 1), (512, 512, 1), (512, 512, 2), (1024, 1024, 2), (1024, 1024, 4)]
+_NORM_QUANT_VARIANTS = [(256, 16, 1), (256, 32, 1), (256, 64, 1), (256, 64, 2), (256, 256, 1), (512, 512, 1), (512, 512, 2), (1024, 1024, 2), (1024, 1024, 4)]
 
 
 @functools.lru_cache(maxsize=None)
@@ -430,7 +430,7 @@ def _norm_quant_plan(h, r, w, eps, group):
         return (), outputs, 3
     _require(rows < 2**31, "too many rows")
     hs, rs = _as_rows(h, "h").stride(0), _as_rows(r, "r").stride(0)
-    # rows of 8 elements' multiples on 16-byte addresses move in 16-byte pieces, any others element by element
+    # rows of 8 elements' multiples on 16-byte addresses, or any others
     wide = (cols | hs | rs) % 8 == 0 and all(_aligned(t) for t in (h, r, w))
     b, t, i = next(v for v in _NORM_QUANT_VARIANTS if cols <= v[1] * v[2] * 8)
     symbol = f"add_rmsnorm_quant_{_ATTN_DTYPES[h.dtype]}_b{b}_t{t}_i{i}{'_g128' if group else ''}{'' if wide else '_odd'}"

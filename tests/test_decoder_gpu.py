@@ -56,7 +56,7 @@ def check_norm(got, h, r, w, eps, group):
 
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("group", [0, 128])
-@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 7), (5, 128), (2, 129), (7, 512), (9, 1000), (4, 1024), (6, 2048), (3, 2051),
+@pytest.mark.parametrize("rows,cols", [(1, 1), (70, 88), (66, 130), (37, 255), (19, 256), (9, 257), (3, 7), (5, 128), (2, 129), (7, 512), (9, 1000), (4, 1024), (6, 2048), (3, 2051),
                                        (33, 4096), (2, 5120), (2, 8192), (2, 16384), (1, 20001), (1, 32768)])
 def test_norm_quant(K, rows, cols, group, dtype):
     announce(f"add_rmsnorm_quant rows={rows} cols={cols} group={group} {dtype}")
