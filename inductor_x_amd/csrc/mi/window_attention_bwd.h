@@ -6,9 +6,9 @@
 //               also forms the row statistics -lse / scale and -D, the values that the accumulators of Q K^T and
 //               dO V^T start from in the kernels after it, so that P = exp2(S' scale log2 e) and dS = P dP' need no
 //               subtraction there; a row that does not exist gets -1e30 and 0, which makes its P zero.
-//               D takes O with what its rounding lost, where the forward kept that, and blocks with at most two key
-//               tiles add it up from P and dP: in rows that see few keys dO V^T and D nearly cancel, and the
-//               roundings of O, and of P in the forward, would be the largest errors of dS.
+//               D takes O with what its rounding lost, where the forward kept that; blocks with at most two key tiles,
+//               and any whose rows see at most kFewKeys, add it up from P and dP: in rows that see few keys dO V^T and
+//               D nearly cancel, and the roundings of O, and of P in the forward, would be the largest errors of dS.
 //               P and dS are rounded to the operand type for the products they enter (half a step each; the
 //               products take 16 bits), everything else is fp32.
 //   dK, dV      32 keys are a pair of wavefronts, a workgroup four pairs, 128 keys of one key head; it walks the query
@@ -44,6 +44,11 @@ struct WindowBwdArgs {
 
 // Matrix steps between an LDS fragment's read and its use; one to four measured alike.
 constexpr int kAhead = 2;
+
+// Visible keys up to which a row's D is added up from P and dP in any block, at the price of two more products: with n
+// keys D from O adds about 1 / n to the two squared roundings that dQ and dK have otherwise (1.53 roundings of the
+// outputs at 4 keys, 1.45 so).
+constexpr int kFewKeys = 8;
 
 // ---- dQ, and the row statistics for the kernels after it ----
 template <typename T, int DH>
@@ -85,8 +90,8 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
   const bool exists = li < me.exist;
   const float m2 = (exists ? -a.lse[row] : -1e30f) * kWinLog2e;
   float delta = 0.f;  // -D
-  const bool few = keys.n <= 2;
-  if (!few) {
+  const bool few = keys.n <= 2, add_up = few || s.window + s.sinks <= kFewKeys;
+  if (!add_up) {
     const long long o_at = w.b * a.os.batch + me.head * a.os.head + qi * a.os.token;
     x8_t of[DS];
     auto add = [&]() {
@@ -162,9 +167,16 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
   if (keys.n == 2) request(1);
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   __syncthreads();
-  if (few) {
-    // every key of the block is at hand: D = sum of P dP itself, free of the roundings that P and O took in the forward
+  if (add_up) {
+    // D = sum of P dP itself, free of the roundings that P and O took in the forward
     for (int i = 0; i < keys.n; ++i) {
+      if (!few) {
+        if (i > 0) {
+          __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): tile i has landed, and nobody reads the buffer of the next
+          __syncthreads();
+        }
+        if (i + 1 < keys.n) request(i + 1);
+      }
       if (!me.active(keys, i)) continue;
       const WinBases at = win_bases(lane_bases, (i & 1) * 4 * TILE);
 #pragma nounroll
@@ -180,6 +192,12 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) delta = fmaf(-__builtin_amdgcn_exp2f(fmaf(sp[0][r], c2, m2)), sp[1][r], delta);
       }
+    }
+    if (!few) {  // from the first tile again
+      __syncthreads();
+      request(0);
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+      __syncthreads();
     }
   }
   delta = exists ? win_half_sum(delta) : 0.f;

@@ -56,8 +56,8 @@ def check_norm(got, h, r, w, eps, group):
 
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("group", [0, 128])
-@pytest.mark.parametrize("rows,cols", [(1, 1), (70, 88), (66, 130), (37, 255), (19, 256), (9, 257), (3, 7), (5, 128), (2, 129), (7, 512), (9, 1000), (4, 1024), (6, 2048), (3, 2051),
-                                       (33, 4096), (2, 5120), (2, 8192), (2, 16384), (1, 20001), (1, 32768)])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 7), (70, 88), (5, 128), (2, 129), (66, 130), (37, 255), (19, 256), (9, 257), (7, 512),
+                                       (9, 1000), (4, 1024), (6, 2048), (3, 2051), (33, 4096), (2, 5120), (2, 8192), (2, 16384), (1, 20001), (1, 32768)])
 def test_norm_quant(K, rows, cols, group, dtype):
     announce(f"add_rmsnorm_quant rows={rows} cols={cols} group={group} {dtype}")
     h, r, w = norm_operands(rows, cols, dtype)
@@ -283,6 +283,10 @@ WINDOW_CASES = [
     (1, 6, 3, 600, 1500, 80, 100, 33, [1400]),
     (1, 1, 1, 1200, 1200, 96, 200, 1, None),
     (1, 2, 1, 900, 900, 64, 100, 200, None),           # seven blocks of first keys
+    # rows that see a few keys in blocks of three and more tiles
+    (2, 3, 1, 300, 300, 128, 3, 1, [300, 150]),
+    (1, 1, 1, 777, 777, 64, 2, 0, None),
+    (2, 2, 2, 200, 500, 128, 5, 3, [433, 500]),
 ]
 
 
