@@ -18,6 +18,9 @@
 //               gradient's sums and one operand, each product is made once and each tile is copied once; two
 //               separate kernels (five products, two copies of each tile) took 670 us where this takes 567 us
 //               ([4,32/8,4096,128], window 1024: 850 TFLOP/s over the four products).
+//               Where there are few blocks of keys several workgroups share a walk (the host's rule); their sums go to
+//               fp32 slots and the join kernel adds those in order and rounds once: [1,8/1,2048,128] causal 104 us for
+//               the whole backward pass with 16 shares, 485 without.
 //   first keys  the keys j < sinks are also seen by every query beyond their window, hundreds of tiles for a few keys
 //               in a long text.  There that part is a kernel of its own: a workgroup takes 32 such keys and a share of
 //               those queries, each wavefront streams its own tiles of 32 queries, and the sums go to fp32 slots; the
@@ -36,9 +39,10 @@ struct WindowBwdArgs {
   void *dq, *dk, *dv;
   const float* lse;  // [B, N, Sq]
   float* stats;      // [2][B, N, Sq]: -lse / scale, -D
-  float* slots;      // [B * Nk][n_slots][2][sink_rows][DH] (dK without its scale, dV); null: no kernel for first keys
+  float* slots;      // [B * Nk][n_slots][2][slot_rows][DH] (dK without its scale, dV) of the first `joined` keys, or null
   WindowShape shape;
-  int n_slots, sink_rows;  // sink_rows: keys below `sinks`, rounded up to 32
+  int n_slots, slot_rows;  // slot_rows: `joined` rounded up to 32
+  int shares, joined;      // workgroups of a block of keys in the dK / dV kernel
   WindowStride qs, ks, vs, os, dos, dqs, dks, dvs;
 };
 
@@ -238,10 +242,11 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int pair = wave % kPairs;
   const bool for_dk = wave >= kPairs;  // the two wavefronts of a pair share a SIMD
-  const WindowBlock w = window_block(s, (s.Sk + kPairKeys - 1) / kPairKeys, 1);
+  const int blocks = (s.Sk + kPairKeys - 1) / kPairKeys;
+  const WindowBlock w = window_block(s, blocks, a.shares);
   if (!w.any) return;
   const int length = s.length(w.b), query_end = s.query_end(w.b), off = s.offset();
-  const int k0 = w.qb * kPairKeys, kw = k0 + 32 * pair;
+  const int k0 = (blocks - 1 - w.qb) * kPairKeys, kw = k0 + 32 * pair;  // the first keys, seen by the most queries, first
   const int exist = min(32, length - kw), rows = min(32, s.Sk - kw);
   f32x16_t acc[DB];
   win_zero(acc);
@@ -249,10 +254,13 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
   // query tiles that see a key of the block: through the window, or all from its first key on where the block holds
   // first keys and there is no kernel for them
   const int t_lo = max(0, k0 - off) / kWinTile;
-  const int sinks = a.slots == nullptr ? s.sinks : 0;
+  const int sinks = a.slots == nullptr || a.shares > 1 ? s.sinks : 0;
   const int q_last = min(query_end - 1, k0 < sinks ? query_end : min(k0 + kPairKeys, length) - 2 + s.window - off);
   const int nt = k0 < length && q_last >= 0 ? max(0, q_last / kWinTile - t_lo + 1) : 0;
-  const int steps = nt * s.group;
+  // this share of the walk
+  const long long walk = static_cast<long long>(nt) * s.group;
+  const int begin = static_cast<int>(walk * w.hg / a.shares), steps = static_cast<int>(walk * (w.hg + 1) / a.shares) - begin;
+  const int first_h = nt > 0 ? begin / nt : 0, first_t = t_lo + begin - first_h * nt;
   const int kj = kw + li, kc = min(kj, s.Sk - 1);
   x8_t kf[DS];  // the lane's key for P, its value for dP
   win_load_row<T>(kf, for_dk ? static_cast<const T*>(a.v) + w.b * a.vs.batch + w.kvh * a.vs.head + kc * a.vs.token
@@ -262,7 +270,7 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
   float* handed = reinterpret_cast<float*>(attn_lds + 2 * BUF + pair * kPairBytes) + 4 * lane;
 
   float sst;
-  int next_h = 0, next_t = t_lo;  // head of the group and query tile of the next request
+  int next_h = first_h, next_t = first_t;  // head of the group and query tile of the next request
   auto request = [&](int i) {
     const int head = w.kvh * s.group + next_h;
     T* dst = reinterpret_cast<T*>(attn_lds + (i & 1) * BUF);
@@ -291,7 +299,7 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
     constexpr bool FOR_DK = decltype(for_dk_c)::value;
     f32x16_t sp[2];  // S and then P, or dP, of the two blocks of 32 queries
     x8_t bf[4];      // P or dS as operands
-    int t = t_lo;
+    int t = first_t;
     for (int i = 0; i < steps; ++i) {
       if (i + 1 < steps) request(i + 1);
       const int p0 = t * kWinTile + off;  // positions p0 .. p0 + 63
@@ -387,8 +395,8 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
   else
     run(std::false_type());
   const int which = for_dk ? 0 : 1;
-  if (a.slots != nullptr && kw < a.sink_rows) {  // kw and sink_rows are multiples of 32
-    float* slot = a.slots + ((static_cast<size_t>(w.b * s.kv_heads + w.kvh) * a.n_slots) * 2 + which) * a.sink_rows * DH;
+  if (a.slots != nullptr && kw < a.slot_rows) {  // kw and slot_rows are multiples of 32
+    float* slot = a.slots + ((static_cast<size_t>(w.b * s.kv_heads + w.kvh) * a.n_slots + w.hg) * 2 + which) * a.slot_rows * DH;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -399,6 +407,7 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
         store_vec<float, 4>(slot + static_cast<size_t>(kj) * DH + 32 * db + 8 * rq + 4 * g, v);
       }
   }
+  if (a.shares > 1) return;  // every key is joined
   const WindowStride& ds = for_dk ? a.dks : a.dvs;
   T* out = static_cast<T*>(for_dk ? a.dk : a.dv) + w.b * ds.batch + w.kvh * ds.head + kw * ds.token;
   win_store<T, DH>(out, ds.token, acc, for_dk ? s.scale : 1.0f, reinterpret_cast<T*>(attn_lds) + wave * (32 * DH), lane, exist, rows, s.dim);
@@ -418,7 +427,7 @@ __device__ __forceinline__ void window_bwd_sinks(const WindowBwdArgs& a) {
   const int lane = threadIdx.x & 63, li = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // workgroups: [sequence and key head][32 keys][split]
-  const int splits = a.n_slots - 1, key_blocks = a.sink_rows / 32;
+  const int splits = a.n_slots - 1, key_blocks = a.slot_rows / 32;
   const int split = blockIdx.x % splits, rest = blockIdx.x / splits;
   const int k0 = rest % key_blocks * 32, unit = rest / key_blocks;
   const int b = unit / s.kv_heads, kvh = unit % s.kv_heads;
@@ -506,27 +515,26 @@ __device__ __forceinline__ void window_bwd_sinks(const WindowBwdArgs& a) {
       store_vec<float, 4>(all + wave * 64 * DH + 32 * DH + at, y);
     }
   __syncthreads();
-  float* slot = a.slots + (static_cast<size_t>(unit) * a.n_slots + 1 + split) * 2 * a.sink_rows * DH;
+  float* slot = a.slots + (static_cast<size_t>(unit) * a.n_slots + 1 + split) * 2 * a.slot_rows * DH;
   for (int j = threadIdx.x; j < 64 * DH; j += 64 * kSinkWaves) {
     float sum = 0.f;
 #pragma unroll
     for (int v = 0; v < kSinkWaves; ++v) sum += all[v * 64 * DH + j];
     const int which = j / (32 * DH), in = j % (32 * DH);
-    slot[static_cast<size_t>(which) * a.sink_rows * DH + static_cast<size_t>(k0) * DH + in] = sum;
+    slot[static_cast<size_t>(which) * a.slot_rows * DH + static_cast<size_t>(k0) * DH + in] = sum;
   }
 }
 
-// Adds the slots of one key row (blockIdx: sequence and key head, key) in order: a thread per column, dK then dV.
+// Adds the slots of one joined key row (blockIdx: sequence and key head, key) in order: a thread per column, dK then dV.
 template <typename T, int DH>
 __device__ __forceinline__ void window_bwd_join(const WindowBwdArgs& a) {
   const WindowShape& s = a.shape;
-  const int keys = min(s.sinks, s.Sk);
-  const int unit = blockIdx.x / keys, j = blockIdx.x % keys;
+  const int unit = blockIdx.x / a.joined, j = blockIdx.x % a.joined;
   const int b = unit / s.kv_heads, kvh = unit % s.kv_heads;
   const int which = threadIdx.x / DH, d = threadIdx.x % DH;
   float sum = 0.f;
   for (int n = 0; n < a.n_slots; ++n)
-    sum += a.slots[(((static_cast<size_t>(unit) * a.n_slots + n) * 2 + which) * a.sink_rows + j) * DH + d];
+    sum += a.slots[(((static_cast<size_t>(unit) * a.n_slots + n) * 2 + which) * a.slot_rows + j) * DH + d];
   if (d < s.dim) {
     if (which == 0)
       static_cast<T*>(a.dk)[b * a.dks.batch + kvh * a.dks.head + j * a.dks.token + d] = static_cast<T>(sum * s.scale);

@@ -1090,7 +1090,7 @@ def _window_plan(q, k, v, scale, window, sinks, lengths, keep_low):
 @functools.lru_cache(maxsize=None)
 def _window_bwd_launchers() -> dict:
     src = codecache.aot_source("window_attention_bwd_kernels.hip")
-    sig = "P" * 12 + _WINDOW_SHAPE + "ii" + "q" * 24
+    sig = "P" * 12 + _WINDOW_SHAPE + "iiii" + "q" * 24
     mk = lambda which, forms: CachingLauncher(  # noqa: E731
         f"window_attention_bwd_{which}", src, sig,
         [LaunchConfig(f"window_attention_bwd_{which}_{t}_{form}", block, lds_bytes=lds)
@@ -1101,6 +1101,19 @@ def _window_bwd_launchers() -> dict:
         "sinks": mk("sinks", [(f"d{d}", 256, 4 * 4 * 32 * d * 2) for d in (64, 128)]),
         "join": mk("join", [(f"d{d}", 2 * d, 0) for d in (64, 128)]),
     }
+
+
+def _dkv_shares(blocks: int, walk: int, growing: bool) -> int:
+    """Workgroups that share the walk of a block of keys over the heads and query tiles that see it (`walk` steps at most):
+    one for each compute unit, half as many again where the walks differ (`growing`: the causal mask alone bounds them), at
+    least four steps each, and at most 16 (the join reads a slot for each).  Measured, us of the backward pass with 1, 2, 3, 4, 6, 8, 12, 16 shares: [2,12/4,1490,64]
+    causal, 96 blocks of up to 72 steps: 135, 99, 84, 78 (4), 84, 85, 95, 103; [1,32/8,2048,128] causal, 128 of 128: 290, 204,
+    176 (3), 173, 187, 200, 227, 294; [1,8/1,8192,128] window 1024, 64 of 144: 325, 210, 170, 155 (4), 181, 170, 182, 195;
+    [1,8/1,2048,128] causal, 16 of 256: 485, 284, 213, 177, 143, 126, 112, 104 (16), with 24 shares 122;
+    [1,16/2,777,128] window 256, 14 of 48: 118, 78, 63, 56, 50, 47, 45 (12), 45; [3,8/8,777,96] window 256, 168 of 6: 38 (1), 63, 65;
+    [4,32/8,1024,128] causal, 256 of 64: 203 (1), 217, 210, 213, 258."""
+    groups = config.hardware().cu_count * (3 if growing else 2) // 2
+    return max(1, min(groups // blocks, walk // 4, 16))
 
 
 def _sink_splits(units: int, key_blocks: int, tiles: int) -> int:
@@ -1147,31 +1160,38 @@ def _window_backward_plan(q, k, v, out, dout, lse, scale, window, sinks, lengths
         return (), (_output_like(q), _output_like(k, zero=True), _output_like(v, zero=True)), 3
     units, group = B * Nk, N // Nk
     # queries at positions >= window see the first keys from beyond their window.  Where they are few, the blocks of dK and
-    # dV that hold those keys walk them too (at most 8 steps of 64 rows more than any other block takes), and where the
+    # dV that hold those keys walk them too (at most 8 steps of 64 rows more a share than in other blocks), and where the
     # first keys are a quarter of the keys or more, so that many blocks share them; else they have a kernel of their own,
     # split over the queries, and a join.  Measured, us with the kernel and without: [1,8/8,512,128] window 128 (6 steps
     # more) 51 and 43, [3,8/8,777,128] (9) 56 and 52, [1,8/8,1536,128] (20) 55 and 70; [2,32/8,384,128] (8) 71 and 66,
     # [2,32/8,448,128] (12) 73 and 75, [2,32/8,777,128] (36) 95 and 125; [2,32/8,4096,128] with 4, 512 and 1024 first keys
     # 226 and 670, 507 and 620, 808 and 683, [1,8/8,2048,128] 58 and 87, 94 and 87, 123 and 100
-    merged = group * (cdiv(Sq, 64) - cdiv(window + _WINDOW_ROWS, 64)) <= 8 or 4 * sinks >= Sk
+    blocks, all_tiles, near_tiles = cdiv(Sk, _WINDOW_ROWS), cdiv(Sq, 64), cdiv(window + _WINDOW_ROWS, 64)
+    shares = _dkv_shares(units * blocks, group * min(all_tiles, near_tiles), near_tiles >= all_tiles)
+    merged = group * (all_tiles - near_tiles) <= 8 * shares or 4 * sinks >= Sk
     far = min(sinks, Sk) if Sk > window and not merged else 0
-    _require(units * far < 2**31, "too many heads and first keys for one launch")
-    sink_rows = 32 * cdiv(far, 32)
-    n_slots = 1 + _sink_splits(units, sink_rows // 32, group * cdiv(min(Sq, Sk - window), 32)) if far else 0
+    if far:
+        shares = 1
+    joined = far or (Sk if shares > 1 else 0)
+    _require(units * max(joined, blocks * shares) < 2**31, "too many heads and keys for one launch")
+    slot_rows = 32 * cdiv(joined, 32)
+    n_slots = 1 + _sink_splits(units, slot_rows // 32, group * cdiv(min(Sq, Sk - window), 32)) if far else shares
     results = [_output_like(t) for t in (q, k, v)]
     strides = tuple(x for t in (q, k, v, out, dout, torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)) for x in _strides3(t))
     shape = _window_shape(q, k, window, sinks, scale)
     share = shape[9]
-    constants = (*shape, n_slots, sink_rows, *strides)
+    constants = (*shape, n_slots, slot_rows, shares, joined, *strides)
     ls, name = _window_bwd_launchers(), f"{_ATTN_DTYPES[q.dtype]}_d{dh}"
     bind = lambda which, grid: _bind(ls[which], f"window_attention_bwd_{which}_{name}", constants, grid)  # noqa: E731
     launches = [bind("dq", (_window_grid(units, cdiv(Sq, _WINDOW_ROWS >> share) * (group >> share)),)),
-                bind("dkv", (_window_grid(units, cdiv(Sk, _WINDOW_ROWS)),))]
+                bind("dkv", (_window_grid(units, blocks * shares),))]
     outputs = [*results, _output((2, B, N, Sq), torch.float32)]
     if far:
-        launches += [bind("sinks", (units * (sink_rows // 32) * (n_slots - 1),)), bind("join", (units * far,))]
-        outputs.append(_output((units, n_slots, 2, sink_rows, dh), torch.float32))
-    pointers = (0, 1, 2, 3, 7, 4, 8, 9, 10, 5, 11, 12 if far else -1, 6)
+        launches.append(bind("sinks", (units * (slot_rows // 32) * (n_slots - 1),)))
+    if joined:
+        launches.append(bind("join", (units * joined,)))
+        outputs.append(_output((units, n_slots, 2, slot_rows, dh), torch.float32))
+    pointers = (0, 1, 2, 3, 7, 4, 8, 9, 10, 5, 11, 12 if joined else -1, 6)
     return tuple((*launch, pointers) for launch in launches), tuple(outputs), 3
 
 

@@ -242,11 +242,13 @@ def test_first_keys_have_a_kernel_of_their_own_or_not(monkeypatch):
 
     assert kernels(1, 4, 4, 832, 832, 256, 4) == 2     # 7 tiles of queries more than a window's
     assert kernels(1, 4, 4, 897, 897, 256, 4) == 4     # 9
-    assert kernels(1, 4, 1, 897, 897, 512, 4) == 4     # 5, of four heads
+    assert kernels(4, 16, 4, 897, 897, 576, 4) == 3    # 4 of four heads, shared by two workgroups: and a join
+    assert kernels(16, 16, 4, 897, 897, 576, 4) == 4   # the same in enough sequences to need no shares
     assert kernels(1, 4, 4, 897, 897, 256, 0) == 2     # no first keys
     assert kernels(1, 4, 4, 897, 897, 256, 225) == 2   # a quarter of the keys
-    assert kernels(1, 4, 1, 256, 5000, 64, 4) == 2     # 1, of four heads
-    assert kernels(1, 4, 4, 897, 897, 897, 4) == 2     # none beyond the window
+    assert kernels(1, 4, 1, 256, 5000, 64, 4) == 3     # shared by three workgroups
+    assert kernels(1, 4, 4, 897, 897, 897, 4) == 3     # none beyond the window, shared by three workgroups
+    assert kernels(16, 4, 4, 897, 897, 897, 4) == 2
 
 
 def test_heads_of_a_workgroup():
@@ -256,6 +258,14 @@ def test_heads_of_a_workgroup():
             for tiles in (1, 15, 100, 10000):
                 n = K._sink_splits(units, blocks, tiles)
                 assert n >= 1 and (n == 1 or tiles // n >= 4)
+
+
+def test_shares_of_a_block_of_keys():
+    for blocks in (1, 7, 64, 200, 257, 5000):
+        for walk in (0, 1, 7, 40, 1000, 100000):
+            for growing in (False, True):
+                n = K._dkv_shares(blocks, walk, growing)
+                assert n == 1 or (walk // n >= 4 and n * blocks <= 384 and n <= 16)
 
 
 def test_splits_of_a_decode():
