@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import functools
 import math
+import threading
 from typing import Optional
 
 import torch
@@ -63,21 +64,30 @@ def _check_here(*tensors: torch.Tensor) -> None:
 # arguments that are no tensors is settled once per such key by the functions named _..._plan, and csrc/mi_ops.cpp answers
 # the calls.  A plan is (launches, outputs, returned): kernels with the places of their pointers among operands
 # and outputs (-1: null), what to allocate, and how many of the outputs are results (the others are workspaces).
-@functools.lru_cache(maxsize=None)
-def _operators():
-    """call(operator, *arguments), after telling the native side which function makes each operator's plans."""
-    ops = launcher.load_operators()
-    makers = {"NORM": (_norm_quant_plan, (0, 1, 2)), "ROTARY": (_rotary_plan, (0, 1, 2, 3)), "WINDOW": (_window_plan, (0, 1, 2, 6)),
-              "WINDOW_BACKWARD": (_window_backward_plan, (0, 1, 2, 3, 4, 5, 9, 10)), "DECODE": (_window_decode_plan, (0, 1, 2, 3))}
-    assert tuple(makers) == _OPERATOR_NAMES
-    numbers = [ops.operator(*entry) for entry in makers.values()]
-    assert numbers == list(range(len(makers)))
-    ops.window(_WINDOW, _WINDOW_BACKWARD)
-    return ops
-
-
-_OPERATOR_NAMES = ("NORM", "ROTARY", "WINDOW", "WINDOW_BACKWARD", "DECODE")
 _NORM, _ROTARY, _WINDOW, _WINDOW_BACKWARD, _DECODE = range(5)
+_native = None
+_native_lock = threading.Lock()
+
+
+def _operators():
+    """The native side, told which function makes each operator's plans and which of its arguments may be tensors."""
+    return _native or _load_operators()
+
+
+def _load_operators():
+    global _native
+    with _native_lock:
+        if _native is None:
+            ops = launcher.load_operators()
+            numbers = [ops.operator(maker, tensors) for maker, tensors in (
+                (_norm_quant_plan, (0, 1, 2)), (_rotary_plan, (0, 1, 2, 3)), (_window_plan, (0, 1, 2, 6)),
+                (_window_backward_plan, (0, 1, 2, 3, 4, 5, 9, 10)), (_window_decode_plan, (0, 1, 2, 3)),
+            )]
+            if numbers != [_NORM, _ROTARY, _WINDOW, _WINDOW_BACKWARD, _DECODE]:
+                raise launcher.LauncherError("the operators of csrc/mi_ops.cpp are in use by another copy of this module")
+            ops.window(_WINDOW, _WINDOW_BACKWARD)
+            _native = ops
+        return _native
 
 
 def _bind(l: CachingLauncher, symbol: str, constants, grid):
