@@ -369,6 +369,23 @@ def test_window_gradients_through_autograd():
         assert (t.grad - want[name]).abs().max() < 1e-12
 
 
+@pytest.mark.parametrize("wanted", [0, 1, 2])
+def test_window_gradient_of_one_operand(wanted):
+    announce(f"decoder.window_attention, a gradient of operand {wanted} alone")
+    from inductor_x_amd import decoder
+
+    q, k, v, dout = window_operands(2, 4, 2, 90, 90, 64, BF, False, seed=16)
+    want = R.attention(q, k, v, 0.125, 30, 2, [90, 20], dout)
+    operands = [t.to(DEV) for t in (q, k, v)]
+    operands[wanted].requires_grad_()
+    decoder.window_attention(*operands, 0.125, 30, 2, device_lengths([90, 20])).backward(dout.to(DEV))
+    for i, (t, name) in enumerate(zip(operands, ("dq", "dk", "dv"))):
+        if i == wanted:
+            within(t.grad, want[name], R.attention_bound(want[name], want[name + "_weight"], BF), name)
+        else:
+            assert t.grad is None
+
+
 def test_rotary_gradients_through_autograd():
     announce("decoder.rotary_axes through autograd")
     from inductor_x_amd import decoder
