@@ -10,18 +10,25 @@
 // Window attention with gradients is an autograd function over the same calls, so that the engine's thread runs
 // no Python between two launches: short training steps are bound by that thread.
 //
+// What rides on torch's dispatcher (a tracer, a dispatch mode, a functorch transform, a tensor subclass) would see nothing
+// of such a call but its allocations.  Where one is there the call goes to the registered op instead, which reaches
+// run() below when it is time for the kernels.
+//
 // Python's lock is held wherever plans are touched.
 #define PY_SSIZE_T_CLEAN
 #include <torch/csrc/python_headers.h>
 
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <memory>
@@ -67,7 +74,7 @@ struct KeyHash {
 };
 
 struct Operator {
-  PyObject* maker;
+  PyObject *maker, *registered;  // the latter takes a call's arguments to the dispatcher
   int operands;  // bit i: argument i may be a tensor
   std::unordered_map<std::vector<int64_t>, std::shared_ptr<const Plan>, KeyHash> plans;
 };
@@ -76,6 +83,7 @@ struct Operator {
 struct Arg {
   enum Kind : int64_t { kNone, kTensor, kInt, kFloat, kInts } kind = kNone;
   const at::Tensor* tensor = nullptr;
+  bool subclass = false;  // of torch.Tensor in Python
   int64_t i = 0;
   double d = 0;
   std::vector<int64_t> list;
@@ -125,6 +133,7 @@ void parse(PyObject* o, bool operand, Arg& a) {
     if (!operand) fail(PyExc_ValueError, "arguments that are no operands must be plain numbers, not tensors");
     a.kind = Arg::kTensor;
     a.tensor = &THPVariable_Unpack(o);
+    a.subclass = !THPVariable_CheckExact(o);
   } else if (o == Py_None) {
     a.kind = Arg::kNone;
   } else if (PyFloat_Check(o)) {
@@ -227,8 +236,35 @@ std::shared_ptr<const Plan> read_plan(PyObject* o) {
   return plan;
 }
 
+// Whether somebody has to see this call through the dispatcher.  Tensors whose numbers are not those in their memory
+// (a negative view) are made plain there too.
+bool watched(const Arg* args, int n) {
+  using c10::DispatchKey;
+  constexpr c10::DispatchKeySet rides({DispatchKey::Python, DispatchKey::FuncTorchBatched, DispatchKey::FuncTorchGradWrapper,
+                                       DispatchKey::BatchedNestedTensor, DispatchKey::Functionalize, DispatchKey::Conjugate,
+                                       DispatchKey::Negative, DispatchKey::ZeroTensor});
+  constexpr c10::DispatchKeySet here({DispatchKey::FuncTorchDynamicLayerFrontMode, DispatchKey::Functionalize, DispatchKey::PreDispatch});
+  if (c10::impl::TorchDispatchModeTLS::any_modes_set() || c10::impl::tls_local_dispatch_key_set().included_.has_any(here) ||
+      torch::jit::tracer::isTracing())
+    return true;
+  for (int i = 0; i < n; ++i)
+    if (args[i].kind == Arg::kTensor && (args[i].subclass || args[i].tensor->key_set().has_any(rides))) return true;
+  return false;
+}
+
+// The arguments as a tuple
+PyObject* given(const Arg* args, int n, PyObject* const* objects) {
+  Ref tuple(PyTuple_New(n));
+  for (int i = 0; i < n; ++i) {
+    PyObject* o = objects ? Py_NewRef(objects[i]) : to_python(args[i]);
+    if (o == nullptr) fail();
+    PyTuple_SET_ITEM(tuple.p, i, o);
+  }
+  return Py_NewRef(tuple.p);
+}
+
 // The outputs of a call (workspaces behind the returned ones); throws python_error.
-void call(int which, const Arg* args, int n, PyObject* const* objects, std::vector<at::Tensor>& outs, int& returned) {
+void run(int which, const Arg* args, int n, PyObject* const* objects, std::vector<at::Tensor>& outs, int& returned) {
   Operator& op = *operators()[which];
   std::vector<int64_t> key;
   key.reserve(128);
@@ -237,13 +273,8 @@ void call(int which, const Arg* args, int n, PyObject* const* objects, std::vect
   if (auto at = op.plans.find(key); at != op.plans.end()) {
     plan = at->second;
   } else {
-    Ref given(PyTuple_New(n));
-    for (int i = 0; i < n; ++i) {
-      PyObject* o = objects ? Py_NewRef(objects[i]) : to_python(args[i]);
-      if (o == nullptr) fail();
-      PyTuple_SET_ITEM(given.p, i, o);
-    }
-    Ref made(PyObject_Call(op.maker, given.p, nullptr));
+    Ref arguments(given(args, n, objects));
+    Ref made(PyObject_Call(op.maker, arguments.p, nullptr));
     plan = read_plan(made.p);
     const at::Tensor* tensors = nullptr;
     int count = static_cast<int>(plan->outputs.size());
@@ -304,8 +335,27 @@ void call(int which, const Arg* args, int n, PyObject* const* objects, std::vect
   }
 }
 
+// run(), or the registered op where somebody watches
+void call(int which, const Arg* args, int n, PyObject* const* objects, std::vector<at::Tensor>& outs, int& returned) {
+  if (!watched(args, n)) return run(which, args, n, objects, outs, returned);
+  Ref arguments(given(args, n, objects));
+  Ref result(PyObject_Call(operators()[which]->registered, arguments.p, nullptr));
+  if (THPVariable_Check(result.p)) {
+    outs.push_back(THPVariable_Unpack(result.p));
+  } else {
+    Ref all(PySequence_Fast(result.p, "tensors"));
+    for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(all.p); ++i) {
+      PyObject* o = PySequence_Fast_GET_ITEM(all.p, i);
+      if (!THPVariable_Check(o)) fail(PyExc_TypeError, "an operator returns tensors");
+      outs.push_back(THPVariable_Unpack(o));
+    }
+  }
+  returned = static_cast<int>(outs.size());
+}
+
 enum { kWindowForward, kWindowBackward };
 int g_window[2] = {-1, -1};
+PyObject* g_window_registered = nullptr;  // the op with its gradient
 
 class WindowAttention : public torch::autograd::Function<WindowAttention> {
  public:
@@ -315,7 +365,7 @@ class WindowAttention : public torch::autograd::Function<WindowAttention> {
     const Arg args[] = {Arg(q), Arg(k), Arg(v), Arg(scale), Arg(window), Arg(sinks), Arg(lengths), Arg(int64_t{1})};
     std::vector<at::Tensor> outs;
     int returned;
-    call(g_window[kWindowForward], args, 8, nullptr, outs, returned);
+    run(g_window[kWindowForward], args, 8, nullptr, outs, returned);  // py_window_attention looked for watchers
     ctx->save_for_backward({q, k, v, outs[0], outs[1], outs[2], lengths});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["window"] = window;
@@ -369,10 +419,11 @@ PyObject* py_bind(PyObject*, PyObject* args) {
 
 PyObject* py_operator(PyObject*, PyObject* args) {
   HANDLE_TH_ERRORS
-  PyObject *maker, *operands;
-  if (!PyArg_ParseTuple(args, "OO", &maker, &operands)) return nullptr;
+  PyObject *maker, *operands, *registered;
+  if (!PyArg_ParseTuple(args, "OOO", &maker, &operands, &registered)) return nullptr;
   auto op = std::make_unique<Operator>();
   op->maker = Py_NewRef(maker);
+  op->registered = Py_NewRef(registered);
   op->operands = 0;
   for (int64_t i : int_list(operands)) op->operands |= 1 << i;
   operators().push_back(std::move(op));
@@ -381,7 +432,9 @@ PyObject* py_operator(PyObject*, PyObject* args) {
 }
 
 PyObject* py_window(PyObject*, PyObject* args) {
-  if (!PyArg_ParseTuple(args, "ii", &g_window[kWindowForward], &g_window[kWindowBackward])) return nullptr;
+  PyObject* registered;
+  if (!PyArg_ParseTuple(args, "iiO", &g_window[kWindowForward], &g_window[kWindowBackward], &registered)) return nullptr;
+  g_window_registered = Py_NewRef(registered);
   Py_RETURN_NONE;
 }
 
@@ -390,7 +443,7 @@ PyObject* py_forget(PyObject*, PyObject*) {
   Py_RETURN_NONE;
 }
 
-PyObject* py_call(PyObject*, PyObject* const* objects, Py_ssize_t nargs) {
+PyObject* call_or_run(PyObject* const* objects, Py_ssize_t nargs, bool kernels) {
   HANDLE_TH_ERRORS
   const int64_t which = nargs > 0 ? to_int(objects[0]) : -1;
   const int n = static_cast<int>(nargs) - 1;
@@ -401,7 +454,7 @@ PyObject* py_call(PyObject*, PyObject* const* objects, Py_ssize_t nargs) {
   std::vector<at::Tensor> outs;
   outs.reserve(8);
   int returned;
-  call(static_cast<int>(which), args, n, objects + 1, outs, returned);
+  (kernels ? run : call)(static_cast<int>(which), args, n, objects + 1, outs, returned);
   if (returned == 1) return THPVariable_Wrap(outs[0]);
   Ref result(PyTuple_New(returned));
   for (int i = 0; i < returned; ++i) {
@@ -410,6 +463,19 @@ PyObject* py_call(PyObject*, PyObject* const* objects, Py_ssize_t nargs) {
     PyTuple_SET_ITEM(result.p, i, o);
   }
   return Py_NewRef(result.p);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_call(PyObject*, PyObject* const* objects, Py_ssize_t nargs) { return call_or_run(objects, nargs, false); }
+PyObject* py_run(PyObject*, PyObject* const* objects, Py_ssize_t nargs) { return call_or_run(objects, nargs, true); }
+
+// watched(operands or None ...): whether a call with them goes through the dispatcher
+PyObject* py_watched(PyObject*, PyObject* const* objects, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  Arg args[kMaxArgs];
+  if (nargs > kMaxArgs) fail(PyExc_TypeError, "watched() takes at most 12 operands");
+  for (Py_ssize_t i = 0; i < nargs; ++i) parse(objects[i], true, args[i]);
+  return PyBool_FromLong(watched(args, static_cast<int>(nargs)));
   END_HANDLE_TH_ERRORS
 }
 
@@ -425,6 +491,7 @@ PyObject* py_window_attention(PyObject*, PyObject* const* objects, Py_ssize_t na
   if (a[3].kind == Arg::kInt) a[3].d = static_cast<double>(a[3].i);
   if ((a[3].kind != Arg::kInt && a[3].kind != Arg::kFloat) || a[4].kind != Arg::kInt || a[5].kind != Arg::kInt)
     fail(PyExc_TypeError, "scale must be a number, window and sinks integers");
+  if (watched(a, 7)) return PyObject_Vectorcall(g_window_registered, objects, nargs, nullptr);
   std::optional<at::Tensor> lengths;
   if (a[6].kind == Arg::kTensor) lengths = *a[6].tensor;
   return THPVariable_Wrap(WindowAttention::apply(*a[0].tensor, *a[1].tensor, *a[2].tensor, lengths, a[3].d, a[4].i, a[5].i));
@@ -433,10 +500,14 @@ PyObject* py_window_attention(PyObject*, PyObject* const* objects, Py_ssize_t na
 
 PyMethodDef methods[] = {
     {"bind", py_bind, METH_VARARGS, "bind(address of mi_launch_packed, raise function for a failed launch, the launcher's namespace)"},
-    {"operator", py_operator, METH_VARARGS, "operator(plan maker, indices of the arguments that may be tensors) -> its number"},
-    {"window", py_window, METH_VARARGS, "window(numbers of window attention's forward and backward)"},
+    {"operator", py_operator, METH_VARARGS, "operator(plan maker, indices of the arguments that may be tensors, the registered op) -> its number"},
+    {"window", py_window, METH_VARARGS, "window(numbers of window attention's forward and backward, the registered op with its gradient)"},
     {"forget", py_forget, METH_NOARGS, "drop every plan"},
     {"call", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_call)), METH_FASTCALL, "call(operator, *arguments) -> its results"},
+    {"run", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_run)), METH_FASTCALL,
+     "run(operator, *arguments) -> its results, by the kernels whoever watches"},
+    {"watched", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_watched)), METH_FASTCALL,
+     "watched(*operands) -> whether a call with them goes to the registered op"},
     {"window_attention_with_gradients", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_window_attention)), METH_FASTCALL,
      "window_attention_with_gradients(q, k, v, scale, window, sinks, lengths) -> out"},
     {nullptr, nullptr, 0, nullptr},

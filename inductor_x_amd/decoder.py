@@ -4,7 +4,7 @@ The entry points of kernels.py (residual norm with an 8-bit result, rotary posit
 sliding window and visible first tokens) registered in the package's operator library npu_graph with shape
 functions, and wrapped with gradients: torch.compile keeps them in its graph and autograd passes through them.  The
 functions of this module are what a model calls; outside a compilation they call the kernels' entry points without
-the dispatcher.
+the dispatcher, unless a tracer, a dispatch mode, a functorch transform or a tensor subclass has to see the call there.
 """
 from __future__ import annotations
 
@@ -36,18 +36,69 @@ npu_def.define(
 )
 
 
+def _add_rmsnorm_quant(h, r, w, eps=1e-6, group=0):
+    return kernels.run(kernels._NORM, h, r, w, eps, group)
+
+
+def _rotary_axes(q, k, positions, inv_freq, sections=None, interleaved=False, inverse=False):
+    return kernels.run(kernels._ROTARY, q, k, positions, inv_freq, None if sections is None else tuple(sections), interleaved, inverse)
+
+
 def _window_attention(q, k, v, scale, window, sinks=0, lengths=None, keep_low=False):
     """kernels.window_attention with three outputs in any case: an empty `low` where it is not kept."""
-    if keep_low:
-        return kernels.window_attention(q, k, v, scale, window, sinks, lengths, True)
-    return (*kernels.window_attention(q, k, v, scale, window, sinks, lengths), q.new_empty(0))
+    outputs = kernels.run(kernels._WINDOW, q, k, v, scale, window, sinks, lengths, keep_low)
+    return outputs if keep_low else (*outputs, q.new_empty(0))
 
 
-gpu_lib.impl("add_rmsnorm_quant", kernels.add_rmsnorm_quant)
-gpu_lib.impl("rotary_axes", kernels.rotary_axes)
-gpu_lib.impl("window_attention", _window_attention)
-gpu_lib.impl("window_attention_backward", kernels.window_attention_backward)
-gpu_lib.impl("window_attention_decode", kernels.window_attention_decode)
+def _window_attention_backward(q, k, v, out, dout, lse, scale, window, sinks=0, lengths=None, low=None):
+    return kernels.run(kernels._WINDOW_BACKWARD, q, k, v, out, dout, lse, scale, window, sinks, lengths, low)
+
+
+def _window_attention_decode(q, k_cache, v_cache, lengths, scale, window, sinks=0):
+    return kernels.run(kernels._DECODE, q, k_cache, v_cache, lengths, scale, window, sinks)
+
+
+IMPLEMENTATIONS = {
+    "add_rmsnorm_quant": _add_rmsnorm_quant, "rotary_axes": _rotary_axes, "window_attention": _window_attention,
+    "window_attention_backward": _window_attention_backward, "window_attention_decode": _window_attention_decode,
+}
+for _name, _implementation in IMPLEMENTATIONS.items():
+    gpu_lib.impl(_name, _implementation)
+
+
+# The kernels' entry points as calls of the registered ops, in the order of kernels._NORM ..., without gradients as those are
+@torch.no_grad()
+def _registered_norm(h, r, w, eps, group):
+    return torch.ops.npu_graph.add_rmsnorm_quant(h, r, w, float(eps), int(group))
+
+
+@torch.no_grad()
+def _registered_rotary(q, k, positions, inv_freq, sections, interleaved, inverse):
+    return torch.ops.npu_graph.rotary_axes(q, k, positions, inv_freq, sections, bool(interleaved), bool(inverse))
+
+
+@torch.no_grad()
+def _registered_window(q, k, v, scale, window, sinks, lengths, keep_low):
+    outputs = torch.ops.npu_graph.window_attention(q, k, v, float(scale), int(window), int(sinks), lengths, bool(keep_low))
+    return outputs if keep_low else outputs[:2]
+
+
+@torch.no_grad()
+def _registered_window_backward(q, k, v, out, dout, lse, scale, window, sinks, lengths, low):
+    return torch.ops.npu_graph.window_attention_backward(q, k, v, out, dout, lse, float(scale), int(window), int(sinks), lengths, low)
+
+
+@torch.no_grad()
+def _registered_decode(q, k_cache, v_cache, lengths, scale, window, sinks):
+    return torch.ops.npu_graph.window_attention_decode(q, k_cache, v_cache, lengths, float(scale), int(window), int(sinks))
+
+
+REGISTERED = (_registered_norm, _registered_rotary, _registered_window, _registered_window_backward, _registered_decode)
+
+
+def registered_window_attention(q, k, v, scale, window, sinks, lengths):
+    """kernels.window_attention_with_gradients as a call of the registered op and its gradient."""
+    return torch.ops.npu_graph.window_attention(q, k, v, float(scale), int(window), int(sinks), lengths, True)[0]
 
 
 def _add_rmsnorm_quant_meta(h, r, w, eps=1e-6, group=0):
@@ -153,7 +204,7 @@ def add_rmsnorm_quant(h: torch.Tensor, r: torch.Tensor, w: torch.Tensor, eps: fl
 def rotary_axes(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
                 sections: Optional[Sequence[int]] = None, interleaved: bool = False, inverse: bool = False):
     """kernels.rotary_axes as a graph op with gradients for q and k."""
-    if torch.compiler.is_compiling():
+    if torch.compiler.is_compiling() or kernels.watched(q, k, positions, inv_freq):
         return torch.ops.npu_graph.rotary_axes(q, k, positions, inv_freq, sections, interleaved, inverse)
     call = RotaryFunction.apply if _needs_grad(q, k) else kernels.rotary_axes
     return call(q, k, positions, inv_freq, sections, interleaved, inverse)

@@ -78,16 +78,29 @@ def _load_operators():
     global _native
     with _native_lock:
         if _native is None:
+            from . import decoder  # the registered ops, which this module's functions go to where somebody watches
+
             ops = launcher.load_operators()
-            numbers = [ops.operator(maker, tensors) for maker, tensors in (
+            numbers = [ops.operator(maker, tensors, registered) for (maker, tensors), registered in zip((
                 (_norm_quant_plan, (0, 1, 2)), (_rotary_plan, (0, 1, 2, 3)), (_window_plan, (0, 1, 2, 6)),
                 (_window_backward_plan, (0, 1, 2, 3, 4, 5, 9, 10)), (_window_decode_plan, (0, 1, 2, 3)),
-            )]
+            ), decoder.REGISTERED)]
             if numbers != [_NORM, _ROTARY, _WINDOW, _WINDOW_BACKWARD, _DECODE]:
                 raise launcher.LauncherError("the operators of csrc/mi_ops.cpp are in use by another copy of this module")
-            ops.window(_WINDOW, _WINDOW_BACKWARD)
+            ops.window(_WINDOW, _WINDOW_BACKWARD, decoder.registered_window_attention)
             _native = ops
         return _native
+
+
+def run(operator: int, *args):
+    """What the registered op of an operator does on a GPU: its kernels, whoever watches."""
+    return _operators().run(operator, *args)
+
+
+def watched(*operands) -> bool:
+    """Whether a call with these operands has to be seen by what rides on torch's dispatcher (a tracer, a dispatch mode,
+    a functorch transform, a tensor subclass) and so goes to the registered op."""
+    return _operators().watched(*operands)
 
 
 def _bind(l: CachingLauncher, symbol: str, constants, grid):

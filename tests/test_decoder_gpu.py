@@ -749,3 +749,38 @@ def test_gradients_compile():
         results.append([out.detach(), *(t.grad for t in leaves)])
     for a, b in zip(*results):
         assert torch.equal(a, b)  # the same kernels on the same operands
+
+
+def test_recorded_calls_replay():
+    announce("graphs recorded by make_fx and torch.jit.trace, replayed on other operands")
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from inductor_x_amd import decoder, kernels as K
+
+    gen = torch.Generator().manual_seed(22)
+    B, S, N, Nk, D = 2, 60, 4, 2, 64
+    draw = lambda: [torch.randn(B, S, n, D, generator=gen).to(BF).to(DEV) for n in (N, Nk, Nk)]  # noqa: E731
+    positions = torch.arange(S, dtype=torch.int32, device=DEV).expand(B, S).contiguous()
+    inv_freq = (100.0 ** (-torch.arange(D // 2).float() / (D // 2))).to(DEV)
+    lengths = torch.tensor([60, 31], dtype=torch.int32, device=DEV)
+    w = torch.ones(D, dtype=BF, device=DEV)
+
+    def f(q, k, v):
+        q, k = decoder.rotary_axes(q, k, positions, inv_freq)
+        out = decoder.window_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), 0.125, 16, 2, lengths)
+        last = K.window_attention_decode(q[:, -1], k.transpose(1, 2), v.transpose(1, 2), lengths, 0.125, 16, 2)
+        return out, *(t.float() for t in decoder.add_rmsnorm_quant(last, last, w))
+
+    def step(q, k, v):
+        q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+        return torch.autograd.grad(f(q, k, v)[0].float().square().sum(), (q, k, v))
+
+    first, second = draw(), draw()
+    for replay in (make_fx(f)(*first), torch.jit.trace(f, tuple(first), check_trace=False)):
+        for args in (first, second):
+            for a, b in zip(replay(*args), f(*args)):
+                assert torch.equal(a, b)
+    replay = make_fx(step)(*first)
+    for args in (first, second):
+        for a, b in zip(replay(*args), step(*args)):
+            assert torch.equal(a, b)
