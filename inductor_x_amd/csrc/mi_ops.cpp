@@ -20,6 +20,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
@@ -265,6 +266,10 @@ PyObject* given(const Arg* args, int n, PyObject* const* objects) {
 
 // The outputs of a call (workspaces behind the returned ones); throws python_error.
 void run(int which, const Arg* args, int n, PyObject* const* objects, std::vector<at::Tensor>& outs, int& returned) {
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    for (int i = 0; i < n; ++i)
+      if (args[i].kind == Arg::kTensor && args[i].tensor->_fw_grad(0).defined())  // a result without its tangent would read as constant
+        fail(PyExc_NotImplementedError, "no forward-mode derivative here (decoder.rotary_axes has one outside of transforms)");
   Operator& op = *operators()[which];
   std::vector<int64_t> key;
   key.reserve(128);

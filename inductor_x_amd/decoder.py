@@ -11,7 +11,7 @@ from __future__ import annotations
 from typing import Optional, Sequence
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.library import register_autograd
 
 from . import kernels
@@ -66,30 +66,42 @@ for _name, _implementation in IMPLEMENTATIONS.items():
     gpu_lib.impl(_name, _implementation)
 
 
+def _refuse_jvp():
+    """Under a functorch jvp a registered op would give a result with a tangent of zero."""
+    layers = torch._C._functorch.get_interpreter_stack() or ()
+    if any(layer.key() == torch._C._functorch.TransformType.Jvp for layer in layers):
+        raise NotImplementedError("the decoder operators have no derivative under torch.func.jvp")
+
+
 # The kernels' entry points as calls of the registered ops, in the order of kernels._NORM ..., without gradients as those are
 @torch.no_grad()
 def _registered_norm(h, r, w, eps, group):
+    _refuse_jvp()
     return torch.ops.npu_graph.add_rmsnorm_quant(h, r, w, float(eps), int(group))
 
 
 @torch.no_grad()
 def _registered_rotary(q, k, positions, inv_freq, sections, interleaved, inverse):
+    _refuse_jvp()
     return torch.ops.npu_graph.rotary_axes(q, k, positions, inv_freq, sections, bool(interleaved), bool(inverse))
 
 
 @torch.no_grad()
 def _registered_window(q, k, v, scale, window, sinks, lengths, keep_low):
+    _refuse_jvp()
     outputs = torch.ops.npu_graph.window_attention(q, k, v, float(scale), int(window), int(sinks), lengths, bool(keep_low))
     return outputs if keep_low else outputs[:2]
 
 
 @torch.no_grad()
 def _registered_window_backward(q, k, v, out, dout, lse, scale, window, sinks, lengths, low):
+    _refuse_jvp()
     return torch.ops.npu_graph.window_attention_backward(q, k, v, out, dout, lse, float(scale), int(window), int(sinks), lengths, low)
 
 
 @torch.no_grad()
 def _registered_decode(q, k_cache, v_cache, lengths, scale, window, sinks):
+    _refuse_jvp()
     return torch.ops.npu_graph.window_attention_decode(q, k_cache, v_cache, lengths, float(scale), int(window), int(sinks))
 
 
@@ -98,6 +110,7 @@ REGISTERED = (_registered_norm, _registered_rotary, _registered_window, _registe
 
 def registered_window_attention(q, k, v, scale, window, sinks, lengths):
     """kernels.window_attention_with_gradients as a call of the registered op and its gradient."""
+    _refuse_jvp()
     return torch.ops.npu_graph.window_attention(q, k, v, float(scale), int(window), int(sinks), lengths, True)[0]
 
 
@@ -136,10 +149,15 @@ def _needs_grad(*tensors: torch.Tensor) -> bool:
     return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
 
 
+def _has_tangent(*tensors: torch.Tensor) -> bool:
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 # Gradients.  A compilation sees those of the registered ops.  Eager calls go through autograd functions over the kernels'
 # entry points: the dispatcher's way to a Python kernel and its gradient costs about 40 us of host time more, half of
 # what a short text's kernels run.  Rotary's function is here and shares its two steps (what the forward keeps, what
-# the backward calls) with the op; window attention's is csrc/mi_ops.cpp's.
+# the backward calls) with the op; window attention's is csrc/mi_ops.cpp's.  Forward-mode derivatives: rotary's function has
+# one, everything else refuses operands with a tangent (csrc/mi_ops.cpp).
 def _rotary_context(ctx, inputs, output):
     _, _, positions, inv_freq, sections, interleaved, inverse = inputs
     ctx.save_for_backward(positions, inv_freq)
@@ -187,11 +205,19 @@ class RotaryFunction(Function):
     def forward(ctx, *inputs):
         output = kernels.rotary_axes(*inputs)
         _rotary_context(ctx, inputs, output)
+        ctx.save_for_forward(*inputs[:4])
         return output
 
     @staticmethod
     def backward(ctx, dq, dk):
         return _rotary_gradient(ctx, rotary_axes, dq, dk)  # a gradient of it can be asked for in turn
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *rest):
+        q, k, positions, inv_freq = ctx.saved_tensors
+        # a linear map: tangents turn as their operands do
+        tq, tk = (torch.zeros_like(x) if t is None else t if t.stride(-1) == 1 else t.contiguous() for t, x in ((tq, q), (tk, k)))
+        return rotary_axes(tq, tk, positions, inv_freq, *ctx.form)
 
 
 def add_rmsnorm_quant(h: torch.Tensor, r: torch.Tensor, w: torch.Tensor, eps: float = 1e-6, group: int = 0):
@@ -203,10 +229,15 @@ def add_rmsnorm_quant(h: torch.Tensor, r: torch.Tensor, w: torch.Tensor, eps: fl
 
 def rotary_axes(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
                 sections: Optional[Sequence[int]] = None, interleaved: bool = False, inverse: bool = False):
-    """kernels.rotary_axes as a graph op with gradients for q and k."""
-    if torch.compiler.is_compiling() or kernels.watched(q, k, positions, inv_freq):
+    """kernels.rotary_axes as a graph op with gradients for q and k, eagerly also in forward mode."""
+    if torch.compiler.is_compiling():
         return torch.ops.npu_graph.rotary_axes(q, k, positions, inv_freq, sections, interleaved, inverse)
-    call = RotaryFunction.apply if _needs_grad(q, k) else kernels.rotary_axes
+    if kernels.watched(q, k, positions, inv_freq):
+        _refuse_jvp()
+        return torch.ops.npu_graph.rotary_axes(q, k, positions, inv_freq, sections, interleaved, inverse)
+    if _has_tangent(inv_freq):
+        raise NotImplementedError("rotary_axes has no derivative for its frequencies")
+    call = RotaryFunction.apply if _needs_grad(q, k) or _has_tangent(q, k) else kernels.rotary_axes
     return call(q, k, positions, inv_freq, sections, interleaved, inverse)
 
 

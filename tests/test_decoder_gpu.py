@@ -784,3 +784,30 @@ def test_recorded_calls_replay():
     for args in (first, second):
         for a, b in zip(replay(*args), step(*args)):
             assert torch.equal(a, b)
+
+
+def test_rotary_tangents():
+    announce("decoder.rotary_axes in forward mode: the tangent turns as the operand does")
+    from torch.autograd import forward_ad as fw
+
+    from inductor_x_amd import decoder
+
+    gen = torch.Generator().manual_seed(23)
+    q, tq = torch.randn(2, 2, 5, 3, 32, generator=gen)
+    k, tk = torch.randn(2, 2, 5, 1, 32, generator=gen)
+    positions = torch.randint(0, 50, (1, 2, 5), generator=gen)
+    inv_freq = 100.0 ** (-torch.arange(12).double() / 12)
+    place = lambda t: t.to(DEV)  # noqa: E731
+    for grad in (False, True):
+        for tangent in (place(tq), torch.ones(1, device=DEV).expand(2, 5, 3, 32)):  # of any layout
+            with fw.dual_level():
+                x = fw.make_dual(place(q).requires_grad_(grad), tangent)
+                y, z = decoder.rotary_axes(x, fw.make_dual(place(k), place(tk)), place(positions), place(inv_freq), None, True)
+                y, z = fw.unpack_dual(y), fw.unpack_dual(z)
+            for got, x in ((y.primal, q), (y.tangent, tangent.cpu()), (z.primal, k), (z.tangent, tk)):
+                check_rotary(got, x, positions, inv_freq, [12], True, False)
+    with fw.dual_level():
+        y, z = decoder.rotary_axes(fw.make_dual(place(q), place(tq)), place(k), place(positions), place(inv_freq))
+        check_rotary(fw.unpack_dual(y).tangent, tq, positions, inv_freq, [12], False, False)
+        t = fw.unpack_dual(z).tangent
+        assert t is None or not t.any()

@@ -175,3 +175,32 @@ def test_a_view_with_its_sign_in_the_metadata():
     freq = torch.complex(torch.zeros(32), torch.ones(32)).conj().imag
     assert freq.is_neg() and K.watched(freq)
     assert K.rotary_axes(*TURN[:3], torch.ones(33)[:32], [20, 12])[0].shape == TURN[0].shape
+
+
+def test_forward_mode_is_refused_or_right():
+    """A result that lost its tangent would read as a constant."""
+    from torch.autograd import forward_ad as fw
+
+    for name, (fn, args, _) in CALLS.items():
+        if name == "decoder rotary":
+            continue
+        for grad in (False, True):
+            with fw.dual_level(), pytest.raises((NotImplementedError, RuntimeError), match="forward|jvp"):
+                x = args[0].clone().requires_grad_(grad)
+                fn(fw.make_dual(x, torch.zeros_like(x)), *args[1:])
+        with pytest.raises(NotImplementedError):
+            torch.func.jvp(lambda x: fn(x, *args[1:]), (args[0],), (args[0],))
+        with pytest.raises(NotImplementedError):
+            torch.func.jvp(lambda x: torch.vmap(lambda y: fn(y, *args[1:]))(x.unsqueeze(0)), (args[0],), (args[0],))
+    q, k, positions, freq = TURN
+    with fw.dual_level():
+        y, z = decoder.rotary_axes(fw.make_dual(q, q.clone()), k, positions, freq, [20, 12])
+        assert fw.unpack_dual(y).tangent is not None
+        with pytest.raises(NotImplementedError, match="frequencies"):
+            decoder.rotary_axes(q, k, positions, fw.make_dual(freq, freq.clone()), [20, 12])
+        with torch.no_grad():
+            y, _ = decoder.rotary_axes(fw.make_dual(q, q.clone()), k, positions, freq, [20, 12])
+        assert fw.unpack_dual(y).tangent is not None
+    with pytest.raises(NotImplementedError):
+        torch.func.jvp(lambda x: decoder.rotary_axes(x, *TURN[1:], [20, 12])[0], (q,), (q,))
+    assert fw.unpack_dual(decoder.rotary_axes(*TURN, [20, 12])[0]).tangent is None
