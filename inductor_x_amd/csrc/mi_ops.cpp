@@ -358,6 +358,14 @@ void call(int which, const Arg* args, int n, PyObject* const* objects, std::vect
   returned = static_cast<int>(outs.size());
 }
 
+// An incoming gradient as the kernels take it, with contiguous columns in 16-byte aligned rows: it may arrive in any
+// layout (a sum's is one number everywhere) and at any address.
+at::Tensor placed(const at::Tensor& dout) {
+  bool fits = dout.dim() == 4 && dout.stride(3) == 1 && (reinterpret_cast<uintptr_t>(dout.const_data_ptr()) & 15) == 0;
+  for (int i = 0; fits && i < 3; ++i) fits = dout.size(i) == 1 || dout.stride(i) % 8 == 0;
+  return fits ? dout : dout.clone(at::MemoryFormat::Contiguous);
+}
+
 enum { kWindowForward, kWindowBackward };
 int g_window[2] = {-1, -1};
 PyObject* g_window_registered = nullptr;  // the op with its gradient
@@ -383,11 +391,8 @@ class WindowAttention : public torch::autograd::Function<WindowAttention> {
     at::Tensor dout = grads[0];
     torch::autograd::variable_list given(7);
     if (!dout.defined()) return given;
-    // contiguous columns in 16-byte aligned rows are what the kernels take; a gradient may arrive in any layout (a
-    // sum's is one number everywhere)
-    bool fits = dout.stride(3) == 1 && (reinterpret_cast<uintptr_t>(dout.const_data_ptr()) & 15) == 0;
-    for (int i = 0; i < 3; ++i) fits &= dout.size(i) == 1 || dout.stride(i) % 8 == 0;
-    if (!fits) dout = dout.clone(at::MemoryFormat::Contiguous);
+    const Arg seen(dout);
+    if (!watched(&seen, 1)) dout = placed(dout);  // else the op's implementation does
     const Arg args[] = {Arg(saved[0]), Arg(saved[1]), Arg(saved[2]), Arg(saved[3]), Arg(dout), Arg(saved[4]),
                         Arg(ctx->saved_data["scale"].toDouble()), Arg(ctx->saved_data["window"].toInt()),
                         Arg(ctx->saved_data["sinks"].toInt()), Arg(saved[6]), Arg(saved[5])};
@@ -474,6 +479,13 @@ PyObject* call_or_run(PyObject* const* objects, Py_ssize_t nargs, bool kernels) 
 PyObject* py_call(PyObject*, PyObject* const* objects, Py_ssize_t nargs) { return call_or_run(objects, nargs, false); }
 PyObject* py_run(PyObject*, PyObject* const* objects, Py_ssize_t nargs) { return call_or_run(objects, nargs, true); }
 
+PyObject* py_placed(PyObject*, PyObject* o) {
+  HANDLE_TH_ERRORS
+  if (!THPVariable_Check(o)) fail(PyExc_TypeError, "placed() takes a tensor");
+  return THPVariable_Wrap(placed(THPVariable_Unpack(o)));
+  END_HANDLE_TH_ERRORS
+}
+
 // watched(operands or None ...): whether a call with them goes through the dispatcher
 PyObject* py_watched(PyObject*, PyObject* const* objects, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
@@ -513,6 +525,7 @@ PyMethodDef methods[] = {
      "run(operator, *arguments) -> its results, by the kernels whoever watches"},
     {"watched", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_watched)), METH_FASTCALL,
      "watched(*operands) -> whether a call with them goes to the registered op"},
+    {"placed", py_placed, METH_O, "placed(gradient of an output) -> it, or a copy where the kernels do not take its layout or address"},
     {"window_attention_with_gradients", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_window_attention)), METH_FASTCALL,
      "window_attention_with_gradients(q, k, v, scale, window, sinks, lengths) -> out"},
     {nullptr, nullptr, 0, nullptr},

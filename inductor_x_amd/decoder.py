@@ -51,7 +51,8 @@ def _window_attention(q, k, v, scale, window, sinks=0, lengths=None, keep_low=Fa
 
 
 def _window_attention_backward(q, k, v, out, dout, lse, scale, window, sinks=0, lengths=None, low=None):
-    return kernels.run(kernels._WINDOW_BACKWARD, q, k, v, out, dout, lse, scale, window, sinks, lengths, low)
+    # the address that counts is known here and not where the gradient's call was traced
+    return kernels.run(kernels._WINDOW_BACKWARD, q, k, v, out, kernels.placed(dout), lse, scale, window, sinks, lengths, low)
 
 
 def _window_attention_decode(q, k_cache, v_cache, lengths, scale, window, sinks=0):
@@ -164,11 +165,16 @@ def _rotary_context(ctx, inputs, output):
     ctx.form = (sections, interleaved, inverse)
 
 
+def _columns(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy with contiguous columns (contiguous() returns an empty tensor as it is)."""
+    return t if t.stride(-1) == 1 else t.clone(memory_format=torch.contiguous_format)
+
+
 def _rotary_gradient(ctx, call, dq, dk):
     positions, inv_freq = ctx.saved_tensors
     sections, interleaved, inverse = ctx.form
     # a rotation's gradient is the rotation back
-    dq, dk = (t if t.stride(-1) == 1 else t.contiguous() for t in (dq, dk))
+    dq, dk = _columns(dq), _columns(dk)
     return (*call(dq, dk, positions, inv_freq, sections, interleaved, not inverse), None, None, None, None, None)
 
 
@@ -186,10 +192,6 @@ def _window_gradient(ctx, call, dout):
     if dout is None:
         return (None,) * 8
     scale, window, sinks = ctx.form
-    # contiguous columns in 16-byte aligned rows are what the kernels take; a gradient may arrive in any layout (a
-    # sum's is one number everywhere)
-    if dout.stride(3) != 1 or any(dout.stride(i) % 8 for i in range(3) if dout.shape[i] > 1) or dout.storage_offset() % 8:
-        dout = dout.contiguous()
     return (*call(q, k, v, out, dout, lse, scale, window, sinks, lengths, low), None, None, None, None, None)
 
 
@@ -216,7 +218,7 @@ class RotaryFunction(Function):
     def jvp(ctx, tq, tk, *rest):
         q, k, positions, inv_freq = ctx.saved_tensors
         # a linear map: tangents turn as their operands do
-        tq, tk = (torch.zeros_like(x) if t is None else t if t.stride(-1) == 1 else t.contiguous() for t, x in ((tq, q), (tk, k)))
+        tq, tk = (torch.zeros_like(x) if t is None else _columns(t) for t, x in ((tq, q), (tk, k)))
         return rotary_axes(tq, tk, positions, inv_freq, *ctx.form)
 
 

@@ -97,6 +97,12 @@ def run(operator: int, *args):
     return _operators().run(operator, *args)
 
 
+def placed(dout: torch.Tensor) -> torch.Tensor:
+    """The gradient of window attention's output as window_attention_backward takes it: itself, or a contiguous copy of one
+    whose columns or rows lie otherwise."""
+    return _operators().placed(dout)
+
+
 def watched(*operands) -> bool:
     """Whether a call with these operands has to be seen by what rides on torch's dispatcher (a tracer, a dispatch mode,
     a functorch transform, a tensor subclass) and so goes to the registered op."""

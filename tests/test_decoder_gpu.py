@@ -811,3 +811,22 @@ def test_rotary_tangents():
         check_rotary(fw.unpack_dual(y).tangent, tq, positions, inv_freq, [12], False, False)
         t = fw.unpack_dual(z).tangent
         assert t is None or not t.any()
+
+
+def test_gradients_arrive_anywhere():
+    announce("window attention's gradient from outputs' gradients off the 16-byte grid: eager, the op, compiled")
+    from inductor_x_amd import decoder
+
+    q, k, v, dout = window_operands(2, 4, 2, 50, 50, 64, BF, False, seed=24)
+    want = R.attention(q, k, v, 0.125, 16, 2, None, dout)
+    flat = torch.empty(dout.numel() + 1, dtype=BF, device=DEV)
+    odd = flat[1:].view(dout.shape).copy_(dout.to(DEV))
+    wide = torch.empty(2, 4, 50, 68, dtype=BF, device=DEV)[..., :64].copy_(dout.to(DEV))
+    f = lambda q, k, v: decoder.window_attention(q, k, v, 0.125, 16, 2)  # noqa: E731
+    op = lambda q, k, v: torch.ops.npu_graph.window_attention(q, k, v, 0.125, 16, 2, None, True)[0]  # noqa: E731
+    for fn in (f, op, torch.compile(f, fullgraph=True), torch.compile(f, fullgraph=True, backend="aot_eager")):
+        for arriving in (odd, wide):
+            leaves = [t.to(DEV).requires_grad_() for t in (q, k, v)]
+            fn(*leaves).backward(arriving)
+            for leaf, name in zip(leaves, ("dq", "dk", "dv")):
+                within(leaf.grad, want[name], R.attention_bound(want[name], want[name + "_weight"], BF), name)

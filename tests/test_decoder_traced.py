@@ -204,3 +204,47 @@ def test_forward_mode_is_refused_or_right():
     with pytest.raises(NotImplementedError):
         torch.func.jvp(lambda x: decoder.rotary_axes(x, *TURN[1:], [20, 12])[0], (q,), (q,))
     assert fw.unpack_dual(decoder.rotary_axes(*TURN, [20, 12])[0]).tangent is None
+
+
+def arrivals(shape):
+    """Gradients of a shape [B, N, S, D] in layouts and at addresses that the kernels do not take."""
+    n = torch.Size(shape).numel()
+    yield torch.ones(n + 1, dtype=BF)[1:].view(shape)                                              # contiguous, off the 16-byte grid
+    yield torch.ones(1, dtype=BF).expand(shape)                                                    # a sum's
+    yield torch.ones(*shape[:3], shape[3] + 4, dtype=BF)[..., : shape[3]]                          # rows off the grid
+    yield torch.ones(*shape[:2], shape[3], shape[2], dtype=BF).transpose(2, 3)                     # columns apart
+
+
+def test_gradients_arrive_anywhere(monkeypatch):
+    """The address that reaches the kernels, through the op and through the native function."""
+    ready = []
+
+    def plan(q, k, v, out, dout, lse, *rest):
+        ready.append(dout.data_ptr() % 16 == 0 and dout.stride(3) == 1 and all(s % 8 == 0 for s in dout.stride()[:3]))
+        return (), tuple((tuple(t.shape), t.contiguous().stride(), t.dtype, True) for t in (q, k, v)), 3
+
+    ops = K._operators()
+    number = ops.operator(plan, (0, 1, 2, 3, 4, 5, 9, 10), lambda *a: None)
+    monkeypatch.setattr(K, "_WINDOW_BACKWARD", number)
+    q, kv, lse = torch.zeros(2, 4, 8, 64, dtype=BF), torch.zeros(2, 2, 16, 64, dtype=BF), torch.zeros(2, 4, 8)
+    for dout in arrivals(q.shape):
+        before = dout.clone()
+        OPS.window_attention_backward(q, kv, kv, q, dout, lse, 0.1, 4)
+        assert ready.pop() and torch.equal(dout, before)
+        ops.forget()
+    empty = torch.zeros(0, 4, 8, 64, dtype=BF)
+    for dout in arrivals(q.shape):
+        again = K.placed(dout)
+        assert torch.equal(again, dout) and again.data_ptr() % 16 == 0 and again.is_contiguous()
+    aligned = torch.ones(q.shape, dtype=BF).transpose(1, 2)
+    assert K.placed(aligned).data_ptr() == aligned.data_ptr() and K.placed(empty).data_ptr() == empty.data_ptr()
+
+
+def test_sums_of_empty_batches():
+    """Their gradient has strides of zero, and contiguous() leaves an empty tensor as it is."""
+    for watched in (False, True):
+        q, k, x = (t.clone().requires_grad_() for t in (Q, KV, TURN[0]))
+        with (Seen() if watched else torch.enable_grad()):
+            decoder.window_attention(q, k, k, 0.1, 4, 1).sum().backward()
+            decoder.rotary_axes(x, *TURN[1:], [20, 12])[0].sum().backward()
+        assert q.grad.shape == q.shape and k.grad.shape == k.shape and x.grad.shape == x.shape
