@@ -90,9 +90,9 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
   win_load_row<T>(qf, static_cast<const T*>(a.q) + w.b * a.qs.batch + me.head * a.qs.head + qi * a.qs.token, s.dim, g);
   win_load_row<T>(dof, static_cast<const T*>(a.dout) + w.b * a.dos.batch + me.head * a.dos.head + qi * a.dos.token, s.dim, g);
   const float c2 = s.scale2;
-  const size_t row = (static_cast<size_t>(w.b) * s.heads + me.head) * s.Sq + me.q0 + li;
+  const size_t row = (static_cast<size_t>(w.b) * s.heads + me.head) * s.Sq + me.q0;  // the first of the 32
   const bool exists = li < me.exist;
-  const float m2 = (exists ? -a.lse[row] : -1e30f) * kWinLog2e;
+  const float m2 = (exists ? -a.lse[row + li] : -1e30f) * kWinLog2e;
   float delta = 0.f;  // -D
   const bool few = keys.n <= 2, add_up = few || s.window + s.sinks <= kFewKeys;
   if (!add_up) {
@@ -120,6 +120,10 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
     T* dst = buffers + (i & 1) * 2 * TILE;
     win_copy_keys<T, DH>(K, a.ks.token, keys, i, length, s.dim, dst, wave, lane);
     win_copy_keys<T, DH>(V, a.vs.token, keys, i, length, s.dim, dst + TILE, wave, lane);
+  };
+  auto clear = [&](int i) {
+    win_clear<T, kWinThreads>(buffers + (i & 1) * 2 * TILE, 2 * TILE, threadIdx.x);
+    __syncthreads();
   };
   const WinBases lane_bases = win_lane_bases<DH>(attn_lds, lane);
   // One tile.  Its matrix steps (per key block the d slices of S and dP, then the updates) read their LDS fragments
@@ -167,53 +171,78 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
       }
     });
   };
-  request(0);
-  if (keys.n == 2) request(1);
-  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-  __syncthreads();
-  if (add_up) {
-    // D = sum of P dP itself, free of the roundings that P and O took in the forward
-    for (int i = 0; i < keys.n; ++i) {
-      if (!few) {
-        if (i > 0) {
-          __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): tile i has landed, and nobody reads the buffer of the next
-          __syncthreads();
-        }
-        if (i + 1 < keys.n) request(i + 1);
-      }
-      if (!me.active(keys, i)) continue;
-      const WinBases at = win_bases(lane_bases, (i & 1) * 4 * TILE);
-#pragma nounroll
-      for (int kb = 0; kb < 2; ++kb) {
-        f32x16_t sp[2];
-        win_zero(sp);
-#pragma unroll
-        for (int d = 0; d < DS; ++d) {
-          sp[0] = E::mfma(win_row_frag<T, DH>(at, 0, kb, d), qf[d], sp[0]);
-          sp[1] = E::mfma(win_row_frag<T, DH>(at, 2 * TILE, kb, d), dof[d], sp[1]);
-        }
-        me.hide(keys, i * kWinTile + 32 * kb, p, g, sp[0]);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) delta = fmaf(-__builtin_amdgcn_exp2f(fmaf(sp[0][r], c2, m2)), sp[1][r], delta);
-      }
-    }
-    if (!few) {  // from the first tile again
-      __syncthreads();
-      request(0);
-      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-      __syncthreads();
-    }
-  }
-  delta = exists ? win_half_sum(delta) : 0.f;
-  if (g == 0 && li < me.rows) {
-    a.stats[row] = exists ? m2 / s.scale2 : -1e30f;
-    a.stats[static_cast<size_t>(s.batch) * s.heads * s.Sq + row] = delta;
-  }
-  for (int i = 0; i < keys.n; ++i) {
-    if (i + 1 < keys.n && !few) request(i + 1);
-    if (me.active(keys, i)) compute(i, me.whole(keys, i));
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the next tile has landed
+  for (bool guarded = false;; guarded = true) {
+    request(win_first());
+    if (keys.n == 2) request(win_first() + 1);
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
     __syncthreads();
+    if (add_up) {
+      // D = sum of P dP itself, free of the roundings that P and O took in the forward
+      for (int i = 0; i < keys.n; ++i) {
+        if (!few) {
+          if (i > 0) {
+            __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): tile i has landed, and nobody reads the buffer of the next
+            __syncthreads();
+          }
+          if (i + 1 < keys.n) request(i + 1);
+        }
+        if (guarded) clear(i);
+        if (!me.active(keys, i)) continue;
+        const WinBases at = win_bases(lane_bases, (i & 1) * 4 * TILE);
+#pragma nounroll
+        for (int kb = 0; kb < 2; ++kb) {
+          f32x16_t sp[2];
+          win_zero(sp);
+#pragma unroll
+          for (int d = 0; d < DS; ++d) {
+            sp[0] = E::mfma(win_row_frag<T, DH>(at, 0, kb, d), qf[d], sp[0]);
+            sp[1] = E::mfma(win_row_frag<T, DH>(at, 2 * TILE, kb, d), dof[d], sp[1]);
+          }
+          me.hide(keys, i * kWinTile + 32 * kb, p, g, sp[0]);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) delta = fmaf(-__builtin_amdgcn_exp2f(fmaf(sp[0][r], c2, m2)), sp[1][r], delta);
+        }
+      }
+      if (!few) {  // from the first tile again
+        __syncthreads();
+        request(win_first());
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+        __syncthreads();
+      }
+    }
+    if (add_up || !guarded) delta = exists ? win_half_sum(delta) : 0.f;
+    if (g == 0 && li < me.rows) {
+      a.stats[row + li] = exists ? m2 / s.scale2 : -1e30f;
+      a.stats[static_cast<size_t>(s.batch) * s.heads * s.Sq + row + li] = delta;
+    }
+    for (int i = 0; i < keys.n; ++i) {
+      if (guarded) clear(i);
+      if (i + 1 < keys.n && !few) request(i + 1);
+      if (me.active(keys, i)) compute(i, me.whole(keys, i));
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the next tile has landed
+      __syncthreads();
+    }
+    if (guarded) {
+      // a key that is no number in a column makes its score or dP none, and so the whole row of whoever sees it
+      for (int i = 0; i < keys.n; ++i) {
+        request(i);
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+        __syncthreads();
+        const T* K = buffers + (i & 1) * 2 * TILE;
+        uint64_t bad = win_all_lost(acc, exists) ? 0 : __ballot(win_bad_row<T, DH>(K, lane) | win_bad_row<T, DH>(K + TILE, lane));
+        bool reached = false;
+        for (; bad != 0; bad &= bad - 1) reached |= me.sees(keys, i * kWinTile + __builtin_ctzll(bad), p);
+        win_reach_all(acc, reached);
+        if (reached && g == 0 && exists) a.stats[static_cast<size_t>(s.batch) * s.heads * s.Sq + row + li] = __builtin_nanf("");
+        __syncthreads();
+      }
+      break;
+    }
+    // the words lie behind the wavefronts' pieces for the store
+    if (!win_any_lost<kWinWaves>(acc, exists, reinterpret_cast<int*>(attn_lds + 4 * TILE * sizeof(T) - 64), wave, lane)) break;
+    __syncthreads();
+    win_zero(acc);
+    if (add_up) delta = 0.f;
   }
   win_store<T, DH>(dQ, a.dqs.token, acc, s.scale, stage, lane, me.exist, me.rows, s.dim);
 }
@@ -295,12 +324,19 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   };
   // the loop of one kind of wavefront; both kinds run it over the same tiles and meet at the same places
-  auto run = [&](auto for_dk_c) {
+  auto run = [&](auto for_dk_c, bool guarded) {
     constexpr bool FOR_DK = decltype(for_dk_c)::value;
     f32x16_t sp[2];  // S and then P, or dP, of the two blocks of 32 queries
     x8_t bf[4];      // P or dS as operands
     int t = first_t;
     for (int i = 0; i < steps; ++i) {
+      if (guarded) {
+        unsigned char* buffer = attn_lds + (i & 1) * BUF;
+        win_clear<T, 128 * kPairs>(reinterpret_cast<T*>(buffer), 2 * TILE, threadIdx.x);
+        float* d = reinterpret_cast<float*>(buffer + 4 * TILE) + kWinTile;  // -D; without -lse there is no probability
+        if (threadIdx.x < kWinTile && !win_is_number(d[threadIdx.x])) d[threadIdx.x] = 0.f;
+        __syncthreads();
+      }
       if (i + 1 < steps) request(i + 1);
       const int p0 = t * kWinTile + off;  // positions p0 .. p0 + 63
       const bool active = exist > 0 && p0 + kWinTile > kw && (p0 < kw + 32 - 1 + s.window || kw < sinks);
@@ -385,15 +421,55 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
       if (++t == t_lo + nt) t = t_lo;
     }
   };
-  if (steps > 0) {
-    request(0);
-    finish(0);
+  for (bool guarded = false;; guarded = true) {
+    if (steps > 0) {
+      const int first = win_first();
+      request(first);
+      finish(first);
+    }
+    __syncthreads();
+    if (for_dk)
+      run(std::true_type(), guarded);
+    else
+      run(std::false_type(), guarded);
+    if (guarded) {
+      next_h = first_h;
+      next_t = first_t;
+      for (int i = 0, t = first_t; i < steps; ++i) {
+        request(i);
+        finish(i);
+        __syncthreads();
+        const T* Q = reinterpret_cast<const T*>(attn_lds + (i & 1) * BUF);
+        const float* d = reinterpret_cast<const float*>(attn_lds + (i & 1) * BUF + 4 * TILE) + kWinTile;
+        auto sees = [&](int row) {
+          const int q = t * kWinTile + row, behind = q + off - kj;
+          return q < query_end && behind >= 0 && (behind < s.window || kj < sinks);
+        };
+        if (!win_all_lost(acc, li < exist)) {
+          const bool bad = win_bad_row<T, DH>(Q + TILE, lane);
+          if (for_dk) {  // dS is no number wherever Q, dO or D is none
+            uint64_t left = __ballot(bad | win_bad_row<T, DH>(Q, lane) | !win_is_number(d[lane]));
+            bool reached = false;
+            for (; left != 0; left &= left - 1) reached |= sees(__builtin_ctzll(left));
+            win_reach_all(acc, reached);
+          } else if (__any(bad)) {
+            win_reach<T, DH, 4>(acc, win_bases(lane_bases, (i & 1) * BUF), 2 * TILE, g, sees);
+          }
+        }
+#pragma unroll
+        for (int db = 0; db < DB; ++db) asm volatile("" : "+v"(acc[db]));  // as in the loop above
+        __syncthreads();
+        if (++t == t_lo + nt) t = t_lo;
+      }
+      break;
+    }
+    // the words lie behind the wavefronts' pieces for the store
+    if (!win_any_lost<2 * kPairs>(acc, li < exist, reinterpret_cast<int*>(attn_lds + 2 * BUF + kPairs * kPairBytes - 64), wave, lane)) break;
+    __syncthreads();
+    win_zero(acc);
+    next_h = first_h;
+    next_t = first_t;
   }
-  __syncthreads();
-  if (for_dk)
-    run(std::true_type());
-  else
-    run(std::false_type());
   const int which = for_dk ? 0 : 1;
   if (a.slots != nullptr && kw < a.slot_rows) {  // kw and slot_rows are multiples of 32
     float* slot = a.slots + ((static_cast<size_t>(w.b * s.kv_heads + w.kvh) * a.n_slots + w.hg) * 2 + which) * a.slot_rows * DH;
@@ -456,46 +532,74 @@ __device__ __forceinline__ void window_bwd_sinks(const WindowBwdArgs& a) {
     win_copy<T, DH, kSinkTile, 1>(static_cast<const T*>(a.dout) + b * a.dos.batch + head * a.dos.head + q0 * a.dos.token, a.dos.token,
                                   query_end - static_cast<int>(q0), s.dim, mine + buf * 2 * TILE + TILE, 0, lane);
   };
-  int i = begin + wave;
-  if (i < end) request(i, 0);
-  for (int buf = 0; i < end; i += kSinkWaves, buf ^= 1) {
-    const int head = kvh * s.group + i / nt;
-    const int q0 = (t_lo + i % nt) * kSinkTile;
-    // statistics of the lane's sixteen rows, requested before the next tile's copies
-    f32x16_t sp[2];
+  for (bool guarded = false;; guarded = true) {
+    int i = begin + wave;
+    if (i < end) request(i, 0);
+    for (int buf = 0; i < end; i += kSinkWaves, buf ^= 1) {
+      const int head = kvh * s.group + i / nt;
+      const int q0 = (t_lo + i % nt) * kSinkTile;
+      // statistics of the lane's sixteen rows, requested before the next tile's copies
+      f32x16_t sp[2];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int q = min(q0 + 8 * (r >> 2) + 4 * g + (r & 3), s.Sq - 1);
+      for (int r = 0; r < 16; ++r) {
+        const int q = min(q0 + 8 * (r >> 2) + 4 * g + (r & 3), s.Sq - 1);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) sp[k][r] = a.stats[((static_cast<size_t>(k) * s.batch + b) * s.heads + head) * s.Sq + q];
-    }
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this tile has landed
-    __builtin_amdgcn_sched_barrier(0);
-    if (i + kSinkWaves < end) request(i + kSinkWaves, buf ^ 1);
-    const WinBases at = win_bases(lane_bases, (wave * 4 + buf * 2) * TILE * 2);
-#pragma unroll
-    for (int d = 0; d < DS; ++d) {
-      sp[0] = E::mfma(win_row_frag<T, DH>(at, 0, 0, d), kf[d], sp[0]);
-      sp[1] = E::mfma(win_row_frag<T, DH>(at, 2 * TILE, 0, d), vf[d], sp[1]);
-    }
-    x8_t pf[2], dsf[2];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int q = q0 + 8 * (r >> 2) + 4 * g + (r & 3);
-      float x = __builtin_amdgcn_exp2f(sp[0][r] * c2);
-      x = (q < query_end) & (q + off - kj >= s.window) & (li < keys) ? x : 0.f;
-      pf[r >> 3][r & 7] = static_cast<T>(x);
-      dsf[r >> 3][r & 7] = static_cast<T>(x * sp[1][r]);
-    }
-#pragma unroll
-    for (int q2 = 0; q2 < 2; ++q2)
-#pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        dv[db] = E::mfma(win_tr_frag<T, DH>(at, 2 * TILE, db, q2), pf[q2], dv[db]);
-        dk[db] = E::mfma(win_tr_frag<T, DH>(at, 0, db, q2), dsf[q2], dk[db]);
+        for (int k = 0; k < 2; ++k) sp[k][r] = a.stats[((static_cast<size_t>(k) * s.batch + b) * s.heads + head) * s.Sq + q];
       }
-    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the reads of this buffer are done before it is refilled
-    __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this tile has landed
+      __builtin_amdgcn_sched_barrier(0);
+      if (i + kSinkWaves < end) request(i + kSinkWaves, buf ^ 1);
+      if (guarded) {
+        win_clear<T, 64>(mine + buf * 2 * TILE, 2 * TILE, lane);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sp[1][r] = win_is_number(sp[1][r]) ? sp[1][r] : 0.f;
+      }
+      const WinBases at = win_bases(lane_bases, (wave * 4 + buf * 2) * TILE * 2);
+#pragma unroll
+      for (int d = 0; d < DS; ++d) {
+        sp[0] = E::mfma(win_row_frag<T, DH>(at, 0, 0, d), kf[d], sp[0]);
+        sp[1] = E::mfma(win_row_frag<T, DH>(at, 2 * TILE, 0, d), vf[d], sp[1]);
+      }
+      x8_t pf[2], dsf[2];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int q = q0 + 8 * (r >> 2) + 4 * g + (r & 3);
+        float x = __builtin_amdgcn_exp2f(sp[0][r] * c2);
+        x = (q < query_end) & (q + off - kj >= s.window) & (li < keys) ? x : 0.f;
+        pf[r >> 3][r & 7] = static_cast<T>(x);
+        dsf[r >> 3][r & 7] = static_cast<T>(x * sp[1][r]);
+      }
+#pragma unroll
+      for (int q2 = 0; q2 < 2; ++q2)
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          dv[db] = E::mfma(win_tr_frag<T, DH>(at, 2 * TILE, db, q2), pf[q2], dv[db]);
+          dk[db] = E::mfma(win_tr_frag<T, DH>(at, 0, db, q2), dsf[q2], dk[db]);
+        }
+      __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the reads of this buffer are done before it is refilled
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (guarded) {
+      for (i = begin + wave; i < end; i += kSinkWaves) {
+        request(i, 0);
+        const int head = kvh * s.group + i / nt, q0 = (t_lo + i % nt) * kSinkTile;
+        const float d = a.stats[((static_cast<size_t>(s.batch) + b) * s.heads + head) * s.Sq + min(q0 + li, s.Sq - 1)];
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+        __builtin_amdgcn_sched_barrier(0);
+        const bool bad_do = win_bad_row<T, DH>(mine + TILE, li), bad = win_bad_row<T, DH>(mine, li) | bad_do | !win_is_number(d);
+        auto sees = [&](int row) { return q0 + row < query_end && q0 + row + off - kj >= s.window && li < keys; };
+        bool reached = false;
+        for (uint32_t left = static_cast<uint32_t>(__ballot(bad)); left != 0; left &= left - 1) reached |= sees(__builtin_ctz(left));
+        win_reach_all(dk, reached);
+        if (__any(bad_do) && !win_all_lost(dv, li < keys)) win_reach<T, DH, 2>(dv, win_bases(lane_bases, wave * 4 * TILE * 2), 2 * TILE, g, sees);
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the reads are done before the next request
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      break;
+    }
+    if (!(win_lost(dk, li < keys) | win_lost(dv, li < keys))) break;
+    win_zero(dk);
+    win_zero(dv);
   }
   // the four wavefronts' sums meet in LDS, [wave][dK, dV][key][DH]
   __syncthreads();

@@ -1095,8 +1095,7 @@ def window_attention(
     do not exist (a right-padded batch): their keys are hidden and not read, their rows of out are zero and
     of lse -inf.  lse is the natural logarithm of the sum of exp(score * scale).  keep_low adds a third tensor, what
     rounding lost of out, which makes the gradients of rows that see few keys more exact (window_attention_backward).
-    A NaN or infinity in the key or value row of a position that exists also reaches queries up to 95 positions away
-    from those that see it: it shares a tile with keys that they see."""
+    A NaN or infinity in a row reaches the queries that see it and no others (a value's infinity as itself)."""
     return _operators().call(_WINDOW, q, k, v, scale, window, sinks, lengths, keep_low)
 
 
@@ -1157,7 +1156,8 @@ def window_attention_backward(
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Gradients (dq, dk, dv) of window_attention; out, lse and (if kept) low are the forward's, dout [B, N, Sq, D] in the
     type of q (strides as for q).  dk and dv are summed over the query heads that share a key head, in fp32 and in a fixed
-    order.  Rows that do not exist get zeros, and what dout holds there is not read into anything else."""
+    order.  Rows that do not exist get zeros, and what dout holds there is not read into anything else.  A NaN or infinity in a
+    row reaches the gradients that its visible pairs enter and no others."""
     return _operators().call(_WINDOW_BACKWARD, q, k, v, out, dout, lse, scale, window, sinks, lengths, low)
 
 

@@ -830,3 +830,94 @@ def test_gradients_arrive_anywhere():
             fn(*leaves).backward(arriving)
             for leaf, name in zip(leaves, ("dq", "dk", "dv")):
                 within(leaf.grad, want[name], R.attention_bound(want[name], want[name + "_weight"], BF), name)
+
+
+# ------------------------------------------------------------------------------------ NaN and infinities in existing rows
+def without(t, rows, columns):
+    """t with the named elements (b, head, row, column) zero."""
+    t = t.clone()
+    for (b, h, r), c in zip(rows, columns):
+        t[b, h, r, c] = 0
+    return t
+
+
+# B, N, Nk, Sq, Sk, D, window, sinks, lengths, rows of keys that hold something else than numbers
+HIDDEN_CASES = [
+    (1, 1, 1, 512, 512, 64, 64, 4, None, [65, 300]),          # a tile of first keys and window, read by four wavefronts
+    (1, 6, 2, 512, 512, 128, 64, 4, None, [65, 130, 511]),    # an odd share of the heads
+    (2, 8, 2, 700, 700, 128, 200, 2, [700, 333], [1, 320, 0]),
+    (1, 4, 2, 200, 900, 128, 100, 40, None, [10, 790, 650]),  # over a cache; one row that nobody sees
+    (1, 2, 1, 300, 300, 96, 2**31 - 1, 0, None, [150]),       # causal alone
+    (1, 3, 1, 300, 300, 128, 3, 1, None, [100, 0]),           # D added up from P and dP over many tiles
+    (2, 3, 1, 60, 60, 64, 5, 0, [60, 41], [20, 40]),          # and in one
+    (1, 2, 1, 900, 900, 64, 100, 200, None, [70, 150, 500]),  # first keys with a kernel of their own
+    (1, 8, 1, 2048, 2048, 128, 2048, 0, None, [1000]),        # a walk shared by workgroups
+]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("source", ["k", "v", "q", "dout"])
+@pytest.mark.parametrize("case", HIDDEN_CASES, ids=str)
+def test_hidden_pairs_do_not_count(K, case, source, dtype):
+    """A NaN or an infinity reaches what sees it, as the formulas say, and nothing else."""
+    announce(f"window_attention {case} with NaN and infinities in rows of {source} {dtype}")
+    B, N, Nk, Sq, Sk, D, window, sinks, lengths, bad = case
+    q, k, v, dout = window_operands(B, N, Nk, Sq, Sk, D, dtype, False, seed=25)
+    t = {"q": q, "k": k, "v": v, "dout": dout}
+    first = Sk - Sq
+    if source in ("q", "dout"):
+        bad = [max(0, r - first) for r in bad]
+    rows = [(i % B, i % t[source].shape[1], r) for i, r in enumerate(bad)]
+    columns = [[3], [D - 1], [0, 5]]
+    clean = dict(t)
+    clean[source] = without(t[source], rows, columns)
+    for i, ((b, h, r), c) in enumerate(zip(rows, columns)):
+        # an infinity in a score may mean a probability of zero, by its sign: NaN there
+        t[source][b, h, r, c] = float("inf") if i == 1 and source in ("v", "dout") else float("nan")
+    want = R.attention(*(clean[x] for x in "qkv"), D**-0.5, window, sinks, lengths, clean["dout"])
+    # what an element that is no number reaches: rows [B, N, Sq], keys [B, Nk, Sk], and where it is by columns, those
+    G = N // Nk
+    lost = {x: torch.zeros_like(want[x], dtype=torch.bool) for x in ("out", "lse", "dq", "dk", "dv")}
+    for (b, h, r), c in zip(rows, columns):
+        see = R.visible(first, Sq, Sk, window, sinks, Sk if lengths is None else lengths[b])
+        if source in "kv":
+            heads = range(h * G, h * G + G)
+            hit = see[:, r].nonzero()[:, 0]
+            for n in heads:
+                if source == "k":  # the score is lost
+                    lost["out"][b, n, hit], lost["lse"][b, n, hit] = True, True
+                else:
+                    lost["out"][b, n, hit.unsqueeze(1), torch.tensor(c)] = True
+                lost["dq"][b, n, hit] = True
+            touched = see[hit].any(0).nonzero()[:, 0]  # keys that a lost row sees
+            lost["dk"][b, h, touched] = True
+            if source == "k":
+                lost["dv"][b, h, touched] = True
+        elif see[r].any():
+            touched = see[r].nonzero()[:, 0]
+            if source == "q":
+                lost["out"][b, h, r], lost["lse"][b, h, r], lost["dv"][b, h // G, touched] = True, True, True
+            else:
+                lost["dv"][b, h // G, touched.unsqueeze(1), torch.tensor(c)] = True
+            lost["dq"][b, h, r], lost["dk"][b, h // G, touched] = True, True
+    ln = device_lengths(lengths)
+    d = {x: y.to(DEV) for x, y in t.items()}
+    out, lse, low = K.window_attention(d["q"], d["k"], d["v"], D**-0.5, window, sinks, ln, keep_low=True)
+    got = {"out": out, "lse": lse}
+    for kept in (None, low):
+        got["dq"], got["dk"], got["dv"] = K.window_attention_backward(d["q"], d["k"], d["v"], out, d["dout"], lse, D**-0.5, window, sinks, ln, kept)
+        for name, x in got.items():
+            x = x.double().cpu()
+            none = torch.isneginf(want[name])  # lse of rows that do not exist
+            fine = ~lost[name] & ~none
+            bound = lse_bound(want[name]) if name == "lse" else R.attention_bound(want[name], want["weight" if name == "out" else name + "_weight"], dtype)
+            assert torch.isfinite(x[fine]).all(), f"{name}: {(~torch.isfinite(x[fine])).sum()} elements lost that see nothing of it"
+            if fine.any():
+                over = ((x - want[name]).abs() - bound)[fine].amax()
+                assert over <= 0, f"{name}: {over:.3g} over the bound"
+            assert not torch.isfinite(x[lost[name]]).any(), f"{name}: a number where there is none"
+        if source == "v":  # an infinity keeps its sign
+            for i, ((b, h, r), c) in enumerate(zip(rows, columns)):
+                one = out[b, h * G : h * G + G][..., c].float().cpu()[lost["out"][b, h * G : h * G + G][..., c]]
+                only = sum(x[:2] == (b, h) for x in rows) == 1
+                assert not only or (torch.isposinf(one) if i == 1 else torch.isnan(one)).all()
