@@ -227,6 +227,9 @@ __device__ __forceinline__ void win_zero(f32x16_t (&acc)[DB]) {
 
 __device__ __forceinline__ bool win_is_number(float x) { return __builtin_fabsf(x) < __builtin_inff(); }
 
+// max(m, |x|) over what is a number
+__device__ __forceinline__ float win_largest(float m, float x) { return win_is_number(x) ? fmaxf(m, __builtin_fabsf(x)) : m; }
+
 // Whether any wavefront of the workgroup has something else than numbers in its sums (of the lanes `mine`).  `words`: LDS that
 // nobody else uses until the workgroup meets again.
 template <int DB>

@@ -28,6 +28,16 @@
 //               rounds once.  Where those queries are few, or the first keys many, the dK / dV kernel walks them
 //               itself (the host's rule has both sides measured).
 // No atomics: results do not depend on the order of execution.
+//
+// fp16 has five bits of exponent: P of 2^-15 (one of 32768 keys) is below its normal numbers, and so is dS = P (dP - D) where dO
+// is small, as in the mean of a loss over many tokens; and dS past 65504 is infinite.  There P enters its product times 2^14, and dS
+// times a power of two which the sums are divided by at the end:
+//   dK   per key, from bounds: |dP| <= max |dO| sum |V| and |D|, over the rows of the walk, reach 2^15 at most.  dQ's
+//        kernel leaves the two maxima of each 32 rows behind the row statistics.
+//   dQ   per row, from max |dO| alone, which becomes 2^7 to 2^8: that takes |dP - D| of up to 2^8 max |dO|, and a
+//        row with more becomes infinite, which starts the workgroup over (win_any_lost) with the bound from max |V|.
+// bf16 has the exponents of fp32 and no such factors.  Backward pass of [4,32/8,4096,128] window 1024 in fp16: 1094 us, 1061
+// without them (bf16 1022); of [3,8/8,777,96] window 256 58 and 54.
 #pragma once
 
 #include "window_attention.h"
@@ -38,7 +48,7 @@ struct WindowBwdArgs {
   const void *q, *k, *v, *o, *low, *dout;  // low may be null
   void *dq, *dk, *dv;
   const float* lse;  // [B, N, Sq]
-  float* stats;      // [2][B, N, Sq]: -lse / scale, -D
+  float* stats;      // [2][B, N, Sq]: -lse / scale, -D; for fp16 behind them [B, N, ceil(Sq / 32)][2]: largest |dO|, |D|
   float* slots;      // [B * Nk][n_slots][2][slot_rows][DH] (dK without its scale, dV) of the first `joined` keys, or null
   WindowShape shape;
   int n_slots, slot_rows;  // slot_rows: `joined` rounded up to 32
@@ -53,6 +63,20 @@ constexpr int kAhead = 2;
 // keys D from O adds about 1 / n to the two squared roundings that dQ and dK have otherwise (1.53 roundings of the
 // outputs at 4 keys, 1.45 so).
 constexpr int kFewKeys = 8;
+
+template <typename T>
+constexpr bool kWinScaled = std::is_same_v<T, f16_t>;
+constexpr int kWinPShift = 14;  // P <= 1 and a little from rounding
+
+// The power of two that brings `bound` to less than 2^top
+__device__ __forceinline__ int win_shift(float bound, int top) { return top - __builtin_amdgcn_frexp_expf(bound); }
+
+// Largest |dO| and |D| of the 32 rows of head `head` that tile t of 32 holds
+__device__ __forceinline__ float* win_maxima(const WindowBwdArgs& a, int b, int head, int t) {
+  const WindowShape& s = a.shape;
+  const size_t rows = static_cast<size_t>(s.batch) * s.heads;
+  return a.stats + 2 * (rows * s.Sq + (static_cast<size_t>(b) * s.heads + head) * ((s.Sq + 31) / 32) + t);
+}
 
 // ---- dQ, and the row statistics for the kernels after it ----
 template <typename T, int DH>
@@ -81,6 +105,7 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
       a.stats[row] = -1e30f;
       a.stats[static_cast<size_t>(s.batch) * s.heads * s.Sq + row] = 0.f;
     }
+    if (kWinScaled<T> && lane < 2 && me.rows > 0) win_maxima(a, w.b, me.head, me.q0 / 32)[lane] = 0.f;
     return;
   }
   const WindowKeys keys = window_keys(block_q0 + s.offset(), min(block_q0 + per_block, query_end) - 1 + s.offset(), s.window, s.sinks,
@@ -112,6 +137,16 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
     }
   }
   const int p = me.p_lo + li;
+  float largest = 0.f;  // |dO| of the row
+  if constexpr (kWinScaled<T>) {
+#pragma unroll
+    for (int d = 0; d < DS; ++d)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) largest = win_largest(largest, static_cast<float>(dof[d][e]));
+    largest = exists ? win_half_max(largest) : 0.f;
+  }
+  int shift = kWinScaled<T> ? win_shift(largest, 8) : 0;
+  float m2s = m2;  // with the shift
 
   const T* K = static_cast<const T*>(a.k) + w.b * a.ks.batch + w.kvh * a.ks.head;
   const T* V = static_cast<const T*>(a.v) + w.b * a.vs.batch + w.kvh * a.vs.head;
@@ -157,7 +192,7 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
           if (!whole) me.hide(keys, i * kWinTile + 32 * kb, p, g, sp[0]);
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const float e = __builtin_amdgcn_exp2f(fmaf(sp[0][r], c2, m2));
+            const float e = __builtin_amdgcn_exp2f(fmaf(sp[0][r], c2, m2s));
             dsf[2 * kb + (r >> 3)][r & 7] = static_cast<T>(e * (sp[1][r] + delta));
           }
           win_pin(dsf[2 * kb]);
@@ -215,6 +250,11 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
       a.stats[row + li] = exists ? m2 / s.scale2 : -1e30f;
       a.stats[static_cast<size_t>(s.batch) * s.heads * s.Sq + row + li] = delta;
     }
+    if constexpr (kWinScaled<T>) {
+      const float all = wave_reduce<kWave>(largest, MaxOp()), d = wave_reduce<kWave>(win_largest(0.f, delta), MaxOp());
+      if (lane < 2 && me.rows > 0) win_maxima(a, w.b, me.head, me.q0 / 32)[lane] = lane == 0 ? all : d;
+      m2s = m2 + static_cast<float>(shift);
+    }
     for (int i = 0; i < keys.n; ++i) {
       if (guarded) clear(i);
       if (i + 1 < keys.n && !few) request(i + 1);
@@ -243,8 +283,28 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
     __syncthreads();
     win_zero(acc);
     if (add_up) delta = 0.f;
+    if constexpr (kWinScaled<T>) {  // |dP| and |D| are at most DH max |dO| max |V|
+      float most = 0.f;
+      for (int i = 0; i < keys.n; ++i) {
+        request(i);
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+        __syncthreads();
+        const T* V = buffers + (i & 1) * 2 * TILE + TILE;
+#pragma nounroll
+        for (int c = threadIdx.x; c < TILE; c += kWinThreads) most = win_largest(most, static_cast<float>(V[c]));
+        __syncthreads();
+      }
+      float* words = reinterpret_cast<float*>(attn_lds);
+      most = wave_reduce<kWave>(most, MaxOp());
+      if (lane == 0) words[wave] = most;
+      __syncthreads();
+#pragma unroll
+      for (int v = 0; v < kWinWaves; ++v) most = fmaxf(most, words[v]);
+      __syncthreads();
+      shift = win_shift(2.f * DH * largest * most, 15);
+    }
   }
-  win_store<T, DH>(dQ, a.dqs.token, acc, s.scale, stage, lane, me.exist, me.rows, s.dim);
+  win_store<T, DH>(dQ, a.dqs.token, acc, __builtin_ldexpf(s.scale, -shift), stage, lane, me.exist, me.rows, s.dim);
 }
 
 // ---- dK and dV: the pairs inside the window ----
@@ -294,6 +354,26 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
   x8_t kf[DS];  // the lane's key for P, its value for dP
   win_load_row<T>(kf, for_dk ? static_cast<const T*>(a.v) + w.b * a.vs.batch + w.kvh * a.vs.head + kc * a.vs.token
                              : static_cast<const T*>(a.k) + w.b * a.ks.batch + w.kvh * a.ks.head + kc * a.ks.token, s.dim, g);
+  float factor = kWinScaled<T> ? __builtin_ldexpf(1.f, kWinPShift) : 1.f;  // of P, in one kind of wavefront
+  auto ds_factor = [&]() {  // of dS beside P's, in the other; every such wavefront for itself
+    float largest = 0.f, d = 0.f, sum = 0.f;
+    const int tiles = (s.Sq + 31) / 32;
+    for (int j = lane; j < 2 * steps; j += 64) {
+      const int at = begin + j / 2, t = 2 * (t_lo + at % nt) + j % 2;
+      if (t < tiles) {
+        const float* m = win_maxima(a, w.b, w.kvh * s.group + at / nt, t);
+        largest = fmaxf(largest, m[0]);
+        d = fmaxf(d, m[1]);
+      }
+    }
+    largest = wave_reduce<kWave>(largest, MaxOp());
+    d = wave_reduce<kWave>(d, MaxOp());
+#pragma unroll
+    for (int i = 0; i < DS; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += win_largest(0.f, static_cast<float>(kf[i][e]));
+    return __builtin_ldexpf(1.f, win_shift(fmaf(largest, win_half_sum(sum), d), 15) - kWinPShift);
+  };
   const float c2 = s.scale2;
   const WinBases lane_bases = win_lane_bases<DH>(attn_lds, lane);
   float* handed = reinterpret_cast<float*>(attn_lds + 2 * BUF + pair * kPairBytes) + 4 * lane;
@@ -382,7 +462,8 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
               Vec<float, 4> v;
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                v[e] = __builtin_amdgcn_exp2f(sp[qb][4 * rq + e] * c2);
+                const float x = sp[qb][4 * rq + e];
+                v[e] = __builtin_amdgcn_exp2f(kWinScaled<T> ? fmaf(x, c2, static_cast<float>(kWinPShift)) : x * c2);
                 bf[2 * qb + (rq >> 1)][4 * (rq & 1) + e] = static_cast<T>(v[e]);
               }
               store_vec<float, 4>(handed + 256 * (4 * qb + rq), v);
@@ -398,7 +479,10 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
             for (int rq = 0; rq < 4; ++rq) {
               const Vec<float, 4> v = load_vec<float, 4>(handed + 256 * (4 * qb + rq));
 #pragma unroll
-              for (int e = 0; e < 4; ++e) bf[2 * qb + (rq >> 1)][4 * (rq & 1) + e] = static_cast<T>(v[e] * sp[qb][4 * rq + e]);
+              for (int e = 0; e < 4; ++e) {
+                const float x = v[e] * sp[qb][4 * rq + e];
+                bf[2 * qb + (rq >> 1)][4 * (rq & 1) + e] = static_cast<T>(kWinScaled<T> ? x * factor : x);
+              }
             }
         }
         // acc += (dO or Q)^T (P or dS)
@@ -425,6 +509,7 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
     if (steps > 0) {
       const int first = win_first();
       request(first);
+      if (kWinScaled<T> && for_dk) factor = ds_factor();
       finish(first);
     }
     __syncthreads();
@@ -470,6 +555,8 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
     next_h = first_h;
     next_t = first_t;
   }
+  // the sums without their factor, a power of two
+  const float unscale = !kWinScaled<T> ? 1.f : for_dk ? __builtin_ldexpf(1.f, -kWinPShift) / factor : 1.f / factor;
   const int which = for_dk ? 0 : 1;
   if (a.slots != nullptr && kw < a.slot_rows) {  // kw and slot_rows are multiples of 32
     float* slot = a.slots + ((static_cast<size_t>(w.b * s.kv_heads + w.kvh) * a.n_slots + w.hg) * 2 + which) * a.slot_rows * DH;
@@ -479,14 +566,14 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
       for (int rq = 0; rq < 4; ++rq) {
         Vec<float, 4> v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = li < exist ? acc[db][4 * rq + e] : 0.f;
+        for (int e = 0; e < 4; ++e) v[e] = li < exist ? acc[db][4 * rq + e] * unscale : 0.f;
         store_vec<float, 4>(slot + static_cast<size_t>(kj) * DH + 32 * db + 8 * rq + 4 * g, v);
       }
   }
   if (a.shares > 1) return;  // every key is joined
   const WindowStride& ds = for_dk ? a.dks : a.dvs;
   T* out = static_cast<T*>(for_dk ? a.dk : a.dv) + w.b * ds.batch + w.kvh * ds.head + kw * ds.token;
-  win_store<T, DH>(out, ds.token, acc, for_dk ? s.scale : 1.0f, reinterpret_cast<T*>(attn_lds) + wave * (32 * DH), lane, exist, rows, s.dim);
+  win_store<T, DH>(out, ds.token, acc, for_dk ? s.scale * unscale : unscale, reinterpret_cast<T*>(attn_lds) + wave * (32 * DH), lane, exist, rows, s.dim);
 }
 
 // ---- dK and dV of the first keys from the queries beyond their window ----
@@ -520,6 +607,22 @@ __device__ __forceinline__ void window_bwd_sinks(const WindowBwdArgs& a) {
   win_load_row<T>(vf, static_cast<const T*>(a.v) + b * a.vs.batch + kvh * a.vs.head + kc * a.vs.token, s.dim, g);
   const float c2 = s.scale2;
   const WinBases lane_bases = win_lane_bases<DH>(attn_lds, lane);
+  float factor = 1.f;  // of dS beside P's
+  if constexpr (kWinScaled<T>) {
+    float largest = 0.f, d = 0.f, sum = 0.f;
+    for (int j = begin + lane; j < end; j += 64) {
+      const float* m = win_maxima(a, b, kvh * s.group + j / nt, t_lo + j % nt);
+      largest = fmaxf(largest, m[0]);
+      d = fmaxf(d, m[1]);
+    }
+    largest = wave_reduce<kWave>(largest, MaxOp());
+    d = wave_reduce<kWave>(d, MaxOp());
+#pragma unroll
+    for (int i = 0; i < DS; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += win_largest(0.f, static_cast<float>(vf[i][e]));
+    factor = __builtin_ldexpf(1.f, win_shift(fmaf(largest, win_half_sum(sum), d), 15) - kWinPShift);
+  }
   f32x16_t dk[DB], dv[DB];
   win_zero(dk);
   win_zero(dv);
@@ -564,10 +667,10 @@ __device__ __forceinline__ void window_bwd_sinks(const WindowBwdArgs& a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int q = q0 + 8 * (r >> 2) + 4 * g + (r & 3);
-        float x = __builtin_amdgcn_exp2f(sp[0][r] * c2);
+        float x = __builtin_amdgcn_exp2f(kWinScaled<T> ? fmaf(sp[0][r], c2, static_cast<float>(kWinPShift)) : sp[0][r] * c2);
         x = (q < query_end) & (q + off - kj >= s.window) & (li < keys) ? x : 0.f;
         pf[r >> 3][r & 7] = static_cast<T>(x);
-        dsf[r >> 3][r & 7] = static_cast<T>(x * sp[1][r]);
+        dsf[r >> 3][r & 7] = static_cast<T>(kWinScaled<T> ? x * sp[1][r] * factor : x * sp[1][r]);
       }
 #pragma unroll
       for (int q2 = 0; q2 < 2; ++q2)
@@ -601,6 +704,7 @@ __device__ __forceinline__ void window_bwd_sinks(const WindowBwdArgs& a) {
     win_zero(dk);
     win_zero(dv);
   }
+  const float unscale_v = kWinScaled<T> ? __builtin_ldexpf(1.f, -kWinPShift) : 1.f, unscale_k = kWinScaled<T> ? unscale_v / factor : 1.f;
   // the four wavefronts' sums meet in LDS, [wave][dK, dV][key][DH]
   __syncthreads();
   float* all = reinterpret_cast<float*>(attn_lds);
@@ -611,8 +715,8 @@ __device__ __forceinline__ void window_bwd_sinks(const WindowBwdArgs& a) {
       Vec<float, 4> x, y;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        x[e] = li < keys ? dk[db][4 * rq + e] : 0.f;
-        y[e] = li < keys ? dv[db][4 * rq + e] : 0.f;
+        x[e] = li < keys ? dk[db][4 * rq + e] * unscale_k : 0.f;
+        y[e] = li < keys ? dv[db][4 * rq + e] * unscale_v : 0.f;
       }
       const int at = li * DH + 32 * db + 8 * rq + 4 * g;
       store_vec<float, 4>(all + wave * 64 * DH + at, x);

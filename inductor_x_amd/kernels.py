@@ -1214,7 +1214,8 @@ def _window_backward_plan(q, k, v, out, dout, lse, scale, window, sinks, lengths
     bind = lambda which, grid: _bind(ls[which], f"window_attention_bwd_{which}_{name}", constants, grid)  # noqa: E731
     launches = [bind("dq", (_window_grid(units, cdiv(Sq, _WINDOW_ROWS >> share) * (group >> share)),)),
                 bind("dkv", (_window_grid(units, blocks * shares),))]
-    outputs = [*results, _output((2, B, N, Sq), torch.float32)]
+    # row statistics; in fp16 also the largest |dO| and |D| of each 32 rows
+    outputs = [*results, _output((2 * B * N * (Sq + (cdiv(Sq, 32) if q.dtype == torch.float16 else 0)),), torch.float32)]
     if far:
         launches.append(bind("sinks", (units * (slot_rows // 32) * (n_slots - 1),)))
     if joined:

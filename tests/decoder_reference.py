@@ -98,3 +98,54 @@ def attention_bound(want, weight, dtype):
     fp16 probabilities below its smallest normal number are off by up to 2^-25 of the largest, which 1e-5 covers."""
     h = half_step(dtype)
     return want.abs() * h + weight * (h + 2e-4) + 1e-5
+
+
+def fp16_gradient_bounds(q, k, v, scale, window, sinks, dout):
+    """(gradients, bounds, spreads) of fp16 operands of any size, for one sequence and scores of normal size.  The spreads are
+    standard deviations of dq and dk when every rounding is an independent error, evenly spread over half a step up and
+    down (its square mean a third of the half step's square).
+
+    Beside what attention_bound counts (each term's rounding, the scores' errors of 2e-4) fp16 has an end of its normal
+    numbers, 2^-14, where a rounding is off by up to 2^-25 absolutely:
+      of the result                2^-25
+      of P 2^14 (dV)               2^-39 a pair
+      of dS 2^s (dK), by the key   s brings B = max |dO| sum |V| + max |D| to 2^14 or more: 2^-25 B 2^-14 a pair
+      of dS 2^s (dQ), by the row   s brings max |dO| to 2^7 or more: 2^-25 max |dO| 2^-7 a pair; where that would pass 65504,
+                                   s brings 2 D max |dO| max |V| to 2^14 or more: 2^-25 of that 2^-14 a pair
+      of out and its remainder in D: P times 2^-24 sum |dO| a pair."""
+    _, N, Sq, D = q.shape
+    Nk, Sk = k.shape[1:3]
+    G = N // Nk
+    h = half_step(torch.float16)
+    q, k, v, g = (t[0].double() for t in (q, k, v, dout))
+    see = visible(Sk - Sq, Sq, Sk, window, sinks, Sk)
+    out = {x: torch.zeros_like(t) for x, t in (("dq", q), ("dk", k), ("dv", v))}
+    bound = {x: torch.zeros_like(t) for x, t in out.items()}
+    square = {x: torch.zeros_like(t) for x, t in out.items()}
+    for n in range(N):
+        j = n // G
+        s = (q[n] @ k[j].T * scale).masked_fill(~see, -math.inf)
+        # the forward's probabilities, relative to the largest, are normal numbers
+        assert (s.amax(-1, keepdim=True) - s)[see].max() < 9.7
+        p = s.softmax(-1)
+        dp = g[n] @ v[j].T
+        delta = (g[n] * (p @ v[j])).sum(-1, keepdim=True)
+        ds = p * (dp - delta)
+        size = p * (dp.abs() + delta.abs() + 2 * (g[n].abs() * (p @ v[j].abs())).sum(-1, keepdim=True))
+        most = g[n].abs().amax(-1, keepdim=True)
+        lost_d = p * 2.0**-24 * g[n].abs().sum(-1, keepdim=True)
+        over = 2.0**8 * (dp - delta).abs().amax(-1, keepdim=True) * p.amax(-1, keepdim=True) > 32768 * most
+        least_q = torch.where(over, torch.maximum(2.0**-32 * most, 2.0**-39 * 2 * D * most * v[j].abs().max()), 2.0**-32 * most)
+        b = g[j * G : j * G + G].abs().max() * v[j].abs().sum(-1) + max(
+            (g[m] * ((q[m] @ k[j].T * scale).masked_fill(~see, -math.inf).softmax(-1) @ v[j])).sum(-1).abs().max() for m in range(j * G, j * G + G))
+        out["dq"][n] = ds @ k[j] * scale
+        bound["dq"][n] = (size * (h + 2e-4) + lost_d + see * least_q) @ k[j].abs() * scale
+        out["dk"][j] += ds.T @ q[n] * scale
+        bound["dk"][j] += (size * (h + 2e-4) + lost_d + see * (2.0**-39 * b)).T @ q[n].abs() * scale
+        least_k = see * (2.0**-39 * b)
+        square["dq"][n] = ((ds * h).square() + (see * least_q).square()) @ k[j].square() * scale**2 / 3
+        square["dk"][j] += ((ds * h).square() + least_k.square()).T @ q[n].square() * scale**2 / 3
+        out["dv"][j] += p.T @ g[n]
+        bound["dv"][j] += (p * (h + 2e-4) + see * 2.0**-39).T @ g[n].abs()
+    spread = {x: (square[x] + (t.half().double() - t).square()).sqrt().unsqueeze(0) for x, t in out.items() if x != "dv"}
+    return {x: t.unsqueeze(0) for x, t in out.items()}, {x: (t + out[x].abs() * h + 2.0**-25).unsqueeze(0) for x, t in bound.items()}, spread

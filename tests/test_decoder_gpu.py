@@ -921,3 +921,42 @@ def test_hidden_pairs_do_not_count(K, case, source, dtype):
                 one = out[b, h * G : h * G + G][..., c].float().cpu()[lost["out"][b, h * G : h * G + G][..., c]]
                 only = sum(x[:2] == (b, h) for x in rows) == 1
                 assert not only or (torch.isposinf(one) if i == 1 else torch.isnan(one)).all()
+
+
+# ------------------------------------------------------------------------------------ sizes of fp16 gradients
+@pytest.mark.parametrize("size_do,size_v,scale", [
+    (1.0, 1.0, 0.1), (1e-3, 1.0, 0.1), (1e-4, 1.0, 0.1), (1.0, 1e-3, 0.1), (1e-2, 1e-2, 0.1), ("mixed", 1.0, 0.1),
+    (1000.0, 1.0, 0.1), (10.0, 1000.0, 0.1),  # |dP| past 2^8 max |dO|
+    (30.0, 1000.0, 0.01),                     # dS past 65504
+])
+@pytest.mark.parametrize("N,Nk,Sq,Sk,window,sinks", [
+    (2, 1, 2000, 2000, 2000, 0),   # probabilities of 2^-15 and less, a walk of keys shared by workgroups
+    (2, 1, 2000, 2000, 128, 4),    # first keys with a kernel of their own
+    (2, 2, 333, 900, 100, 300),    # many of them
+    (3, 1, 250, 250, 3, 1),        # D from P and dP
+])
+def test_fp16_gradients_of_any_size(K, N, Nk, Sq, Sk, window, sinks, size_do, size_v, scale):
+    announce(f"window_attention_backward fp16 {N, Nk, Sq, Sk, window, sinks} dout x {size_do} v x {size_v} scale {scale}")
+    gen = torch.Generator().manual_seed(26)
+    q, dout = (torch.randn(1, N, Sq, 64, generator=gen) for _ in range(2))
+    k, v = (torch.randn(1, Nk, Sk, 64, generator=gen) for _ in range(2))
+    if size_do == "mixed":
+        dout = dout * 10.0 ** (-4 * torch.rand(1, N, Sq, 1, generator=gen))
+    else:
+        dout = dout * size_do
+    q, k, v, dout = (t.to(HF) for t in (q, k, v * size_v, dout))
+    want, bound, spread = R.fp16_gradient_bounds(q, k, v, scale, window, sinks, dout)
+    d = [t.to(DEV) for t in (q, k, v, dout)]
+    out, lse, low = K.window_attention(*d[:3], scale, window, sinks, keep_low=True)
+    got = K.window_attention_backward(*d[:3], out, d[3], lse, scale, window, sinks, None, low)
+    for name, x in zip(("dq", "dk", "dv"), got):
+        # the gradient itself may be past the largest fp16 number (the first key of every row: 102468 in one case here)
+        fits = want[name].abs() + bound[name] < 65504
+        assert not torch.isfinite(x.cpu()[want[name].abs() - bound[name] > 65520]).any()
+        x, want[name] = (torch.where(fits, t.double(), torch.zeros_like(want[name])) for t in (x.cpu(), want[name]))
+        within(x, want[name], bound[name], name)
+        if name in spread:
+            # root mean square over all elements: the spread of dS's and the result's rounding, and as much again for P's in the
+            # forward, which D carries (over few keys as large as dS's), rounded up to twice
+            error = (x.double().cpu() - want[name]).square().mean().sqrt()
+            assert error <= 2 * spread[name].square().mean().sqrt(), f"{name}: {error / spread[name].square().mean().sqrt():.2f} spreads"
