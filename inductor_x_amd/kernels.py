@@ -118,6 +118,12 @@ def _bind(l: CachingLauncher, symbol: str, constants, grid):
     return fn.describe(l.signature, constants, grid, (cfg.block,), cfg.lds_bytes)
 
 
+def _grid(blocks: int, threads: int) -> tuple:
+    """A launch's grid of that many workgroups; the runtime counts all their threads in 32 bits."""
+    _require(blocks * threads < 2**32, "too many rows, heads or positions for one launch")
+    return (blocks,)
+
+
 def _output(shape, dtype: torch.dtype, zero: bool = False) -> tuple:
     """A contiguous output of a plan."""
     shape, strides = tuple(shape), [1]
@@ -457,13 +463,12 @@ def _norm_quant_plan(h, r, w, eps, group):
     outputs = (_output(h.shape, torch.float8_e4m3fn), _output(scales_shape, torch.float32), _output(h.shape, h.dtype))
     if rows == 0:
         return (), outputs, 3
-    _require(rows < 2**31, "too many rows")
     hs, rs = _as_rows(h, "h").stride(0), _as_rows(r, "r").stride(0)
     # rows of 8 elements' multiples on 16-byte addresses, or any others
     wide = (cols | hs | rs) % 8 == 0 and all(_aligned(t) for t in (h, r, w))
     b, t, i = next(v for v in _NORM_QUANT_VARIANTS if cols <= v[1] * v[2] * 8)
     symbol = f"add_rmsnorm_quant_{_ATTN_DTYPES[h.dtype]}_b{b}_t{t}_i{i}{'_g128' if group else ''}{'' if wide else '_odd'}"
-    return ((*_bind(_norm_quant_launcher(), symbol, (rows, cols, hs, rs, float(eps)), (cdiv(rows, b // t),)), range(6)),), outputs, 3
+    return ((*_bind(_norm_quant_launcher(), symbol, (rows, cols, hs, rs, float(eps)), _grid(cdiv(rows, b // t), b)), range(6)),), outputs, 3
 
 
 def _snap_split_plan(plan: SplitPlan, rows: int, cols: int) -> SplitPlan:
@@ -993,7 +998,7 @@ def _rotary_plan(q, k, positions, inv_freq, sections, interleaved, inverse):
         _rotary_launcher(), f"rotary_axes_{_ROTARY_DTYPES[q.dtype]}_{'beside' if interleaved else 'half'}{'' if wide else '_odd'}",
         (*strides, N, k.shape[2], positions.dtype == torch.int64, inv_freq.dtype == torch.float64, tokens, S, D, 2 * pairs,
          ends[0], ends[1], ends[2], per_block, -1.0 if inverse else 1.0),
-        (cdiv(tokens, per_block),),
+        _grid(cdiv(tokens, per_block), 256),
     )
     return ((*launch, (0, 4, 1, 5, 2, 3)),), outputs, 2
 
@@ -1055,8 +1060,8 @@ def _window_shape(q, k, window, sinks, scale):
             float(scale) * 1.4426950408889634)
 
 
-def _window_grid(units: int, blocks: int) -> int:
-    return 8 * cdiv(units * blocks, 8)
+def _window_grid(units: int, blocks: int, threads: int) -> tuple:
+    return _grid(8 * cdiv(units * blocks, 8), threads)
 
 
 def _window_check(q, k, v, scale, window, sinks, lengths):
@@ -1110,7 +1115,7 @@ def _window_plan(q, k, v, scale, window, sinks, lengths, keep_low):
     launch = _bind(
         _window_fwd_launcher(), f"window_attention_fwd_{_ATTN_DTYPES[q.dtype]}_d{dh}",
         (*shape, *_strides3(q), *_strides3(k), *_strides3(v), *_strides3(torch.empty_like(q))),
-        (_window_grid(units, cdiv(q.shape[2], _WINDOW_ROWS >> share) * (group >> share)),),
+        _window_grid(units, cdiv(q.shape[2], _WINDOW_ROWS >> share) * (group >> share), 256),
     )
     return ((*launch, (0, 1, 2, 4, 6 if keep_low else -1, 5, 3)),), outputs, len(outputs)
 
@@ -1202,7 +1207,6 @@ def _window_backward_plan(q, k, v, out, dout, lse, scale, window, sinks, lengths
     if far:
         shares = 1
     joined = far or (Sk if shares > 1 else 0)
-    _require(units * max(joined, blocks * shares) < 2**31, "too many heads and keys for one launch")
     slot_rows = 32 * cdiv(joined, 32)
     n_slots = 1 + _sink_splits(units, slot_rows // 32, group * cdiv(min(Sq, Sk - window), 32)) if far else shares
     results = [_output_like(t) for t in (q, k, v)]
@@ -1212,14 +1216,14 @@ def _window_backward_plan(q, k, v, out, dout, lse, scale, window, sinks, lengths
     constants = (*shape, n_slots, slot_rows, shares, joined, *strides)
     ls, name = _window_bwd_launchers(), f"{_ATTN_DTYPES[q.dtype]}_d{dh}"
     bind = lambda which, grid: _bind(ls[which], f"window_attention_bwd_{which}_{name}", constants, grid)  # noqa: E731
-    launches = [bind("dq", (_window_grid(units, cdiv(Sq, _WINDOW_ROWS >> share) * (group >> share)),)),
-                bind("dkv", (_window_grid(units, blocks * shares),))]
+    launches = [bind("dq", _window_grid(units, cdiv(Sq, _WINDOW_ROWS >> share) * (group >> share), 256)),
+                bind("dkv", _window_grid(units, blocks * shares, 512))]
     # row statistics; in fp16 also the largest |dO| and |D| of each 32 rows
     outputs = [*results, _output((2 * B * N * (Sq + (cdiv(Sq, 32) if q.dtype == torch.float16 else 0)),), torch.float32)]
     if far:
-        launches.append(bind("sinks", (units * (slot_rows // 32) * (n_slots - 1),)))
+        launches.append(bind("sinks", _grid(units * (slot_rows // 32) * (n_slots - 1), 256)))
     if joined:
-        launches.append(bind("join", (units * joined,)))
+        launches.append(bind("join", _grid(units * joined, 2 * dh)))
         outputs.append(_output((units, n_slots, 2, slot_rows, dh), torch.float32))
     pointers = (0, 1, 2, 3, 7, 4, 8, 9, 10, 5, 11, 12 if joined else -1, 6)
     return tuple((*launch, pointers) for launch in launches), tuple(outputs), 3
@@ -1272,18 +1276,17 @@ def _window_decode_plan(q, k_cache, v_cache, lengths, scale, window, sinks):
     units = B * Nk * cdiv(group, 16)
     tiles = cdiv(min(window, capacity), 32) + cdiv(min(sinks, max(capacity - window, 0)), 32)
     splits = _decode_splits(units, tiles)
-    _require(units * splits < 2**31, "too many heads and sequences for one launch")
     main, join = _window_decode_launchers()
     name = f"{_ATTN_DTYPES[q.dtype]}_d{dh}"
     launch = _bind(
         main, f"window_decode_{name}",
         (q.stride(0), q.stride(1), *_strides3(k_cache), *_strides3(v_cache), N * D, D, Nk, group, splits, capacity, D, window,
          sinks, float(scale) * 1.4426950408889634),
-        (units * splits,))
+        _grid(units * splits, 256))
     result = _output(q.shape, q.dtype)
     if splits == 1:
         return ((*launch, (0, 1, 2, 4, -1, 3)),), (result,), 1
-    second = _bind(join, f"window_decode_join_{name}", (N, splits, D, N * D, D), (B * N,))
+    second = _bind(join, f"window_decode_join_{name}", (N, splits, D, N * D, D), _grid(B * N, dh))
     return ((*launch, (0, 1, 2, 4, 5, 3)), (*second, (5, 4, 3))), (result, _output((B, N, splits, dh + 2), torch.float32)), 1
 
 

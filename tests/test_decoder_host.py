@@ -302,3 +302,45 @@ def test_gradient_formulas_against_differences():
         turned = R.rotary(x, at, freq, [2, 3], beside, False)
         back = R.rotary(y, at, freq, [2, 3], beside, True)
         assert abs((turned * y).sum() - (x * back).sum()) < 1e-12  # a linear map and its transpose
+
+
+def test_more_than_a_launch_takes():
+    """Refused with the other operands: the runtime counts the threads of a launch in 32 bits."""
+    def norm(rows, cols):
+        h = torch.zeros(1, cols, dtype=BF).expand(rows, cols)
+        return lambda: K.add_rmsnorm_quant(h, h, h[0])
+
+    def rotary(tokens, pairs):
+        x = torch.zeros(1, 1, 1, 2 * pairs, dtype=BF).expand(tokens, 1, 1, 2 * pairs)
+        return lambda: K.rotary_axes(x, x, torch.empty(tokens, 1, dtype=torch.int32), torch.ones(pairs))
+
+    def window(B):
+        q = torch.zeros(1, 1, 1, 8, dtype=BF).expand(B, 1, 1, 8)
+        return lambda: K.window_attention(q, q, q, 0.1, 1)
+
+    def backward(B, Sk=1):
+        q, k = (torch.zeros(1, 1, 1, 8, dtype=BF).expand(B, 1, s, 8) for s in (1, Sk))
+        return lambda: K.window_attention_backward(q, k, k, q, q, torch.empty(B, 1, 1), 0.1, 1)
+
+    def decode(B, N=1):
+        q, k = torch.zeros(1, 1, 8, dtype=BF).expand(B, N, 8), torch.zeros(1, 1, 1, 8, dtype=BF).expand(B, 1, 1, 8)
+        return lambda: K.window_attention_decode(q, k, k, torch.empty(B, dtype=torch.int32), 0.1, 1)
+
+    for fits, too_many in ((norm(2**28 - 16, 128), norm(2**28, 128)), (norm(2**24 - 1, 2000), norm(2**24, 2000)),
+                           (rotary(2**24 - 1, 128), rotary(2**24, 128)), (window(2**24 - 8), window(2**24)),
+                           (decode(2**24 - 1), decode(2**24)), (decode(2**24 - 1, 16), decode(2**24, 16))):
+        with pytest.raises(Launched):
+            fits()
+        with pytest.raises(ValueError, match="one launch"):
+            too_many()
+    with pytest.raises(ValueError, match="one launch"):
+        backward(2**24)()
+
+
+def test_each_kernel_of_a_backward_pass_fits(monkeypatch):
+    bound = []
+    monkeypatch.setattr(K, "_bind", lambda l, symbol, constants, grid: bound.append(symbol) or (0, (1,) * 6 + (0,), b"", symbol))
+    q = torch.zeros(1, 1, 1, 8, dtype=BF).expand(2**23, 1, 1, 8)
+    with pytest.raises(ValueError, match="one launch"):  # dK and dV have workgroups of 512
+        K.window_attention_backward(q, q, q, q, q, torch.empty(2**23, 1, 1), 0.1, 1)
+    assert ["dq" in x for x in bound] == [True]
