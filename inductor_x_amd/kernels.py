@@ -132,9 +132,14 @@ def _output(shape, dtype: torch.dtype, zero: bool = False) -> tuple:
     return shape, tuple(strides[::-1][: len(shape)]), dtype, zero
 
 
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """torch.empty_like(t) without its memory."""
+    return torch.empty_like(torch.empty_strided(t.shape, t.stride(), dtype=t.dtype, device="meta"))
+
+
 def _output_like(t: torch.Tensor, zero: bool = False) -> tuple:
     """An output of a plan in the layout that torch.empty_like gives."""
-    return tuple(t.shape), torch.empty_like(t).stride(), t.dtype, zero
+    return tuple(t.shape), _like(t).stride(), t.dtype, zero
 
 
 # ---------------------------------------------------------------------------
@@ -987,7 +992,7 @@ def _rotary_plan(q, k, positions, inv_freq, sections, interleaved, inverse):
     _require(tokens < 2**31 and N + k.shape[2] < 2**16, "extents must fit int32 indexing")
     vec = 16 // q.element_size()
     strides = []
-    for x in (q, torch.empty_like(q), k, torch.empty_like(k)):  # operand and result
+    for x in (q, _like(q), k, _like(k)):  # operand and result
         _require(D <= 1 or x.stride(3) == 1, "columns of a head must be contiguous")
         strides += x.stride()[:3]
     step = vec if interleaved else 2 * vec
@@ -1114,7 +1119,7 @@ def _window_plan(q, k, v, scale, window, sinks, lengths, keep_low):
     share = shape[9]
     launch = _bind(
         _window_fwd_launcher(), f"window_attention_fwd_{_ATTN_DTYPES[q.dtype]}_d{dh}",
-        (*shape, *_strides3(q), *_strides3(k), *_strides3(v), *_strides3(torch.empty_like(q))),
+        (*shape, *_strides3(q), *_strides3(k), *_strides3(v), *_strides3(_like(q))),
         _window_grid(units, cdiv(q.shape[2], _WINDOW_ROWS >> share) * (group >> share), 256),
     )
     return ((*launch, (0, 1, 2, 4, 6 if keep_low else -1, 5, 3)),), outputs, len(outputs)
@@ -1210,7 +1215,7 @@ def _window_backward_plan(q, k, v, out, dout, lse, scale, window, sinks, lengths
     slot_rows = 32 * cdiv(joined, 32)
     n_slots = 1 + _sink_splits(units, slot_rows // 32, group * cdiv(min(Sq, Sk - window), 32)) if far else shares
     results = [_output_like(t) for t in (q, k, v)]
-    strides = tuple(x for t in (q, k, v, out, dout, torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)) for x in _strides3(t))
+    strides = tuple(x for t in (q, k, v, out, dout, _like(q), _like(k), _like(v)) for x in _strides3(t))
     shape = _window_shape(q, k, window, sinks, scale)
     share = shape[9]
     constants = (*shape, n_slots, slot_rows, shares, joined, *strides)

@@ -344,3 +344,17 @@ def test_each_kernel_of_a_backward_pass_fits(monkeypatch):
     with pytest.raises(ValueError, match="one launch"):  # dK and dV have workgroups of 512
         K.window_attention_backward(q, q, q, q, q, torch.empty(2**23, 1, 1), 0.1, 1)
     assert ["dq" in x for x in bound] == [True]
+
+
+def test_plans_take_no_memory():
+    """What a plan needs to know of its results are strides: making it allocates none of them (these would be terabytes)."""
+    x = torch.zeros(1, 1, 1, 64, dtype=BF).as_strided((2**6, 2**12, 2**10, 64), (0, 0, 0, 1))
+    y = torch.zeros(1, 1, 1, 64, dtype=BF).as_strided((1, 2**10, 2**19, 64), (0, 0, 0, 1))
+    with pytest.raises(Launched):
+        K.rotary_axes(x, x, torch.empty(2**6, 2**12, dtype=torch.int32), torch.ones(32))
+    with pytest.raises(Launched):
+        K.window_attention(y, y, y, 0.1, 100)
+    for shape, strides in (((2, 3, 5, 8), (120, 40, 8, 1)), ((2, 3, 5, 8), (120, 8, 24, 1)), ((2, 3, 5, 8), (0, 8, 24, 1)), ((2, 3, 5, 8), (240, 16, 48, 2)),
+                           ((1, 3, 1, 8), (7, 8, 3, 1)), ((2, 0, 5, 8), (120, 40, 8, 1)), ((2, 3, 5, 8), (400, 16, 80, 1))):
+        t = torch.zeros(2000, dtype=BF).as_strided(shape, strides)
+        assert K._output_like(t)[1] == torch.empty_like(t).stride()
