@@ -134,7 +134,7 @@ def _output(shape, dtype: torch.dtype, zero: bool = False) -> tuple:
 
 def _like(t: torch.Tensor) -> torch.Tensor:
     """torch.empty_like(t) without its memory."""
-    return torch.empty_like(torch.empty_strided(t.shape, t.stride(), dtype=t.dtype, device="meta"))
+    return t.detach().to("meta")
 
 
 def _output_like(t: torch.Tensor, zero: bool = False) -> tuple:
