@@ -57,7 +57,7 @@ __device__ __forceinline__ void rotary_axes(const RotaryTensor& q, const RotaryT
   const int turned = pairs / PAIRS;
   const int per_head = turned + (dim - rotary) / VEC;
   const int heads = q.heads + k.heads;
-  for (int i = blockIdx.y * kRotaryThreads + threadIdx.x; i < here * heads * per_head; i += gridDim.y * kRotaryThreads) {
+  for (int i = threadIdx.x; i < here * heads * per_head; i += kRotaryThreads) {
     const int j = i % per_head;
     const int rest = i / per_head;
     const int head = rest % heads, tok = rest / heads;

@@ -997,8 +997,11 @@ def _rotary_plan(q, k, positions, inv_freq, sections, interleaved, inverse):
         strides += x.stride()[:3]
     step = vec if interleaved else 2 * vec
     wide = (2 * pairs) % step == 0 and D % vec == 0 and all(x % vec == 0 for x in strides) and _aligned(q) and _aligned(k)
-    # tokens per workgroup: 128 angles' worth, fewer where that would leave compute units idle
-    per_block = max(1, min(128 // pairs, tokens // (2 * config.hardware().cu_count)))
+    # tokens per workgroup: 128 angles' worth, fewer where that would leave compute units idle, or where the elements of
+    # their heads, which a workgroup counts in 32 bits, would be too many
+    most = (2**31 - 257) // ((N + k.shape[2]) * D)
+    _require(most > 0, "heads of a token hold too many elements for one workgroup")
+    per_block = max(1, min(128 // pairs, tokens // (2 * config.hardware().cu_count), most))
     launch = _bind(
         _rotary_launcher(), f"rotary_axes_{_ROTARY_DTYPES[q.dtype]}_{'beside' if interleaved else 'half'}{'' if wide else '_odd'}",
         (*strides, N, k.shape[2], positions.dtype == torch.int64, inv_freq.dtype == torch.float64, tokens, S, D, 2 * pairs,

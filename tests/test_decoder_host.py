@@ -358,3 +358,22 @@ def test_plans_take_no_memory():
                            ((1, 3, 1, 8), (7, 8, 3, 1)), ((2, 0, 5, 8), (120, 40, 8, 1)), ((2, 3, 5, 8), (400, 16, 80, 1))):
         t = torch.zeros(2000, dtype=BF).as_strided(shape, strides)
         assert K._output_like(t)[1] == torch.empty_like(t).stride()
+
+
+def test_elements_of_a_rotary_workgroup(monkeypatch):
+    """A workgroup counts the elements of its tokens' heads in 32 bits."""
+    def call(tokens, N, D):
+        x = torch.zeros(1, 1, 1, D, dtype=BF).expand(1, tokens, N, D)
+        q = x.as_strided((1, tokens, N, D), (0, 0, 0, 1))
+        return lambda: K.rotary_axes(q, q[:, :, :1], torch.empty(1, tokens, dtype=torch.int32), torch.ones(1))
+
+    for fits in (call(1, 2**14 - 2, 2**17), call(2**15, 128, 2**9)):
+        with pytest.raises(Launched):
+            fits()
+    with pytest.raises(ValueError, match="one workgroup"):
+        call(1, 2**14, 2**17)()
+    counted = []
+    monkeypatch.setattr(K, "_bind", lambda l, symbol, constants, grid: counted.append(constants[-2]) or (0, (1,) * 6 + (0,), b"", symbol))
+    with pytest.raises(ValueError, match="current GPU"):
+        call(2**16, 2**10, 2**15)()
+    assert counted[0] * (2**10 + 1) * 2**15 < 2**31 - 256 <= (counted[0] + 1) * (2**10 + 1) * 2**15
