@@ -149,3 +149,52 @@ def fp16_gradient_bounds(q, k, v, scale, window, sinks, dout):
         bound["dv"][j] += (p * (h + 2e-4) + see * 2.0**-39).T @ g[n].abs()
     spread = {x: (square[x] + (t.half().double() - t).square()).sqrt().unsqueeze(0) for x, t in out.items() if x != "dv"}
     return {x: t.unsqueeze(0) for x, t in out.items()}, {x: (t + out[x].abs() * h + 2.0**-25).unsqueeze(0) for x, t in bound.items()}, spread
+
+
+def wide_attention(q, k, v, scale, window, sinks, lengths, dout, dtype):
+    """(results, bounds) of attention and its gradients for scores of any size.
+
+    As attention_bound, with the errors of scores by their size: a score is off by (D + 2) 2^-24 sum |q k| scale, and where
+    the row's lse is what a sum starts from by as much of |lse|; E is twice that, for the term and for the sum it is
+    divided by.  fp16 adds the ends of its normal numbers: 2^-25 a probability of the forward, which are relative to a
+    value of at least 1, and what fp16_gradient_bounds lists."""
+    B, N, Sq, D = q.shape
+    Nk, Sk = k.shape[1:3]
+    G = N // Nk
+    h, tiny = half_step(dtype), (1.0 if dtype == torch.float16 else 0.0)
+    q, k, v, dout = (t.double() for t in (q, k, v, dout))
+    out = {x: torch.zeros_like(t, memory_format=torch.contiguous_format) for x, t in (("out", q), ("dq", q), ("dk", k), ("dv", v))}
+    out["lse"] = torch.full((B, N, Sq), -math.inf, dtype=torch.float64)
+    bound = {x: torch.zeros_like(t) for x, t in out.items()}
+    for b in range(B):
+        see = visible(Sk - Sq, Sq, Sk, window, sinks, Sk if lengths is None else lengths[b])
+        rows = see.any(-1, keepdim=True)
+        for n in range(N):
+            j = n // G
+            qq, g = q[b, n] * rows, dout[b, n] * rows
+            s = (qq @ k[b, j].T * scale).masked_fill(~see, -math.inf)
+            z = torch.logsumexp(s, -1, keepdim=True)
+            zz = torch.where(rows, z, torch.zeros_like(z))
+            p = torch.where(see, (s - zz).exp(), torch.zeros_like(s))
+            e = 2 * (D + 2) * 2.0**-24 * ((qq.abs() @ k[b, j].abs().T * scale * see).amax(-1, keepdim=True) + zz.abs())
+            o, weight = p @ v[b, j], p @ v[b, j].abs()
+            floor = tiny * 2.0**-25 * (see.double() @ v[b, j].abs())
+            out["out"][b, n], out["lse"][b, n] = o, z[:, 0]
+            bound["out"][b, n] = o.abs() * h + weight * (h + e) + floor + 2.0**-25
+            bound["lse"][b, n] = (e + 2.0**-22 * zz.abs() + 2.0**-20)[:, 0]
+            dp = g @ v[b, j].T
+            delta = (g * o).sum(-1, keepdim=True)
+            ds = p * (dp - delta)
+            size = p * (dp.abs() + delta.abs() + 2 * (g.abs() * weight).sum(-1, keepdim=True))
+            lost_d = p * (g.abs() * (floor + 2.0**-24)).sum(-1, keepdim=True)
+            most, all_v = g.abs().amax(-1, keepdim=True), v[b, j].abs()
+            least_q = tiny * 2.0**-39 * 2 * D * most * all_v.max()  # of the two the larger
+            least_k = tiny * 2.0**-39 * (dout[b].abs().max() * all_v.sum(-1) + dout[b].abs().max() * all_v.sum(-1).max())
+            err_ds = size * (h + e) + lost_d
+            out["dq"][b, n], out["dv"][b, j], out["dk"][b, j] = ds @ k[b, j] * scale, out["dv"][b, j] + p.T @ g, out["dk"][b, j] + ds.T @ qq * scale
+            bound["dq"][b, n] = (err_ds + see * torch.maximum(least_q, 2.0**-32 * tiny * most)) @ k[b, j].abs() * scale
+            bound["dk"][b, j] += (err_ds + see * least_k).T @ qq.abs() * scale
+            bound["dv"][b, j] += (p * (h + e) + see * tiny * 2.0**-39).T @ g.abs()
+    for x in ("dq", "dk", "dv"):
+        bound[x] += out[x].abs() * h + 2.0**-25
+    return out, bound

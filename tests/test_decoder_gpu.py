@@ -960,3 +960,60 @@ def test_fp16_gradients_of_any_size(K, N, Nk, Sq, Sk, window, sinks, size_do, si
             # forward, which D carries (over few keys as large as dS's), rounded up to twice
             error = (x.double().cpu() - want[name]).square().mean().sqrt()
             assert error <= 2 * spread[name].square().mean().sqrt(), f"{name}: {error / spread[name].square().mean().sqrt():.2f} spreads"
+
+
+# ------------------------------------------------------------------------------------ wide scores
+def scored(kind, B, N, Nk, Sq, Sk, D, dtype, seed=27):
+    """Operands whose scores, in units of the softmax's exponent, spread over hundreds: `rising` by 13 from a tile of 64 keys to
+    the next (a new maximum in each), `creeping` by 3 (a maximum that stays behind for two), `falling` (the first stays),
+    `wide` at random."""
+    gen = torch.Generator().manual_seed(seed)
+    q, dout = (torch.randn(B, N, Sq, D, generator=gen) for _ in range(2))
+    k, v = (torch.randn(B, Nk, Sk, D, generator=gen) for _ in range(2))
+    if kind == "wide":
+        return *(t.to(dtype) for t in (q * 6, k * 2, v, dout)), D**-0.5
+    slope = {"rising": 13.0, "creeping": 3.0, "falling": -13.0}[kind] * math.log(2) / 64
+    q[..., 0], k[..., 0] = 8.0, 0.0
+    k[..., 0] += slope * D**0.5 / 8 * (torch.arange(Sk) - Sk / 2)
+    return *(t.to(dtype) for t in (q, k, v, dout)), D**-0.5
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("kind", ["rising", "creeping", "falling", "wide"])
+@pytest.mark.parametrize("B,N,Nk,Sq,Sk,D,window,sinks,lengths", [
+    (1, 2, 2, 700, 700, 128, 2**31 - 1, 0, None),
+    (2, 6, 2, 700, 700, 64, 300, 5, [700, 333]),
+    (1, 4, 1, 130, 1000, 96, 400, 70, None),
+    (1, 2, 1, 900, 900, 64, 100, 200, None),     # first keys' gradients in a kernel of their own
+    (1, 8, 1, 1500, 1500, 64, 1500, 0, None),    # a walk of keys shared by workgroups
+    (1, 3, 1, 300, 300, 128, 4, 2, None),        # D from P and dP
+])
+def test_window_attention_of_wide_scores(K, B, N, Nk, Sq, Sk, D, window, sinks, lengths, kind, dtype):
+    announce(f"window_attention {B, N, Nk, Sq, Sk, D, window, sinks, lengths} {kind} scores {dtype}")
+    q, k, v, dout, scale = scored(kind, B, N, Nk, Sq, Sk, D, dtype)
+    want, bound = R.wide_attention(q, k, v, scale, window, sinks, lengths, dout, dtype)
+    d = [t.to(DEV) for t in (q, k, v, dout)]
+    ln = device_lengths(lengths)
+    out, lse, low = K.window_attention(*d[:3], scale, window, sinks, ln, True)
+    within(out, want["out"], bound["out"], "out")
+    live = ~torch.isinf(want["lse"])
+    within(lse.cpu()[live], want["lse"][live], bound["lse"][live], "lse")
+    for kept in (None, low):
+        got = K.window_attention_backward(*d[:3], out, d[3], lse, scale, window, sinks, ln, kept)
+        for name, x in zip(("dq", "dk", "dv"), got):
+            within(x, want[name], bound[name], name)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("kind", ["rising", "creeping", "falling", "wide"])
+@pytest.mark.parametrize("B,N,Nk,capacity,D,window,sinks,lengths", [
+    (2, 8, 2, 700, 128, 700, 0, [700, 333]),
+    (1, 40, 2, 5000, 64, 4096, 70, [4999]),   # many shares
+])
+def test_decode_of_wide_scores(K, B, N, Nk, capacity, D, window, sinks, lengths, kind, dtype):
+    announce(f"window_attention_decode {B, N, Nk, capacity, D, window, sinks, lengths} {kind} scores {dtype}")
+    q, k, v, dout, scale = scored(kind, B, N, Nk, 1, capacity, D, dtype, seed=28)
+    got = K.window_attention_decode(q.to(DEV)[:, :, 0], k.to(DEV), v.to(DEV), device_lengths(lengths), scale, window, sinks)
+    for b, n in enumerate(lengths):
+        want, bound = R.wide_attention(*(t[b : b + 1] for t in (q, k[:, :, :n], v[:, :, :n])), scale, window, sinks, None, dout[b : b + 1], dtype)
+        within(got[b : b + 1], want["out"][:, :, 0], bound["out"][:, :, 0], "decode")
