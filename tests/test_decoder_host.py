@@ -377,3 +377,26 @@ def test_elements_of_a_rotary_workgroup(monkeypatch):
     with pytest.raises(ValueError, match="current GPU"):
         call(2**16, 2**10, 2**15)()
     assert counted[0] * (2**10 + 1) * 2**15 < 2**31 - 256 <= (counted[0] + 1) * (2**10 + 1) * 2**15
+
+
+def test_plans_are_kept_and_start_over(monkeypatch):
+    """A key's plan is made once; after 4096 keys of an operator the table starts over, and an early key is planned again."""
+    made, check = [], K._window_check
+    monkeypatch.setattr(K, "_window_check", lambda *a: made.append(a[4]) or check(*a))
+    q = torch.empty(0, 4, 1, 64, dtype=BF)
+
+    def call(n):
+        kv = torch.empty(0, 2, n, 64, dtype=BF)
+        out, lse = K.window_attention(q, kv, kv, 0.1, n)
+        assert out.shape == q.shape and lse.shape == q.shape[:3]
+        return len(made)
+
+    assert [call(1), call(1), call(2), call(1), call(2)] == [1, 1, 2, 2, 2]
+    for n in range(3, 4097):
+        assert call(n) == n
+    assert call(1) == 4096 and call(4096) == 4096     # all of them still there
+    assert call(4097) == 4097                         # the table is full: this key starts a new one
+    assert call(4097) == 4097 and call(1) == 4098 and call(1) == 4098 and call(4096) == 4099
+    h = torch.empty(0, 8, dtype=BF)
+    K.add_rmsnorm_quant(h, h, torch.empty(8, dtype=BF))  # another operator's plans are its own
+    assert call(4097) == 4099
