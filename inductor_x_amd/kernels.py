@@ -12,7 +12,6 @@ in-tree store; a missing code object is compiled with hipcc on first use.
 from __future__ import annotations
 
 import functools
-import math
 import threading
 from typing import Optional
 
@@ -871,7 +870,8 @@ def fused_attention(
     _require(not causal or Sq == Sk, "a causal mask needs equal query and key lengths")
     _require(q.is_contiguous() and k.is_contiguous() and v.is_contiguous(), "q, k, v must be contiguous (BNSD)")
     _require(all(_aligned(t) for t in (q, k, v)), "q, k, v must be 16-byte aligned")
-    _require(scale > 0 and math.isfinite(scale), "scale must be positive and finite")
+    # the kernels work with scale and with -lse / scale in 32 bits
+    _require(1e-30 <= scale <= 1e30, "scale must be positive and finite, 1e-30 to 1e30")
     _require(B * N * max(Sq, Sk) * D < 2**31, "numel must fit int32 indexing")
     out = torch.empty_like(q)
     smax = torch.empty((B, N, Sq, 8), dtype=torch.float32, device=q.device)
@@ -1037,7 +1037,8 @@ def _window_operands(q, k, v, scale, window, sinks, what="k and v"):
         _require(t.stride(-1) == 1 and _aligned(t) and all(s % 8 == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1),
                  "columns must be contiguous, and rows 16-byte aligned")
     _require(_strides3(k)[2] < _STRIDE_LIMIT and _strides3(v)[2] < _STRIDE_LIMIT, "tokens lie too far apart")
-    _require(scale > 0 and math.isfinite(scale), "scale must be positive and finite")
+    # the kernels work with scale and with -lse / scale in 32 bits
+    _require(1e-30 <= scale <= 1e30, "scale must be positive and finite, 1e-30 to 1e30")
     _require(window >= 1 and sinks >= 0, "window must be at least 1 and sinks at least 0")
     return 64 if D <= 64 else 128, min(int(window), _WINDOW_LIMIT), min(int(sinks), _WINDOW_LIMIT)
 
@@ -1368,7 +1369,8 @@ def fused_attention_backward(
     _require(S % 64 == 0 and S > 0, "sequence length must be a positive multiple of 64")
     for t in (softmax_max, softmax_sum):
         _require(t.dtype == torch.float32 and t.shape == (B, N, S, 8) and t.is_contiguous(), "statistics must be contiguous fp32 [B, N, S, 8]")
-    _require(scale > 0 and math.isfinite(scale), "scale must be positive and finite")
+    # the kernels work with scale and with -lse / scale in 32 bits
+    _require(1e-30 <= scale <= 1e30, "scale must be positive and finite, 1e-30 to 1e30")
     _require(B * N * S * D < 2**31, "numel must fit int32 indexing")
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
     heads = B * N

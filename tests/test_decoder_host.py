@@ -400,3 +400,18 @@ def test_plans_are_kept_and_start_over(monkeypatch):
     h = torch.empty(0, 8, dtype=BF)
     K.add_rmsnorm_quant(h, h, torch.empty(8, dtype=BF))  # another operator's plans are its own
     assert call(4097) == 4099
+
+
+def test_scales_that_32_bits_do_not_hold():
+    """The kernels take the scale, and its inverse, in 32 bits."""
+    q, k, v = window_operands()
+    n, lse = torch.ones(2, dtype=torch.int32), torch.zeros(2, 4, 8)
+    for scale in (1e-46, 1e-39, 1e-31, 1e31, 1e39, 1e300):
+        for call in (lambda: K.window_attention(q, k, v, scale, 4), lambda: K.window_attention_backward(q, k, v, q, q, lse, scale, 4),
+                     lambda: K.window_attention_decode(q[:, :, 0].contiguous(), k, v, n, scale, 4),
+                     lambda: K.window_attention_with_gradients(q, k, v, scale, 4)):
+            with pytest.raises(ValueError, match="scale"):
+                call()
+    for scale in (1e-30, 1e30):
+        with pytest.raises(Launched):
+            K.window_attention(q, k, v, scale, 4)
