@@ -1017,3 +1017,47 @@ def test_decode_of_wide_scores(K, B, N, Nk, capacity, D, window, sinks, lengths,
     for b, n in enumerate(lengths):
         want, bound = R.wide_attention(*(t[b : b + 1] for t in (q, k[:, :, :n], v[:, :, :n])), scale, window, sinks, None, dout[b : b + 1], dtype)
         within(got[b : b + 1], want["out"][:, :, 0], bound["out"][:, :, 0], "decode")
+
+
+def test_graphs_are_released():
+    announce("a forward pass whose gradient is never asked for keeps nothing")
+    from inductor_x_amd import decoder
+
+    q, k, v, dout = (t.to(DEV) for t in window_operands(2, 8, 2, 600, 600, 128, BF, False, seed=29))
+    at, freq = torch.arange(8, dtype=torch.int32, device=DEV).view(1, 8).expand(2, 8).contiguous(), torch.ones(64, device=DEV)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    held = []
+    for i in range(6):
+        out = decoder.window_attention(*leaves, 0.1, 100, 4)
+        turned = decoder.rotary_axes(leaves[0][:, :, :8].transpose(1, 2), leaves[1][:, :, :8].transpose(1, 2), at, freq)
+        if i % 3 == 0:
+            out.backward(dout)
+        del out, turned
+        for t in leaves:
+            t.grad = None
+        torch.cuda.synchronize()
+        held.append(torch.cuda.memory_allocated())
+    assert len(set(held[1:])) == 1, held
+
+
+@pytest.mark.parametrize("source", ["k", "v", "q", "dout"])
+def test_hidden_pairs_in_narrow_heads(K, source):
+    announce(f"NaN in rows of {source}: heads of 80 columns beside tokens, repeated calls, other sequences of the batch")
+    B, N, Nk, S, D, window, sinks = 3, 4, 2, 300, 80, 60, 3
+    t = dict(zip(("q", "k", "v", "dout"), window_operands(B, N, Nk, S, S, D, BF, True, seed=30)))
+    lengths = [300, 300, 177]
+    want = R.attention(t["q"], t["k"], t["v"], 0.1, window, sinks, lengths, t["dout"])
+    t[source][1] = float("nan")  # a whole sequence
+    d = {x: same_memory(y) for x, y in t.items()}
+    ln = device_lengths(lengths)
+    first = None
+    for _ in range(2):
+        out, lse, low = K.window_attention(d["q"], d["k"], d["v"], 0.1, window, sinks, ln, True)
+        got = (out, *K.window_attention_backward(d["q"], d["k"], d["v"], out, d["dout"], lse, 0.1, window, sinks, ln, low))
+        for name, x in zip(("out", "dq", "dk", "dv"), got):
+            bound = R.attention_bound(want[name], want["weight" if name == "out" else name + "_weight"], BF)
+            within(x[::2], want[name][::2], bound[::2], name)
+            lost = {"out": source != "dout", "dq": True, "dk": True, "dv": source != "v"}[name]
+            assert torch.isnan(x[1]).all() if lost else torch.isfinite(x[1]).all(), name
+        assert first is None or all(torch.equal(a.nan_to_num(), b.nan_to_num()) for a, b in zip(first, got))
+        first = got
