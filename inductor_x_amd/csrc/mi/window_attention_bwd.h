@@ -36,8 +36,8 @@
 //        kernel leaves the two maxima of each 32 rows behind the row statistics.
 //   dQ   per row, from max |dO| alone, which becomes 2^7 to 2^8: that takes |dP - D| of up to 2^8 max |dO|, and a
 //        row with more becomes infinite, which starts the workgroup over (win_any_lost) with the bound from max |V|.
-// bf16 has the exponents of fp32 and no such factors.  Backward pass of [4,32/8,4096,128] window 1024 in fp16: 1094 us, 1061
-// without them (bf16 1022); of [3,8/8,777,96] window 256 58 and 54.
+// bf16 has the exponents of fp32 and no such factors.  Backward pass of [4,32/8,4096,128] window 1024 in fp16: 1093 us, 1061
+// without them (bf16 1022); of [3,8/8,777,96] window 256 56 and 54.
 #pragma once
 
 #include "window_attention.h"
@@ -142,8 +142,9 @@ __device__ __forceinline__ void window_bwd_dq(const WindowBwdArgs& a) {
 #pragma unroll
     for (int d = 0; d < DS; ++d)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) largest = win_largest(largest, static_cast<float>(dof[d][e]));
+      for (int e = 0; e < 8; ++e) largest = fmaxf(largest, __builtin_fabsf(static_cast<float>(dof[d][e])));
     largest = exists ? win_half_max(largest) : 0.f;
+    if (!win_is_number(largest)) largest = 0.f;  // a row that is lost
   }
   int shift = kWinScaled<T> ? win_shift(largest, 8) : 0;
   float m2s = m2;  // with the shift
@@ -371,7 +372,7 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
 #pragma unroll
     for (int i = 0; i < DS; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum += win_largest(0.f, static_cast<float>(kf[i][e]));
+      for (int e = 0; e < 8; ++e) sum += __builtin_fabsf(static_cast<float>(kf[i][e]));  // no number: a key that is lost
     return __builtin_ldexpf(1.f, win_shift(fmaf(largest, win_half_sum(sum), d), 15) - kWinPShift);
   };
   const float c2 = s.scale2;
@@ -442,6 +443,14 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
           sp[n / DS] = E::mfma(qa[n], kf[n % DS], sp[n / DS]);
           __builtin_amdgcn_sched_barrier(0);
         });
+        if constexpr (FOR_DK && kWinScaled<T>) {  // here, where this wavefront waits for P
+#pragma unroll
+          for (int qb = 0; qb < 2; ++qb) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sp[qb][r] *= factor;
+            asm volatile("" : "+v"(sp[qb]));
+          }
+        }
         if constexpr (!FOR_DK) {
           if (!(p0 >= kw + 31 && (p0 + kWinTile - 1 < kw + s.window || kw + 32 <= sinks))) {
 #pragma unroll
@@ -479,10 +488,7 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
             for (int rq = 0; rq < 4; ++rq) {
               const Vec<float, 4> v = load_vec<float, 4>(handed + 256 * (4 * qb + rq));
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float x = v[e] * sp[qb][4 * rq + e];
-                bf[2 * qb + (rq >> 1)][4 * (rq & 1) + e] = static_cast<T>(kWinScaled<T> ? x * factor : x);
-              }
+              for (int e = 0; e < 4; ++e) bf[2 * qb + (rq >> 1)][4 * (rq & 1) + e] = static_cast<T>(v[e] * sp[qb][4 * rq + e]);
             }
         }
         // acc += (dO or Q)^T (P or dS)
@@ -620,7 +626,7 @@ __device__ __forceinline__ void window_bwd_sinks(const WindowBwdArgs& a) {
 #pragma unroll
     for (int i = 0; i < DS; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum += win_largest(0.f, static_cast<float>(vf[i][e]));
+      for (int e = 0; e < 8; ++e) sum += __builtin_fabsf(static_cast<float>(vf[i][e]));
     factor = __builtin_ldexpf(1.f, win_shift(fmaf(largest, win_half_sum(sum), d), 15) - kWinPShift);
   }
   f32x16_t dk[DB], dv[DB];
