@@ -1,6 +1,7 @@
 // Instantiations of the gradients of attention with a sliding window and visible first tokens (window_attention_bwd.h).
-// As in the forward, two workgroups of four wavefronts per CU: 1219 against 1264 us with eight at [4,32/8,4096,128],
-// window 1024.
+// dQ: as in the forward, two workgroups of four wavefronts per CU, 1219 against 1264 us for the backward pass with eight at
+// [4,32/8,4096,128], window 1024.  dK and dV: one workgroup of eight wavefronts per CU, whose 99 KB of LDS (128 columns) leave
+// no room for another; the bound of two wavefronts per SIMD is those eight.
 #include "../mi/window_attention_bwd.h"
 
 using namespace mi;

@@ -13,11 +13,13 @@
 // No mask exists in memory: a wavefront compares positions in the few tiles that are neither wholly visible nor
 // wholly hidden to it.
 //
-// Measured on MI355X (bf16, 32 query heads on 8 key heads, 128 columns): 4096 queries at the end of 32768 keys, window
-// 8192, 128 first keys: 541 us, 1032 TFLOP/s over the visible pairs, 89 % of what a large library product reaches
-// (1165); 8192 queries, window 1024: 163 us, 795 TFLOP/s.  The matrix pipe is busy 51 % and 42 % of the cycles: beside it
-// run 6 (8) vector instructions per product, and every product reads one operand from LDS.  In short windows a block's
-// first loads and last stores are the rest, which the second workgroup of the CU covers in part.  A two-phase software
+// Measured on MI355X (bf16, 32 query heads on 8 key heads, 128 columns; several cards): 4096 queries at the end of 32768
+// keys, window 8192, 128 first keys: 532 to 552 us, 1012 to 1050 TFLOP/s over the visible pairs, 87 to 90 % of what a large
+// library product reaches (1165); 8192 queries, window 1024: 162 to 166 us, 780 to 800 TFLOP/s.  The matrix pipe is busy 52 %
+// and 42 % of the cycles: beside it run 6 (8) vector instructions per product, and every product reads one operand from
+// LDS.  A block of 18 tiles takes about 37 us at the long rows' pace and 42 as it is: its first loads and last stores, which the
+// second workgroup of the CU covers in part.  Blocks are not split over their keys: few blocks of long rows leave CUs idle, and
+// their time is one block's chain, 50 us for [1,8/1,2048,128] causal (floor 7).  A two-phase software
 // pipeline like attention_v5.h's was 4 % faster in rows of thousands of keys and 25 % slower in windows of 256.
 //
 // Operand layouts and the transposed products are those of attention.h.  Tiles travel memory -> LDS by direct

@@ -16,10 +16,10 @@
 //               makes S and P and adds to dV; it hands P to the other through LDS, in fp32, lane to lane (both hold the
 //               same rows and keys), which has made dP meanwhile and adds to dK.  Neither holds more than one
 //               gradient's sums and one operand, each product is made once and each tile is copied once; two
-//               separate kernels (five products, two copies of each tile) took 670 us where this takes 567 us
-//               ([4,32/8,4096,128], window 1024: 850 TFLOP/s over the four products).
+//               separate kernels (five products, two copies of each tile) took 670 us where this took 567 us on the same card
+//               ([4,32/8,4096,128], window 1024; 565 to 572 us on average in later traces, 840 TFLOP/s over the four products).
 //               Where there are few blocks of keys several workgroups share a walk (the host's rule); their sums go to
-//               fp32 slots and the join kernel adds those in order and rounds once: [1,8/1,2048,128] causal 104 us for
+//               fp32 slots and the join kernel adds those in order and rounds once: [1,8/1,2048,128] causal 106 us for
 //               the whole backward pass with 16 shares, 485 without.
 //   first keys  the keys j < sinks are also seen by every query beyond their window, hundreds of tiles for a few keys
 //               in a long text.  There that part is a kernel of its own: a workgroup takes 32 such keys and a share of
