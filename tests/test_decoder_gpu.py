@@ -1061,3 +1061,32 @@ def test_hidden_pairs_in_narrow_heads(K, source):
             assert torch.isnan(x[1]).all() if lost else torch.isfinite(x[1]).all(), name
         assert first is None or all(torch.equal(a.nan_to_num(), b.nan_to_num()) for a, b in zip(first, got))
         first = got
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_replays_see_what_is_no_number(K, dtype):
+    announce(f"a captured forward and backward pass replayed with NaN, infinities and numbers again {dtype}")
+    gen = torch.Generator().manual_seed(31)
+    q, k, v, dout = (t.to(DEV) for t in window_operands(2, 4, 2, 400, 400, 128, dtype, False, seed=31))
+    lengths = torch.tensor([400, 290], dtype=torch.int32, device=DEV)
+    call = lambda: training_call(K, q, k, v, dout, 64, 4, lengths)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = call()
+    for step in range(5):
+        for t in (q, k, v, dout):
+            t.copy_(torch.randn(t.shape, generator=gen).to(dtype))
+        if step == 1:
+            k[0, 1, 130], v[1, 0, 77, 5], dout[0, 2, 300, 8] = float("nan"), float("inf"), float("-inf")
+        if step == 2:
+            v *= 2000
+        if step == 3:
+            dout *= 1e-4
+        graph.replay()
+        torch.cuda.synchronize()
+        want = call()
+        lost = [x.isnan().sum().item() for x in want]
+        assert all(torch.equal(a.nan_to_num(), b.nan_to_num()) and torch.equal(a.isnan(), b.isnan()) for a, b in zip(held, want)), f"replay {step}"
+        assert (max(lost) > 0) == (step == 1), (step, lost)
