@@ -415,3 +415,15 @@ def test_scales_that_32_bits_do_not_hold():
     for scale in (1e-30, 1e30):
         with pytest.raises(Launched):
             K.window_attention(q, k, v, scale, 4)
+
+
+def test_other_operators_keep_their_scales(monkeypatch):
+    monkeypatch.setattr(K, "_find", lambda l, symbol: (_ for _ in ()).throw(Launched(symbol)))
+    monkeypatch.setattr(K.codecache, "aot_source", lambda name: "")
+    q = torch.zeros(1, 1, 64, 128, dtype=BF)
+    for scale in (1e-31, 1e31):
+        with pytest.raises(Exception) as e:
+            K.fused_attention(q, q, q, scale, False)
+        assert "scale" not in str(e.value)
+    with pytest.raises(ValueError, match="scale must be positive and finite$"):
+        K.fused_attention(q, q, q, -1.0, False)
