@@ -280,6 +280,15 @@ __device__ __forceinline__ void win_clear(T* tile, int elements, int thread) {
     if (clear) *reinterpret_cast<x8_t*>(tile + c) = f;
   }
 }
+// The same for the fragments of a row
+template <typename T, int DS>
+__device__ __forceinline__ void win_clear_row(typename AttnElem<T>::x8 (&f)[DS]) {
+#pragma unroll
+  for (int i = 0; i < DS; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (!win_is_number(static_cast<float>(f[i][e]))) f[i][e] = static_cast<T>(0.f);
+}
 // Whether row `row` of a tile holds something else than numbers
 template <typename T, int DH>
 __device__ __forceinline__ bool win_bad_row(const T* tile, int row) {

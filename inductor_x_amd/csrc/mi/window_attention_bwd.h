@@ -560,6 +560,7 @@ __device__ __forceinline__ void window_bwd_dkv(const WindowBwdArgs& a) {
     win_zero(acc);
     next_h = first_h;
     next_t = first_t;
+    if (for_dk) win_clear_row<T>(kf);  // whoever sees such a value has no D
   }
   // the sums without their factor, a power of two
   const float unscale = !kWinScaled<T> ? 1.f : for_dk ? __builtin_ldexpf(1.f, -kWinPShift) / factor : 1.f / factor;
@@ -709,6 +710,7 @@ __device__ __forceinline__ void window_bwd_sinks(const WindowBwdArgs& a) {
     if (!(win_lost(dk, li < keys) | win_lost(dv, li < keys))) break;
     win_zero(dk);
     win_zero(dv);
+    win_clear_row<T>(vf);  // whoever sees such a value has no D
   }
   const float unscale_v = kWinScaled<T> ? __builtin_ldexpf(1.f, -kWinPShift) : 1.f, unscale_k = kWinScaled<T> ? unscale_v / factor : 1.f;
   // the four wavefronts' sums meet in LDS, [wave][dK, dV][key][DH]

@@ -1040,6 +1040,20 @@ def test_graphs_are_released():
     assert len(set(held[1:])) == 1, held
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("case", [
+    (1, 6, 3, 63, 149, 128, 2, 55, None, [141, 64]),
+    (1, 2, 1, 130, 500, 64, 30, 4, None, [200]),
+    (1, 8, 1, 300, 1600, 128, 1000, 0, None, [100, 299]),    # shared by workgroups
+    (1, 2, 1, 900, 1200, 64, 100, 150, None, [199, 160]),    # first keys with a kernel of their own
+    (2, 2, 1, 90, 90, 64, 20, 2, [0, 50], [10, 70]),         # a sequence without a position, a row that does not exist
+], ids=str)
+@pytest.mark.parametrize("source", ["k", "v"])
+def test_rows_that_nobody_sees(K, case, source, dtype):
+    """Their gradients are zero, whatever they hold."""
+    test_hidden_pairs_do_not_count(K, case, source, dtype)
+
+
 @pytest.mark.parametrize("source", ["k", "v", "q", "dout"])
 def test_hidden_pairs_in_narrow_heads(K, source):
     announce(f"NaN in rows of {source}: heads of 80 columns beside tokens, repeated calls, other sequences of the batch")
